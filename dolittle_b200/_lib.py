@@ -55,6 +55,25 @@ class ServeStats(C.Structure):
                 ("kernels_per_decode_step", C.c_uint64)]
 
 
+class SharedAttention(C.Structure):
+    _fields_ = [("batch", C.c_size_t), ("rows", C.c_size_t), ("query_heads", C.c_size_t), ("kv_heads", C.c_size_t),
+                ("width", C.c_size_t), ("query_stride", C.c_size_t), ("output_stride", C.c_size_t),
+                ("prefix_key", C.c_void_p), ("prefix_value", C.c_void_p), ("prefix_capacity", C.c_size_t),
+                ("prefix_row_stride", C.c_size_t), ("prefix_lengths", C.c_void_p), ("suffix_key", C.c_void_p),
+                ("suffix_value", C.c_void_p), ("suffix_capacity", C.c_size_t), ("suffix_row_stride", C.c_size_t),
+                ("suffix_sequence_stride", C.c_size_t), ("suffix_lengths", C.c_void_p)]
+
+
+class CacheEviction(C.Structure):
+    _fields_ = [("caches", C.c_size_t), ("kv_heads", C.c_size_t), ("width", C.c_size_t), ("capacity", C.c_size_t),
+                ("budget", C.c_size_t), ("first", C.c_size_t), ("recent", C.c_size_t), ("key", C.c_void_p),
+                ("value", C.c_void_p), ("row_stride", C.c_size_t), ("cache_stride", C.c_size_t),
+                ("weights", C.c_void_p), ("positions", C.c_void_p), ("lengths", C.c_void_p),
+                ("key_out", C.c_void_p), ("value_out", C.c_void_p), ("out_capacity", C.c_size_t),
+                ("out_row_stride", C.c_size_t), ("out_cache_stride", C.c_size_t), ("weights_out", C.c_void_p),
+                ("positions_out", C.c_void_p), ("lengths_out", C.c_void_p)]
+
+
 _lib = None
 
 vp, sz, u32p, u16p = C.c_void_p, C.c_size_t, C.POINTER(C.c_uint32), C.POINTER(C.c_uint16)
@@ -145,6 +164,10 @@ SIGNATURES = {
     "dl_gemm_bf16_parts": (C.c_int, [vp, sz, vp, vp, sz, sz, sz, sz, C.c_int, sz, vp, vp]),
     "dl_attention_decode_batched_workspace_bytes": (sz, [sz, sz, sz, sz]),
     "dl_attention_decode_batched_plan": (C.c_int, [sz, sz, sz, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
+    "dl_attention_shared_workspace_bytes": (sz, [C.POINTER(SharedAttention), C.c_int]),
+    "dl_attention_shared": (C.c_int, [C.POINTER(SharedAttention), vp, vp, vp, vp, vp, vp, vp]),
+    "dl_cache_evict_workspace_bytes": (sz, [C.POINTER(CacheEviction)]),
+    "dl_cache_evict": (C.c_int, [C.POINTER(CacheEviction), vp, vp]),
     "dl_attention_decode_batched": (C.c_int, [vp, vp, sz, sz, sz, vp, sz, sz, sz, sz, vp, vp, vp]),
 }
 

@@ -12,6 +12,7 @@
 
 #include "../../include/dolittle_b200.h"
 #include "attention_prefill_tc.h"
+#include "cache_evict.h"
 #include "engine.h"
 #include "gemm_tcgen05.h"
 #include "gemv.cuh"
@@ -19,6 +20,7 @@
 #include "sampler.h"
 #include "serve.h"
 #include "serve_kernels.h"
+#include "shared_attention.h"
 #include "steering.h"
 
 namespace {
@@ -800,6 +802,175 @@ DL_API dl_status dl_attention_decode_batched(const void* query, const void* kv, 
                                                          static_cast<float*>(workspace),
                                                          static_cast<bf16*>(output), st(stream)),
                      "attention decode batched");
+}
+
+}  // extern "C"
+
+namespace {
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+int device_sms() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+// The kernels' view of a call, or the reason why there is none.
+dl_status shared_args(const dl_shared_attention* a, dl::SharedAttnArgs* o) {
+  if (!a) return fail(DL_INVALID_ARGUMENT, "attention shared: null arguments");
+  if (!a->batch || !a->rows || !a->query_heads || !a->kv_heads)
+    return fail(DL_INVALID_ARGUMENT, "attention shared: empty shape");
+  if (a->width != 64 && a->width != 128) return fail(DL_UNSUPPORTED, "attention shared: head width 64 or 128");
+  if (a->query_heads % a->kv_heads || a->query_heads / a->kv_heads > 64)
+    return fail(DL_UNSUPPORTED, "attention shared: query heads a multiple of KV heads, group <= 64");
+  const size_t most = size_t(1) << 30;
+  if (a->batch > 65535 || a->kv_heads > 65535 || a->query_heads > 65535 || a->rows > most ||
+      a->batch * a->rows > most / a->query_heads || a->prefix_capacity > most || a->suffix_capacity > most)
+    return fail(DL_UNSUPPORTED, "attention shared: size out of range");
+  const size_t q_width = a->query_heads * a->width, kv_width = a->kv_heads * a->width;
+  const size_t ldq = a->query_stride ? a->query_stride : q_width, ldo = a->output_stride ? a->output_stride : q_width;
+  if (ldq % 8 || ldo % 8 || ldq < q_width || ldo < q_width)
+    return fail(DL_UNSUPPORTED, "attention shared: query and output strides multiples of 8, at least a token's heads");
+  if (a->prefix_capacity) {
+    if (!a->prefix_key || !a->prefix_value || !a->prefix_lengths)
+      return fail(DL_INVALID_ARGUMENT, "attention shared: null prefix pointer");
+    if (a->prefix_row_stride % 8 || a->prefix_row_stride < kv_width || misaligned(a->prefix_key) ||
+        misaligned(a->prefix_value))
+      return fail(DL_UNSUPPORTED, "attention shared: prefix rows 16-byte aligned, stride at least a position's heads");
+  }
+  if (a->suffix_capacity) {
+    if (!a->suffix_key || !a->suffix_value || !a->suffix_lengths)
+      return fail(DL_INVALID_ARGUMENT, "attention shared: null suffix pointer");
+    if ((a->suffix_row_stride | a->suffix_sequence_stride) % 8 || a->suffix_row_stride < kv_width ||
+        misaligned(a->suffix_key) || misaligned(a->suffix_value))
+      return fail(DL_UNSUPPORTED, "attention shared: suffix rows 16-byte aligned, stride at least a position's heads");
+  }
+  o->batch = int(a->batch);
+  o->rows = int(a->rows);
+  o->query_heads = int(a->query_heads);
+  o->kv_heads = int(a->kv_heads);
+  o->width = int(a->width);
+  o->group = int(a->query_heads / a->kv_heads);
+  o->ldq = ldq;
+  o->ldo = ldo;
+  o->pk = static_cast<const bf16*>(a->prefix_key);
+  o->pv = static_cast<const bf16*>(a->prefix_value);
+  o->pcap = int(a->prefix_capacity);
+  o->p_row = a->prefix_row_stride;
+  o->plens = reinterpret_cast<const long long*>(a->prefix_lengths);
+  o->sk = static_cast<const bf16*>(a->suffix_key);
+  o->sv = static_cast<const bf16*>(a->suffix_value);
+  o->scap = int(a->suffix_capacity);
+  o->s_row = a->suffix_row_stride;
+  o->s_seq = a->suffix_sequence_stride;
+  o->slens = reinterpret_cast<const long long*>(a->suffix_lengths);
+  return DL_OK;
+}
+
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
+dl_status evict_args(const dl_cache_eviction* e, dl::EvictArgs* o) {
+  if (!e) return fail(DL_INVALID_ARGUMENT, "cache evict: null arguments");
+  if (!e->caches || !e->kv_heads || !e->width || !e->capacity || !e->budget)
+    return fail(DL_INVALID_ARGUMENT, "cache evict: empty shape");
+  if (e->first > e->budget || e->recent > e->budget - e->first)
+    return fail(DL_INVALID_ARGUMENT, "cache evict: first + recent must not exceed the budget");
+  const size_t budget = e->budget < e->capacity ? e->budget : e->capacity;
+  if (e->out_capacity < budget) return fail(DL_INVALID_ARGUMENT, "cache evict: output capacity below the budget");
+  if (e->width % 8 || (e->row_stride | e->cache_stride | e->out_row_stride | e->out_cache_stride) % 8)
+    return fail(DL_UNSUPPORTED, "cache evict: width and strides must be multiples of 8");
+  const size_t most = size_t(1) << 30;
+  if (e->width > 1024 || e->caches > most / e->kv_heads || e->capacity > most || e->out_capacity > most ||
+      e->caches * e->kv_heads > most / (budget * e->width / 4096 + 1))
+    return fail(DL_UNSUPPORTED, "cache evict: size out of range");
+  if (e->row_stride < e->kv_heads * e->width || e->out_row_stride < e->kv_heads * e->width)
+    return fail(DL_UNSUPPORTED, "cache evict: row stride below a position's heads");
+  o->caches = int(e->caches);
+  o->kv_heads = int(e->kv_heads);
+  o->width = int(e->width);
+  o->capacity = int(e->capacity);
+  o->out_capacity = int(e->out_capacity);
+  o->budget = int(budget);
+  o->first = int(e->first < most ? e->first : most);
+  o->recent = int(e->recent < most ? e->recent : most);
+  o->key = static_cast<const bf16*>(e->key);
+  o->value = static_cast<const bf16*>(e->value);
+  o->row_stride = e->row_stride;
+  o->cache_stride = e->cache_stride;
+  o->weights = e->weights;
+  o->positions = e->positions;
+  o->lengths = reinterpret_cast<const long long*>(e->lengths);
+  o->key_out = static_cast<bf16*>(e->key_out);
+  o->value_out = static_cast<bf16*>(e->value_out);
+  o->out_row_stride = e->out_row_stride;
+  o->out_cache_stride = e->out_cache_stride;
+  o->weights_out = e->weights_out;
+  o->positions_out = e->positions_out;
+  o->lengths_out = reinterpret_cast<long long*>(e->lengths_out);
+  return DL_OK;
+}
+}  // namespace
+
+extern "C" {
+
+DL_API size_t dl_attention_shared_workspace_bytes(const dl_shared_attention* a, int weights) {
+  dl::SharedAttnArgs o = {};
+  if (shared_args(a, &o) != DL_OK) return 0;
+  return dl::shared_attention_workspace_bytes(o, weights != 0, device_sms());
+}
+
+DL_API dl_status dl_attention_shared(const dl_shared_attention* a, const void* query, void* output, float* lse,
+                                     float* prefix_weights, float* suffix_weights, void* workspace, void* stream) {
+  dl::SharedAttnArgs o = {};
+  const dl_status s = shared_args(a, &o);
+  if (s != DL_OK) return s;
+  if (!query || !output || !workspace) return fail(DL_INVALID_ARGUMENT, "attention shared: null pointer");
+  if (misaligned(query) || misaligned(output) || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(DL_UNSUPPORTED, "attention shared: query and output 16-byte, workspace 256-byte aligned");
+  o.q = static_cast<const bf16*>(query);
+  o.out = static_cast<bf16*>(output);
+  o.lse = lse;
+  o.pw = o.pcap ? prefix_weights : nullptr;
+  o.sw = o.scap ? suffix_weights : nullptr;
+  return cuda_status(dl::launch_shared_attention(o, workspace, device_sms(), st(stream)), "attention shared");
+}
+
+DL_API size_t dl_cache_evict_workspace_bytes(const dl_cache_eviction* e) {
+  dl::EvictArgs o = {};
+  if (evict_args(e, &o) != DL_OK) return 0;
+  return dl::cache_evict_workspace_bytes(o.caches, o.kv_heads, o.budget);
+}
+
+DL_API dl_status dl_cache_evict(const dl_cache_eviction* e, void* workspace, void* stream) {
+  dl::EvictArgs o = {};
+  const dl_status s = evict_args(e, &o);
+  if (s != DL_OK) return s;
+  if (!e->key || !e->value || !e->weights || !e->positions || !e->lengths || !e->key_out || !e->value_out ||
+      !e->weights_out || !e->positions_out || !e->lengths_out || !workspace)
+    return fail(DL_INVALID_ARGUMENT, "cache evict: null pointer");
+  if (misaligned(e->key) || misaligned(e->value) || misaligned(e->key_out) || misaligned(e->value_out) ||
+      misaligned(workspace))
+    return fail(DL_UNSUPPORTED, "cache evict: caches and workspace 16-byte aligned");
+  o.in_place = e->key_out == e->key && e->value_out == e->value && e->weights_out == e->weights &&
+               e->positions_out == e->positions;
+  if (o.in_place) {
+    if (e->out_capacity != e->capacity || e->out_row_stride != e->row_stride || e->out_cache_stride != e->cache_stride)
+      return fail(DL_INVALID_ARGUMENT, "cache evict: in place needs the input's strides and capacity");
+  } else {
+    const size_t row = e->kv_heads * e->width;
+    const size_t in = 2 * ((e->caches - 1) * e->cache_stride + (e->capacity - 1) * e->row_stride + row);
+    const size_t out = 2 * ((e->caches - 1) * e->out_cache_stride + (size_t(o.budget) - 1) * e->out_row_stride + row);
+    const size_t in4 = 4 * e->caches * e->kv_heads * e->capacity, out4 = 4 * e->caches * e->kv_heads * e->out_capacity;
+    if (overlap(e->key_out, out, e->key, in) || overlap(e->key_out, out, e->value, in) ||
+        overlap(e->value_out, out, e->key, in) || overlap(e->value_out, out, e->value, in) ||
+        overlap(e->weights_out, out4, e->weights, in4) || overlap(e->positions_out, out4, e->positions, in4))
+      return fail(DL_INVALID_ARGUMENT, "cache evict: outputs overlap the inputs without being them");
+  }
+  return cuda_status(dl::launch_cache_evict(o, workspace, st(stream)), "cache evict");
 }
 
 }  // extern "C"

@@ -462,6 +462,88 @@ DL_API dl_status dl_attention_decode_batched(const void* query, const void* kv, 
                                              void* output, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Shared-prefix serving.  A batch of sequences that continue one prompt:    */
+/* the prompt's keys and values are held and read once for the whole batch,  */
+/* each sequence keeps only its own.  No counterpart in the reference, which */
+/* runs every continuation through a plan and a cache of its own             */
+/* (src/experiment/run.cpp:871-929).  BF16 storage, FP32 statistics.         */
+/* ------------------------------------------------------------------------ */
+/* Shapes, caches and lengths of one call.  Strides count elements; element
+ * (position, KV head, feature) of a cache lies at position * row_stride +
+ * head * width + feature, so a block of an engine's cache is a prefix as it
+ * stands.  Lengths are int64 in device memory, one per sequence, read on the
+ * device (a captured graph follows them) and clamped to [0, capacity].
+ * Sequence b attends prefix keys j < prefix_lengths[b] (sequences may leave
+ * the prompt at different tokens) and its own suffix; its `rows` newest
+ * suffix positions are the query rows, so row i sees suffix keys
+ * j < suffix_lengths[b] - (rows - 1 - i).  A side with capacity 0 is absent
+ * and its pointers are not read. */
+typedef struct {
+  size_t batch, rows, query_heads, kv_heads, width;
+  size_t query_stride, output_stride; /* between tokens; 0 = query_heads * width */
+  const void* prefix_key;             /* [prefix_capacity][kv_heads][width] */
+  const void* prefix_value;
+  size_t prefix_capacity, prefix_row_stride;
+  const int64_t* prefix_lengths;      /* device [batch] */
+  const void* suffix_key;             /* [batch][suffix_capacity][kv_heads][width] */
+  const void* suffix_value;
+  size_t suffix_capacity, suffix_row_stride, suffix_sequence_stride;
+  const int64_t* suffix_lengths;      /* device [batch] */
+} dl_shared_attention;
+/* query [batch][rows][query_heads][width] -> output alike (strides above)
+ * and, when lse is not NULL, the natural log of each row's softmax
+ * denominator, FP32 [batch][rows][query_heads].  scale = 1 / sqrt(width).  A
+ * row without keys gives zeros and -infinity.  prefix_weights FP32
+ * [kv_heads][prefix_capacity] and suffix_weights FP32
+ * [batch][kv_heads][suffix_capacity], either NULL or added to: the softmax
+ * weight each key received from every row, and query head of its group (and
+ * from every sequence, for prefix keys), in this call.  width 64 or 128,
+ * query_heads a multiple of kv_heads with a ratio up to 64, pointers 16-byte
+ * aligned, strides multiples of 8.  Rows of a cache at or past every length
+ * may hold anything (NaN too); a key some row attends must be finite.  Same
+ * inputs, same bits: no sum depends on the order in which blocks run.
+ * workspace: dl_attention_shared_workspace_bytes() bytes, 256-byte aligned,
+ * any contents; not shared by calls that may overlap on the device. */
+DL_API size_t dl_attention_shared_workspace_bytes(const dl_shared_attention* a, int weights);
+DL_API dl_status dl_attention_shared(const dl_shared_attention* a, const void* query, void* output, float* lse,
+                                     float* prefix_weights, float* suffix_weights, void* workspace, void* stream);
+/* Eviction from caches by accumulated weight.  Each (cache, KV head) keeps
+ * min(length, budget) of its slots: first the protected ones (position below
+ * `first`, or among the `recent` newest positions: above the head's largest
+ * position - recent), then by weight, largest first (NaN last), ties to the
+ * lowest slot.  Kept slots below that count stay where they are; the kept
+ * slots from there on move, in ascending order, into the vacated ones, so an
+ * eviction of few slots moves few rows.  Keys carry their rotary position, so
+ * attention does not depend on the order of slots; `positions` says which
+ * token each holds.  first + recent <= budget.
+ * key/value: element (cache, slot, head, feature) at cache * cache_stride +
+ * slot * row_stride + head * width + feature, likewise *_out; weights and
+ * positions [caches][kv_heads][capacity], their outputs
+ * [caches][kv_heads][out_capacity].  The outputs are either all the inputs
+ * themselves (same pointers, strides and capacity: eviction in place, only
+ * moved rows are touched) or buffers that overlap none of them; slots from
+ * min(length, budget) on are not written.  lengths_out may be lengths.
+ * width a multiple of 8, pointers 16-byte aligned, strides multiples of 8.
+ * workspace: dl_cache_evict_workspace_bytes() bytes, any contents. */
+typedef struct {
+  size_t caches, kv_heads, width, capacity, budget, first, recent;
+  const void* key;
+  const void* value;
+  size_t row_stride, cache_stride;
+  const float* weights;
+  const int32_t* positions;
+  const int64_t* lengths; /* device [caches], clamped to [0, capacity] */
+  void* key_out;
+  void* value_out;
+  size_t out_capacity, out_row_stride, out_cache_stride; /* out_capacity >= min(budget, capacity) */
+  float* weights_out;
+  int32_t* positions_out;
+  int64_t* lengths_out;
+} dl_cache_eviction;
+DL_API size_t dl_cache_evict_workspace_bytes(const dl_cache_eviction* e);
+DL_API dl_status dl_cache_evict(const dl_cache_eviction* e, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Device-side generation loop (DeviceSequence, src/inference/decoding/     */
 /* device.h:84-139): dl_engine_start enqueues the prompt pass, the first    */
 /* selection and ONE graph launch whose conditional WHILE node replays the  */
