@@ -1,0 +1,236 @@
+// What the kernels of the shared-prefix attention have in common: row and
+// length arithmetic, the workspace, tensor-core and copy primitives.
+#pragma once
+
+#include <atomic>
+#include <cmath>
+
+#include "shared_attention.h"
+#include "tcgen05.cuh"
+#include "tensor_map.h"
+
+namespace dl {
+namespace sa {
+
+constexpr int kRows = 128;   // query rows of a tile = TMEM lanes
+constexpr int kKeys = 128;   // keys of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// A query row's softmax in the base-2 domain: weight = exp2(s * scale - m) * r.
+// A row without keys has m = 0, r = 0.
+struct RowNorm {
+  float m, r;
+};
+
+// Workspace: FP32 partial outputs of key ranges, one 128-row tile per (range,
+// tile) stored row by row with 16-byte pieces permuted (piece c of row r lies
+// at c ^ (r & 7)), their running maximum (base 2) and sum, the rows' norms
+// [tokens][Hq] and, for the weights, the suffix scores of the few-row kernel.
+struct Workspace {
+  float* part_o;    // [splits][tiles][128][D]
+  float2* part_ml;  // [splits][tiles][128]
+  RowNorm* norm;    // [tokens * Hq]
+  float* scores;    // [B][Hq * rows][scap]
+};
+
+// How a call is cut into work, from sizes alone.
+struct Plan {
+  bool pooled;    // row tiles hold tokens of several sequences and cover the prefix; the few-row kernel adds the suffixes
+  int per_tile;   // tokens of a row tile: 128 / group
+  int tiles;      // row tiles of a unit
+  int units;      // KV heads (pooled) or sequences x KV heads
+  bool wide;      // two row tiles per CTA share its key tiles; otherwise one row tile, key tiles in two interleaved streams
+  int splits;     // key ranges of a row tile (0: no tile kernel)
+  int suffix_splits;  // CTAs (one cluster) per sequence and KV head in the few-row kernel
+  int weight_ranks;   // CTAs (one cluster) per key tile in the weights kernel
+};
+
+cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+
+// Launch configuration of a programmatic dependent launch (every kernel here
+// waits for its predecessor before it touches global memory).
+struct DependentLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  DependentLaunch(dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster = 1) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = cluster;
+      attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+  }
+};
+
+// Dynamic shared memory above 48 KB, allowed once per kernel and device.
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};  // devices 0 .. 63
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// Tiles of [rows][64 features], one KV head: `per_tile` tokens x the head
+// group, and 128 positions of a cache.
+inline bool encode_query_map(CUtensorMap* m, const SharedAttnArgs& a, int per_tile) {
+  const uint64_t dims[3] = {uint64_t(a.width), uint64_t(a.query_heads), uint64_t(a.batch) * a.rows};
+  const uint64_t strides[2] = {uint64_t(a.width), a.ldq};
+  const uint32_t box[3] = {64, uint32_t(a.group), uint32_t(per_tile)};
+  return encode_bf16_map(m, a.q, 3, dims, strides, box);
+}
+inline bool encode_prefix_map(CUtensorMap* m, const SharedAttnArgs& a, const bf16* base) {
+  const uint64_t dims[3] = {uint64_t(a.width), uint64_t(a.kv_heads), uint64_t(a.pcap)};
+  const uint64_t strides[2] = {uint64_t(a.width), a.p_row};
+  const uint32_t box[3] = {64, 1, kKeys};
+  return encode_bf16_map(m, base, 3, dims, strides, box);
+}
+inline bool encode_suffix_map(CUtensorMap* m, const SharedAttnArgs& a, const bf16* base) {
+  const uint64_t dims[4] = {uint64_t(a.width), uint64_t(a.kv_heads), uint64_t(a.scap), uint64_t(a.batch)};
+  const uint64_t strides[3] = {uint64_t(a.width), a.s_row, a.batch > 1 ? a.s_seq : a.s_row * a.scap};
+  const uint32_t box[4] = {64, 1, kKeys, 1};
+  return encode_bf16_map(m, base, 4, dims, strides, box);
+}
+
+__device__ __forceinline__ int clamp_len(long long n, int cap) { return int(n < 0 ? 0 : n > cap ? cap : n); }
+__device__ __forceinline__ int prefix_len(const SharedAttnArgs& a, int b) {
+  return a.pcap ? clamp_len(a.plens[b], a.pcap) : 0;
+}
+__device__ __forceinline__ int suffix_len(const SharedAttnArgs& a, int b) {
+  return a.scap ? clamp_len(a.slens[b], a.scap) : 0;
+}
+// Suffix keys that row i sees of a suffix of n keys.
+__device__ __forceinline__ int suffix_seen(int n, int rows, int i) { return max(0, n - (rows - 1 - i)); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two softmax weights as BF16 pairs hi + lo: hi the upper halves, lo the exact
+// rest rounded, so hi + lo is good to 2^-16 and the second product, run with
+// both, keeps the accuracy of FP32 weights.  (One BF16 rounding alone, 2^-8,
+// would cost as much as the rounding of the output itself.)
+__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  hi = __byte_perm(x, y, 0x7632);
+  lo = pack_bf16(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
+}
+
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+      "%5}], [%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// MN-major operand with 128-byte swizzle (64 contiguous elements of M or N per
+// 128-byte row, one row per K): leading offset between 64-element columns,
+// 1024 bytes between groups of 8 K.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t addr, uint32_t column_bytes) {
+  return tc::smem_desc_sw128(addr) & ~(uint64_t(0x3FFF) << 16) | (uint64_t(column_bytes >> 4) << 16);
+}
+
+// D (TMEM) += A (TMEM, BF16 pairs) * B (shared memory).
+__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 columns of this warp's lanes, not yet waited for.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for the loads issued so far; the values in r are only valid after it.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Wait of one role of a warp-specialised kernel: bounded (~2 s), and over at
+// once when another role already gave up.  *failed is shared memory.
+__device__ __forceinline__ bool role_wait(uint64_t* bar, unsigned parity, volatile int* failed) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (!*failed) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - start > (1ll << 32)) break;
+  }
+  *failed = 1;
+  return false;
+}
+
+// The same for a whole warp: one answer for all lanes, which stay together.
+__device__ __forceinline__ bool role_wait_warp(uint64_t* bar, unsigned parity, volatile int* failed) {
+  return __all_sync(0xffffffffu, role_wait(bar, parity, failed));
+}
+
+}  // namespace sa
+}  // namespace dl

@@ -1,4 +1,5 @@
-// Attention of a batch that shares a prefix (shared_attention.cu).
+// Attention of a batch that shares a prefix (shared_attention.cu and the
+// kernels it plans: shared_tile.cu, shared_rows.cu, shared_weights.cu).
 #pragma once
 
 #include "launch.h"

@@ -1,0 +1,548 @@
+// Tensor-core kernel of the shared-prefix attention: 128-row tiles of query
+// rows against 128-key tiles, online softmax, on tcgen05.
+//
+// The rows of a tile are tokens x the query heads of one KV head.  Pooled
+// tiles take the tokens of several sequences (a decode step's batch), so the
+// prefix is read once for all of them; otherwise a tile's tokens belong to one
+// sequence and its key tiles run through the prefix and on into that
+// sequence's suffix.  Roles of a CTA: one warp loads tiles by TMA into a ring,
+// one issues the products, and two groups of four warps ("streams") own the
+// softmax of a 128 x 128 score tile each, one thread per row.  Wide CTAs give
+// the streams two row tiles that share the key tiles; with a single row tile
+// the streams take alternate key tiles and are joined at the end.  While one
+// stream is in its softmax the tensor core works for the other:
+//
+//   S[x] = Q K^T       (both operands in shared memory, K-major)
+//   P[x] = exp2(S * scale - m), two BF16 halves written over S[x] in TMEM
+//   O[x] += (Phi + Plo)[x] V   (P from TMEM, V as it lies in the cache: the
+//                       MN-major form of the operand needs no transposed copy)
+//
+// S[x] of the next key tile is issued behind O[x] += P[x] V: products run in
+// issue order, so it cannot overwrite P[x] early, and when S[x] is ready O[x]
+// is too.  The row's reference m only moves when its maximum has grown by more
+// than 2^8, then the thread rescales its row of O in TMEM; sums stay FP32 far
+// from overflow.  The tensor core wants P in the type of V: P is split in two
+// BF16 numbers, half again as many products, for FP32's accuracy.
+#include "shared_attention.cuh"
+
+namespace dl {
+namespace sa {
+namespace {
+
+using namespace tc;
+
+constexpr int kThreads = 320;  // 8 softmax warps, TMA warp, MMA warp
+constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kAtom = kRows * 128;  // [128 rows][64 BF16]
+constexpr uint32_t kTmemCols = 512;  // S0, S1, O0, O1
+constexpr float kRescale = 8.f;     // base-2 growth of the maximum that moves the reference
+
+template <int D, bool WIDE>
+struct Shape {
+  static constexpr int slot = D / 64 * kAtom;  // a K, V or Q tile
+  static constexpr int stages = D == 64 ? 8 : WIDE ? 5 : 4;
+  static constexpr int smem = (WIDE ? 2 : 1) * slot + stages * slot + 1024;
+};
+
+struct alignas(64) TileArgs {
+  CUtensorMap q, pk, pv, sk, sv;
+  SharedAttnArgs a;
+  Plan plan;
+  Workspace ws;
+  float scale_log2;
+  bool norms;  // write the rows' norms (the weights follow)
+};
+
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t tmem_s, uint32_t q_tile, uint32_t k_tile) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint32_t atom = uint32_t(kk >> 2) * kAtom;
+    const uint64_t off = uint64_t((kk & 3) * 2);
+    mma_bf16(tmem_s, smem_desc_sw128(q_tile + atom) + off, smem_desc_sw128(k_tile + atom) + off,
+             instr_desc_bf16(kRows, kKeys), kk ? 1u : 0u);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_tile, bool accumulate) {
+  constexpr uint32_t idesc = instr_desc_bf16(kRows, D) | (1u << 16);  // B is MN-major
+#pragma unroll
+  for (int kk = 0; kk < kKeys / 16; ++kk) {
+    const uint64_t v = smem_desc_sw128_mn(v_tile + uint32_t(kk * 2048), kAtom);
+    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kk * 8), v, idesc, (accumulate || kk) ? 1u : 0u);
+    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kKeys / 2 + kk * 8), v, idesc, 1u);
+  }
+}
+
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_constant__ TileArgs t) {
+  using S = Shape<D, WIDE>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int most[2];  // keys of the prefix / suffix that any row sees
+  __shared__ int failed_s;
+  __shared__ float2 other[kRows];  // second stream's (m, l)
+  volatile int* failed = &failed_s;
+  const SharedAttnArgs& a = t.a;
+  const Plan& pl = t.plan;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring = base + (WIDE ? 2 : 1) * S::slot;
+  float* stage = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Work of this CTA: row tiles fastest, so CTAs side by side read the same keys.
+  const int per_cta = WIDE ? 2 : 1, groups = (pl.tiles + per_cta - 1) / per_cta;
+  int at = blockIdx.x;
+  const int tile0 = at % groups * per_cta;
+  at /= groups;
+  const int split = at % pl.splits;
+  at /= pl.splits;
+  const int h = at % a.kv_heads, seq = at / a.kv_heads;  // seq = 0 when pooled
+  const int unit_tokens = pl.pooled ? a.batch * a.rows : a.rows;
+  const int streams = WIDE && tile0 + 1 >= pl.tiles ? 1 : 2;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < S::stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], kRows);
+      mbar_init(&o_full[x], 1);
+    }
+    mbar_init(&drained, 1);
+    most[0] = most[1] = 0;
+    failed_s = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemCols);
+  wait_prior();
+  allow_next();  // after the wait: the next kernel may read what this one's inputs are before it waits itself
+  __syncthreads();
+
+  // Rows of the softmax threads.
+  const int x = (warp >> 2) & 1, r = threadIdx.x & (kRows - 1);
+  const int tile = WIDE ? tile0 + x : tile0;
+  const int local = tile * pl.per_tile + r / a.group;  // token within the unit
+  const bool live = warp < kTmaWarp && r / a.group < pl.per_tile && local < unit_tokens && tile < pl.tiles;
+  const int token = pl.pooled ? local : seq * a.rows + local;
+  const int seen_p = live ? prefix_len(a, token / a.rows) : 0;
+  const int seen_s = live && !pl.pooled ? suffix_seen(suffix_len(a, seq), a.rows, local) : 0;
+  if (warp < kTmaWarp) {
+    const int p = __reduce_max_sync(0xffffffffu, seen_p), s = __reduce_max_sync(0xffffffffu, seen_s);
+    if (lane == 0) {
+      atomicMax(&most[0], p);
+      atomicMax(&most[1], s);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int np = (most[0] + kKeys - 1) / kKeys, nt = np + (most[1] + kKeys - 1) / kKeys;
+  const int k0 = int((long long)nt * split / pl.splits), n = int((long long)nt * (split + 1) / pl.splits) - k0;
+  // Key tiles of stream s, and the i-th one's place among the n.
+  auto count = [&](int s) { return WIDE ? (s < streams ? n : 0) : (n + 1 - s) / 2; };
+  auto nth = [&](int s, int i) { return WIDE ? i : 2 * i + s; };
+  const int steps = count(0);  // count(1) is at most that
+
+  if (warp == kTmaWarp) {
+    if (lane == 0 && n > 0) {
+      const int boxes = D / 64, q_bytes = pl.per_tile * a.group * 128 * boxes;
+      unsigned c = 0;
+      auto load = [&](int i, bool value) {
+        const int s = c % S::stages;
+        if (c >= S::stages && !role_wait(&empty[s], (c / S::stages + 1) & 1, failed)) return false;
+        mbar_arrive_expect_tx(&full[s], unsigned(S::slot));
+        unsigned char* dst = smem_raw + (ring + s * S::slot - smem_addr(smem_raw));
+        const int g = k0 + i;
+        for (int b = 0; b < boxes; ++b) {
+          if (g < np) tma_3d(dst + b * kAtom, value ? &t.pv : &t.pk, 64 * b, h, g * kKeys, &full[s]);
+          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, seq, &full[s]);
+        }
+        ++c;
+        return true;
+      };
+      mbar_arrive_expect_tx(&q_full, unsigned(q_bytes * (WIDE ? streams : 1)));
+      for (int s = 0; s < (WIDE ? streams : 1); ++s)
+        for (int b = 0; b < boxes; ++b)
+          tma_3d(smem_raw + (base + s * S::slot + b * kAtom - smem_addr(smem_raw)), &t.q, 64 * b, h * a.group,
+                 (pl.pooled ? 0 : seq * a.rows) + (tile0 + s) * pl.per_tile, &q_full);
+      // The order in which the products use them.
+      const int feeds = WIDE ? 1 : 2;
+      bool ok = true;
+      for (int s = 0; s < feeds && ok; ++s)
+        if (count(s) > 0) ok = load(nth(s, 0), false);
+      for (int i = 0; i < steps && ok; ++i)
+        for (int s = 0; s < feeds && ok; ++s) {
+          if (i < count(s)) ok = load(nth(s, i), true);
+          if (ok && i + 1 < count(s)) ok = load(nth(s, i + 1), false);
+        }
+      if (!ok) {  // gave up: the copies in flight still land in this CTA's memory
+        mbar_wait(&q_full, 0);
+        for (unsigned j = c > S::stages ? c - S::stages : 0; j < c; ++j)
+          mbar_wait(&full[j % S::stages], (j / S::stages) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    unsigned c = 0;  // ring position
+    bool ok = n == 0 || role_wait_warp(&q_full, 0, failed);
+    auto slot_addr = [&](unsigned p) { return ring + p % S::stages * S::slot; };
+    auto wait_full = [&](unsigned p) {
+      const bool got = role_wait_warp(&full[p % S::stages], (p / S::stages) & 1, failed);
+      fence_after_sync();
+      return got;
+    };
+    auto scores = [&](int s, unsigned p) {
+      if (lane == 0) {
+        mma_scores<D>(tmem + s * kKeys, base + (WIDE ? s : 0) * S::slot, slot_addr(p));
+        mma_commit(&s_full[s]);
+      }
+    };
+    auto release = [&](unsigned p) {
+      if (lane == 0) mma_commit(&empty[p % S::stages]);
+    };
+    // Rows past every length hold anything: as values times a weight of zero
+    // they would still count, so they become zeros.
+    auto clear_tail = [&](unsigned p, int i) {
+      const int g = k0 + i, left = g < np ? most[0] - g * kKeys : most[1] - (g - np) * kKeys;
+      if (left >= kKeys) return;
+      unsigned char* v = smem_raw + (slot_addr(p) - smem_addr(smem_raw));
+      for (int b = 0; b < D / 64; ++b)
+        for (int o = left * 128 + lane * 16; o < kAtom; o += 512)
+          *reinterpret_cast<uint4*>(v + b * kAtom + o) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    auto output = [&](int s, unsigned p, int i) {
+      const bool got = role_wait_warp(&p_full[s], i & 1, failed);
+      fence_after_sync();
+      if (got && lane == 0) mma_output<D>(tmem + 256 + s * 128, tmem + s * kKeys, slot_addr(p), i > 0);
+      return got;
+    };
+    if constexpr (WIDE) {
+      if (ok && n > 0) {
+        ok = wait_full(0);
+        for (int s = 0; s < streams && ok; ++s) scores(s, 0);
+        if (ok) release(0);
+        c = 1;
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const unsigned pv = c++, pk = c;
+        ok = wait_full(pv);
+        if (!ok) break;
+        clear_tail(pv, i);
+        for (int s = 0; s < streams && ok; ++s) {
+          ok = output(s, pv, i);
+          if (ok && s == streams - 1) release(pv);
+          if (!ok) break;
+          if (i + 1 < n) {
+            if (s == 0) ok = wait_full(pk);
+            if (!ok) break;
+            scores(s, pk);
+            if (s == streams - 1) release(pk);
+          } else if (lane == 0) {
+            mma_commit(&o_full[s]);
+          }
+        }
+        if (i + 1 < n) ++c;
+      }
+    } else {
+      for (int s = 0; s < 2 && ok; ++s)
+        if (count(s) > 0) {
+          ok = wait_full(c);
+          if (ok) scores(s, c);
+          if (ok) release(c);
+          ++c;
+        }
+      for (int i = 0; i < steps && ok; ++i)
+        for (int s = 0; s < 2 && ok; ++s) {
+          if (i >= count(s)) continue;
+          ok = wait_full(c);
+          if (!ok) break;
+          clear_tail(c, nth(s, i));
+          ok = output(s, c, i);
+          if (!ok) break;
+          release(c++);
+          if (i + 1 < count(s)) {
+            ok = wait_full(c);
+            if (!ok) break;
+            scores(s, c);
+            release(c++);
+          } else if (lane == 0) {
+            mma_commit(&o_full[s]);
+          }
+        }
+    }
+    if (!ok) {  // products in flight read shared memory and write TMEM
+      if (lane == 0) mma_commit(&drained);
+      mbar_wait(&drained, 0);
+    }
+  } else {
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + x * kKeys, t_o = tmem + lanes + 256 + x * 128;
+    const int mine = count(x);
+    const float c = t.scale_log2;
+    float m = -INFINITY, l = 0.f;  // m: unscaled reference of the row
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const int g = k0 + nth(x, i);
+      const int lim = g < np ? seen_p - g * kKeys : seen_s - (g - np) * kKeys;  // keys of the tile this row sees
+      ok = role_wait_warp(&s_full[x], i & 1, failed);
+      if (!ok) break;
+      fence_after_sync();
+      uint32_t s[kKeys];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tmem_ld32_async(t_s + 32 * j, s + 32 * j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tmem_ld_wait32(s + 32 * j);
+      if (__any_sync(0xffffffffu, lim < kKeys)) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+          if (j >= lim) s[j] = 0xff800000u;  // -infinity
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool grow = (top - m) * c > kRescale;  // also from -infinity
+      if (i == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, grow)) {
+        const float alpha = grow ? exp2_approx((m - top) * c) : 1.f;
+#pragma unroll 1
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32_async(t_o + 32 * j, o);
+          tmem_ld_wait32(o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+          tmem_st32(t_o + 32 * j, o);
+        }
+        l *= alpha;
+        if (grow) m = top;
+      }
+      const float shift = m == -INFINITY ? 0.f : -m * c;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float e0 = exp2_approx(fmaf(__uint_as_float(s[32 * j + 2 * k]), c, shift));
+          const float e1 = exp2_approx(fmaf(__uint_as_float(s[32 * j + 2 * k + 1]), c, shift));
+          sum[(2 * k) & 3] += e0;
+          sum[(2 * k + 1) & 3] += e1;
+          split_bf16(e0, e1, hi[k], lo[k]);
+        }
+        tmem_st16(t_s + 16 * j, hi);
+        tmem_st16(t_s + kKeys / 2 + 16 * j, lo);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      fence_before_sync();
+      mbar_arrive(&p_full[x]);
+    }
+    // Both streams' products must be over before the ring becomes scratch.
+    for (int s = 0; s < 2; ++s)
+      if (count(s) > 0) ok = role_wait_warp(&o_full[s], 0, failed) && ok;
+    fence_after_sync();
+    float m2 = m == -INFINITY ? -INFINITY : m * c, mine_f = 1.f, other_f = 0.f;
+    auto piece = [&](int i, int row) { return stage + (WIDE ? x * kRows * D : 0) + row * D + ((i ^ (row & 7)) << 2); };
+    if constexpr (!WIDE) {
+      if (x == 1) {
+        other[r] = make_float2(m2, l);
+        if (mine > 0 && ok) {
+#pragma unroll 1
+          for (int j = 0; j < D / 32; ++j) {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_ld32_async(t_o + 32 * j, o);
+            tmem_ld_wait32(o);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<uint4*>(piece(8 * j + k, r)) =
+                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        }
+      }
+      named_sync(1, 2 * kRows);
+      if (x == 0 && count(1) > 0) {
+        const float2 ml = other[r];
+        const float top = fmaxf(m2, ml.x);
+        mine_f = m2 == -INFINITY ? 0.f : exp2_approx(m2 - top);
+        other_f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+        l = l * mine_f + ml.y * other_f;
+        m2 = top;
+      }
+    }
+    ok = ok && !*failed;
+    if (!ok) l = NAN;
+    if (WIDE || x == 0) {
+      const bool has = mine > 0 && ok;
+      if (!pl.pooled && pl.splits == 1) {  // the whole softmax of the row
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+        const int hq = h * a.group + r % a.group;
+        bf16* out = a.out + size_t(token) * a.ldo + size_t(hq) * D;
+#pragma unroll 1
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32_async(t_o + 32 * j, o);
+          tmem_ld_wait32(o);
+          if (!live) continue;
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = has ? __uint_as_float(o[4 * k + u]) * mine_f : 0.f;
+            if (!WIDE && other_f != 0.f) {
+              const float4 y = *reinterpret_cast<const float4*>(piece(8 * j + k, r));
+              const float4 z = *reinterpret_cast<const float4*>(piece(8 * j + k + 1, r));
+              const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+              for (int u = 0; u < 8; ++u) v[u] = fmaf(w[u], other_f, v[u]);
+            }
+            reinterpret_cast<uint4*>(out)[4 * j + k / 2] =
+                make_uint4(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv),
+                           pack_bf16(v[4] * inv, v[5] * inv), pack_bf16(v[6] * inv, v[7] * inv));
+          }
+        }
+        if (live) {
+          const size_t row = size_t(token) * a.query_heads + hq;
+          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * kLn2;
+          if (t.norms) t.ws.norm[row] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{m2, inv};
+        }
+      } else if (tile < pl.tiles) {
+        const size_t part = (size_t(split) * pl.units + seq * a.kv_heads + h) * pl.tiles + tile;
+        t.ws.part_ml[part * kRows + r] = make_float2(m2, l);
+#pragma unroll 1
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32_async(t_o + 32 * j, o);
+          tmem_ld_wait32(o);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = has ? __uint_as_float(o[4 * k + u]) * mine_f : 0.f;
+            if (!WIDE && other_f != 0.f) {
+              const float4 y = *reinterpret_cast<const float4*>(piece(8 * j + k, r));
+              v[0] = fmaf(y.x, other_f, v[0]);
+              v[1] = fmaf(y.y, other_f, v[1]);
+              v[2] = fmaf(y.z, other_f, v[2]);
+              v[3] = fmaf(y.w, other_f, v[3]);
+            }
+            *reinterpret_cast<float4*>(piece(8 * j + k, r)) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        named_sync(2 + x, kRows);
+        if (r == 0) {
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(t.ws.part_o +
+                                                                                            part * kRows * D),
+                       "r"(smem_addr(stage + (WIDE ? x * kRows * D : 0))), "r"(kRows * D * 4)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+        }
+      }
+    }
+    fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the key ranges of each (token, query head): one warp per row, the
+// ranges in order.
+template <int D>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws,
+                                                           bool norms) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  wait_prior();
+  allow_next();
+  if (row >= a.batch * a.rows * a.query_heads) return;
+  const int token = row / a.query_heads, hq = row % a.query_heads, h = hq / a.group, g = hq % a.group;
+  const int seq = pl.pooled ? 0 : token / a.rows, local = pl.pooled ? token : token % a.rows;
+  const int r = local % pl.per_tile * a.group + g;
+  const size_t first = size_t(seq * a.kv_heads + h) * pl.tiles + local / pl.per_tile;
+  const size_t stride = size_t(pl.units) * pl.tiles;
+  float top = -INFINITY;
+  for (int s = 0; s < pl.splits; ++s) top = fmaxf(top, ws.part_ml[(first + s * stride) * kRows + r].x);
+  constexpr int F = D / 32;  // consecutive features of a lane
+  const int where = ((lane * F / 4) ^ (r & 7)) * 4 + lane * F % 4;
+  float l = 0.f, o[F] = {};
+  for (int s = 0; s < pl.splits; ++s) {
+    const size_t part = (first + s * stride) * kRows + r;
+    const float2 ml = ws.part_ml[part];
+    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+    l = fmaf(ml.y, f, l);
+    if (f == 0.f) continue;
+    const float* src = ws.part_o + part * D + where;
+    float v[F];
+    if constexpr (F == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(src);
+      v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(src);
+      v[0] = y.x, v[1] = y.y;
+    }
+#pragma unroll
+    for (int c = 0; c < F; ++c) o[c] = fmaf(v[c], f, o[c]);
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.out + size_t(token) * a.ldo + size_t(hq) * D + lane * F);
+#pragma unroll
+  for (int c = 0; c < F; c += 2) out[c / 2] = pack_bf16(o[c] * inv, o[c + 1] * inv);
+  if (lane == 0) {
+    if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    if (norms) ws.norm[row] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{top, inv};
+  }
+}
+
+template <int D, bool WIDE>
+cudaError_t launch_tiles_shape(const TileArgs& t, cudaStream_t stream) {
+  using S = Shape<D, WIDE>;
+  cudaError_t e = allow_smem<shared_tile_kernel<D, WIDE>>(S::smem);
+  if (e != cudaSuccess) return e;
+  const int per_cta = WIDE ? 2 : 1;
+  const unsigned grid = unsigned((t.plan.tiles + per_cta - 1) / per_cta) * t.plan.splits * t.plan.units;
+  DependentLaunch d(dim3(grid), kThreads, S::smem, stream);
+  return cudaLaunchKernelEx(&d.cfg, shared_tile_kernel<D, WIDE>, t);
+}
+
+}  // namespace
+
+cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+  TileArgs t = {};
+  t.a = a;
+  t.plan = p;
+  t.ws = ws;
+  t.scale_log2 = attention_scale(a.width) * kLog2e;
+  t.norms = a.pw || a.sw;
+  if (!encode_query_map(&t.q, a, p.per_tile)) return cudaErrorInvalidValue;
+  if (a.pcap && !(encode_prefix_map(&t.pk, a, a.pk) && encode_prefix_map(&t.pv, a, a.pv))) return cudaErrorInvalidValue;
+  if (a.scap && !p.pooled && !(encode_suffix_map(&t.sk, a, a.sk) && encode_suffix_map(&t.sv, a, a.sv)))
+    return cudaErrorInvalidValue;
+  if (a.width == 64) return p.wide ? launch_tiles_shape<64, true>(t, stream) : launch_tiles_shape<64, false>(t, stream);
+  return p.wide ? launch_tiles_shape<128, true>(t, stream) : launch_tiles_shape<128, false>(t, stream);
+}
+
+cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+  const int rows = a.batch * a.rows * a.query_heads;
+  DependentLaunch d(dim3((rows + 7) / 8), 256, 0, stream);
+  const bool norms = a.pw || a.sw;
+  return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<64>, a, p, ws, norms)
+                       : cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<128>, a, p, ws, norms);
+}
+
+}  // namespace sa
+}  // namespace dl
