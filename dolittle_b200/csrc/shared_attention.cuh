@@ -130,15 +130,63 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Two softmax weights as BF16 pairs hi + lo: hi the upper halves, lo the exact
-// rest rounded, so hi + lo is good to 2^-16 and the second product, run with
-// both, keeps the accuracy of FP32 weights.  (One BF16 rounding alone, 2^-8,
-// would cost as much as the rounding of the output itself.)
-__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Pairs of FP32 numbers in one 64-bit register (one instruction for both).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Two softmax weights as BF16 pairs hi + lo: the upper halves of the numbers
+// and of what they leave, so hi + lo is good to 2^-14 (the dropped rest is
+// below 2^-7 of lo, lo below 2^-7 of the weight) and the second product, run
+// with both, keeps the accuracy of FP32 weights.  One BF16 rounding alone,
+// 2^-8, would cost as much as the rounding of the output itself.  Byte
+// permutes instead of conversions, which share the exponential's slow pipe.
+__device__ __forceinline__ void split_bf16(uint64_t ab, uint32_t& hi, uint32_t& lo) {
+  float a, b, ra, rb;
+  unpair(ab, a, b);
   const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
   hi = __byte_perm(x, y, 0x7632);
-  lo = pack_bf16(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
+  const uint64_t rest = add2(ab, pair(__uint_as_float((x & 0xffff0000u) ^ 0x80000000u),
+                                      __uint_as_float((y & 0xffff0000u) ^ 0x80000000u)));
+  unpair(rest, ra, rb);
+  lo = __byte_perm(__float_as_uint(ra), __float_as_uint(rb), 0x7632);
 }
+
+// True in one lane of a converged warp; the compiler then knows that a single
+// thread issues (a tensor instruction under `lane == 0` issues at half the rate).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Position in a ring of N buffers and the parity of the pass over it.
+template <int N>
+struct RingPos {
+  int slot = 0;
+  unsigned parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t hi, lo;
-        split_bf16(e[2 * u], e[2 * u + 1], hi, lo);
+        split_bf16(pair(e[2 * u], e[2 * u + 1]), hi, lo);
         p_hi[nb][u] = transpose8(hi);
         p_lo[nb][u] = transpose8(lo);
       }

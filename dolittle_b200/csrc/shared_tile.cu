@@ -31,8 +31,8 @@ namespace {
 
 using namespace tc;
 
-constexpr int kThreads = 320;  // 8 softmax warps, TMA warp, MMA warp
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 352;  // 8 softmax warps, one each for loads, products and clearing
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kClearWarp = 10;
 constexpr int kAtom = kRows * 128;  // [128 rows][64 BF16]
 constexpr uint32_t kTmemCols = 512;  // S0, S1, O0, O1
 constexpr float kRescale = 8.f;     // base-2 growth of the maximum that moves the reference
@@ -64,13 +64,16 @@ __device__ __forceinline__ void mma_scores(uint32_t tmem_s, uint32_t q_tile, uin
   }
 }
 
+// Half of the key tile's keys (kk of 8 steps of 16).
 template <int D>
-__device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_tile, bool accumulate) {
+__device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_tile, int half,
+                                           bool accumulate) {
   constexpr uint32_t idesc = instr_desc_bf16(kRows, D) | (1u << 16);  // B is MN-major
 #pragma unroll
-  for (int kk = 0; kk < kKeys / 16; ++kk) {
+  for (int i = 0; i < 4; ++i) {
+    const int kk = 4 * half + i;
     const uint64_t v = smem_desc_sw128_mn(v_tile + uint32_t(kk * 2048), kAtom);
-    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kk * 8), v, idesc, (accumulate || kk) ? 1u : 0u);
+    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kk * 8), v, idesc, (accumulate || i) ? 1u : 0u);
     mma_bf16_ts(tmem_o, tmem_p + uint32_t(kKeys / 2 + kk * 8), v, idesc, 1u);
   }
 }
@@ -79,7 +82,9 @@ template <int D, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_constant__ TileArgs t) {
   using S = Shape<D, WIDE>;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_half[2], p_full[2], o_full[2];
+  __shared__ uint64_t dirty, clean, drained;
+  __shared__ uint32_t dirty_from, dirty_to;  // bytes of a value tile's first 64 features to clear
   __shared__ uint32_t tmem_slot;
   __shared__ int most[2];  // keys of the prefix / suffix that any row sees
   __shared__ int failed_s;
@@ -111,9 +116,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], kRows);
+      mbar_init(&p_half[x], 4);
+      mbar_init(&p_full[x], 4);
       mbar_init(&o_full[x], 1);
     }
+    mbar_init(&dirty, 1);
+    mbar_init(&clean, 1);
     mbar_init(&drained, 1);
     most[0] = most[1] = 0;
     failed_s = 0;
@@ -150,20 +158,28 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
   auto nth = [&](int s, int i) { return WIDE ? i : 2 * i + s; };
   const int steps = count(0);  // count(1) is at most that
 
+  // Keys of the i-th tile that exist; a tile that holds fewer than 128 ends its side.
+  auto filled = [&](int i) {
+    const int g = k0 + i;
+    return g < np ? most[0] - g * kKeys : most[1] - (g - np) * kKeys;
+  };
+
   if (warp == kTmaWarp) {
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       const int boxes = D / 64, q_bytes = pl.per_tile * a.group * 128 * boxes;
+      RingPos<S::stages> at;
       unsigned c = 0;
       auto load = [&](int i, bool value) {
-        const int s = c % S::stages;
-        if (c >= S::stages && !role_wait(&empty[s], (c / S::stages + 1) & 1, failed)) return false;
-        mbar_arrive_expect_tx(&full[s], unsigned(S::slot));
-        unsigned char* dst = smem_raw + (ring + s * S::slot - smem_addr(smem_raw));
+        if (c >= S::stages && !role_wait(&empty[at.slot], at.parity ^ 1, failed)) return false;
+        uint64_t* bar = &full[at.slot];
+        mbar_arrive_expect_tx(bar, unsigned(S::slot));
+        unsigned char* dst = smem_raw + (ring + at.slot * S::slot - smem_addr(smem_raw));
         const int g = k0 + i;
         for (int b = 0; b < boxes; ++b) {
-          if (g < np) tma_3d(dst + b * kAtom, value ? &t.pv : &t.pk, 64 * b, h, g * kKeys, &full[s]);
-          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, seq, &full[s]);
+          if (g < np) tma_3d(dst + b * kAtom, value ? &t.pv : &t.pk, 64 * b, h, g * kKeys, bar);
+          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, seq, bar);
         }
+        at.next();
         ++c;
         return true;
       };
@@ -190,100 +206,115 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    unsigned c = 0;  // ring position
-    bool ok = n == 0 || role_wait_warp(&q_full, 0, failed);
-    auto slot_addr = [&](unsigned p) { return ring + p % S::stages * S::slot; };
-    auto wait_full = [&](unsigned p) {
-      const bool got = role_wait_warp(&full[p % S::stages], (p / S::stages) & 1, failed);
-      fence_after_sync();
-      return got;
-    };
-    auto scores = [&](int s, unsigned p) {
-      if (lane == 0) {
-        mma_scores<D>(tmem + s * kKeys, base + (WIDE ? s : 0) * S::slot, slot_addr(p));
+    if (n > 0 && elect_one()) {
+      RingPos<S::stages> at;
+      unsigned cleared = 0;
+      bool ok = role_wait(&q_full, 0, failed);
+      auto slot_addr = [&](int slot) { return ring + uint32_t(slot) * S::slot; };
+      auto wait_key = [&] {
+        ok = ok && role_wait(&full[at.slot], at.parity, failed);
+        fence_after_sync();
+      };
+      auto wait_value = [&](int i) {
+        ok = ok && role_wait(&full[at.slot], at.parity, failed);
+        const int left = filled(i);
+        if (ok && left < kKeys) {
+          dirty_from = slot_addr(at.slot) + uint32_t(left) * 128;
+          dirty_to = slot_addr(at.slot) + kAtom;
+          mbar_arrive(&dirty);
+          ok = role_wait(&clean, cleared++ & 1, failed);
+        }
+        fence_after_sync();
+      };
+      auto scores = [&](int s, int slot) {
+        mma_scores<D>(tmem + s * kKeys, base + (WIDE ? s : 0) * S::slot, slot_addr(slot));
         mma_commit(&s_full[s]);
+      };
+      auto output = [&](int s, int slot, int i) {
+        const uint32_t o = tmem + 256 + s * 128, p = tmem + s * kKeys, v = slot_addr(slot);
+        ok = role_wait(&p_half[s], i & 1, failed);
+        fence_after_sync();
+        if (!ok) return;
+        mma_output<D>(o, p, v, 0, i > 0);
+        ok = role_wait(&p_full[s], i & 1, failed);
+        fence_after_sync();
+        if (ok) mma_output<D>(o, p, v, 1, true);
+      };
+      if constexpr (WIDE) {
+        wait_key();
+        if (ok) {
+          for (int s = 0; s < streams; ++s) scores(s, at.slot);
+          mma_commit(&empty[at.slot]);
+          at.next();
+        }
+        for (int i = 0; i < n && ok; ++i) {
+          wait_value(i);
+          const int v = at.slot;
+          at.next();
+          for (int s = 0; s < streams && ok; ++s) {
+            output(s, v, i);
+            if (!ok) break;
+            if (s == streams - 1) mma_commit(&empty[v]);
+            if (i + 1 == n) {
+              mma_commit(&o_full[s]);
+              continue;
+            }
+            if (s == 0) wait_key();
+            if (!ok) break;
+            scores(s, at.slot);
+            if (s == streams - 1) mma_commit(&empty[at.slot]);
+          }
+          if (i + 1 < n) at.next();
+        }
+      } else {
+        for (int s = 0; s < 2; ++s) {
+          if (!ok || count(s) == 0) continue;
+          wait_key();
+          if (!ok) break;
+          scores(s, at.slot);
+          mma_commit(&empty[at.slot]);
+          at.next();
+        }
+        for (int i = 0; i < steps && ok; ++i)
+          for (int s = 0; s < 2 && ok; ++s) {
+            if (i >= count(s)) continue;
+            wait_value(nth(s, i));
+            if (ok) output(s, at.slot, i);
+            if (!ok) break;
+            mma_commit(&empty[at.slot]);
+            at.next();
+            if (i + 1 == count(s)) {
+              mma_commit(&o_full[s]);
+              continue;
+            }
+            wait_key();
+            if (!ok) break;
+            scores(s, at.slot);
+            mma_commit(&empty[at.slot]);
+            at.next();
+          }
       }
-    };
-    auto release = [&](unsigned p) {
-      if (lane == 0) mma_commit(&empty[p % S::stages]);
-    };
-    // Rows past every length hold anything: as values times a weight of zero
-    // they would still count, so they become zeros.
-    auto clear_tail = [&](unsigned p, int i) {
-      const int g = k0 + i, left = g < np ? most[0] - g * kKeys : most[1] - (g - np) * kKeys;
-      if (left >= kKeys) return;
-      unsigned char* v = smem_raw + (slot_addr(p) - smem_addr(smem_raw));
+      if (!ok) {  // products in flight read shared memory and write TMEM
+        mma_commit(&drained);
+        mbar_wait(&drained, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kClearWarp) {
+    // Value rows past every length hold anything: times a weight of zero they
+    // would still count, so the products wait until they are zeros.
+    unsigned events = 0;
+    for (int i = 0; i < n; ++i) events += filled(i) < kKeys;
+    for (unsigned e = 0; e < events; ++e) {
+      if (!role_wait_warp(&dirty, e & 1, failed)) break;
       for (int b = 0; b < D / 64; ++b)
-        for (int o = left * 128 + lane * 16; o < kAtom; o += 512)
-          *reinterpret_cast<uint4*>(v + b * kAtom + o) = make_uint4(0, 0, 0, 0);
+        for (uint32_t o = dirty_from + b * kAtom + lane * 16; o < dirty_to + b * kAtom; o += 512)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(o), "r"(0) : "memory");
       fence_proxy_async_smem();
       __syncwarp();
-    };
-    auto output = [&](int s, unsigned p, int i) {
-      const bool got = role_wait_warp(&p_full[s], i & 1, failed);
-      fence_after_sync();
-      if (got && lane == 0) mma_output<D>(tmem + 256 + s * 128, tmem + s * kKeys, slot_addr(p), i > 0);
-      return got;
-    };
-    if constexpr (WIDE) {
-      if (ok && n > 0) {
-        ok = wait_full(0);
-        for (int s = 0; s < streams && ok; ++s) scores(s, 0);
-        if (ok) release(0);
-        c = 1;
-      }
-      for (int i = 0; i < n && ok; ++i) {
-        const unsigned pv = c++, pk = c;
-        ok = wait_full(pv);
-        if (!ok) break;
-        clear_tail(pv, i);
-        for (int s = 0; s < streams && ok; ++s) {
-          ok = output(s, pv, i);
-          if (ok && s == streams - 1) release(pv);
-          if (!ok) break;
-          if (i + 1 < n) {
-            if (s == 0) ok = wait_full(pk);
-            if (!ok) break;
-            scores(s, pk);
-            if (s == streams - 1) release(pk);
-          } else if (lane == 0) {
-            mma_commit(&o_full[s]);
-          }
-        }
-        if (i + 1 < n) ++c;
-      }
-    } else {
-      for (int s = 0; s < 2 && ok; ++s)
-        if (count(s) > 0) {
-          ok = wait_full(c);
-          if (ok) scores(s, c);
-          if (ok) release(c);
-          ++c;
-        }
-      for (int i = 0; i < steps && ok; ++i)
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (i >= count(s)) continue;
-          ok = wait_full(c);
-          if (!ok) break;
-          clear_tail(c, nth(s, i));
-          ok = output(s, c, i);
-          if (!ok) break;
-          release(c++);
-          if (i + 1 < count(s)) {
-            ok = wait_full(c);
-            if (!ok) break;
-            scores(s, c);
-            release(c++);
-          } else if (lane == 0) {
-            mma_commit(&o_full[s]);
-          }
-        }
+      if (lane == 0) mbar_arrive(&clean);
     }
-    if (!ok) {  // products in flight read shared memory and write TMEM
-      if (lane == 0) mma_commit(&drained);
-      mbar_wait(&drained, 0);
-    }
-  } else {
+  } else if (warp < kTmaWarp) {
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + x * kKeys, t_o = tmem + lanes + 256 + x * 128;
     const int mine = count(x);
@@ -307,10 +338,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
         for (int j = 0; j < kKeys; ++j)
           if (j >= lim) s[j] = 0xff800000u;  // -infinity
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[8];
 #pragma unroll
-      for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      for (int j = 0; j < 8; ++j) mx[j] = fmaxf(__uint_as_float(s[j]), __uint_as_float(s[8 + j]));
+#pragma unroll
+      for (int j = 16; j < kKeys; j += 16)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[j + k]), __uint_as_float(s[j + 8 + k])));
+      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                              fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
       const bool grow = (top - m) * c > kRescale;  // also from -infinity
       if (i == 0) {
         m = top;
@@ -319,7 +356,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
 #pragma unroll 1
         for (int j = 0; j < D / 32; ++j) {
           uint32_t o[32];
-          __syncwarp();
           tmem_ld32_async(t_o + 32 * j, o);
           tmem_ld_wait32(o);
 #pragma unroll
@@ -330,25 +366,32 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
         if (grow) m = top;
       }
       const float shift = m == -INFINITY ? 0.f : -m * c;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
+      uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float e0 = exp2_approx(fmaf(__uint_as_float(s[32 * j + 2 * k]), c, shift));
-          const float e1 = exp2_approx(fmaf(__uint_as_float(s[32 * j + 2 * k + 1]), c, shift));
-          sum[(2 * k) & 3] += e0;
-          sum[(2 * k + 1) & 3] += e1;
-          split_bf16(e0, e1, hi[k], lo[k]);
+          float x0, x1;
+          unpair(fma2(pair(__uint_as_float(s[32 * j + 2 * k]), __uint_as_float(s[32 * j + 2 * k + 1])), c2, shift2),
+                 x0, x1);
+          const uint64_t e = pair(exp2_approx(x0), exp2_approx(x1));
+          sum[k & 3] = add2(sum[k & 3], e);
+          split_bf16(e, hi[k], lo[k]);
         }
         tmem_st16(t_s + 16 * j, hi);
         tmem_st16(t_s + kKeys / 2 + 16 * j, lo);
+        if (j & 1) {  // 64 keys are there: their products may begin
+          tmem_st_wait();
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(j == 1 ? &p_half[x] : &p_full[x]);
+        }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      fence_before_sync();
-      mbar_arrive(&p_full[x]);
+      float s0, s1;
+      unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+      l += s0 + s1;
     }
     // Both streams' products must be over before the ring becomes scratch.
     for (int s = 0; s < 2; ++s)

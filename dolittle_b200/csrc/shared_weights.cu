@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) shared_weights_kernel(const __grid_c
 
   float sum = 0.f;
   if (warp == 4) {
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       auto mem = [&](uint32_t off) { return smem_raw + (base + off - smem_addr(smem_raw)); };
       const unsigned q_bytes = unsigned(w.per_tile * a.group * 128 * (D / 64));
       auto load_q = [&](int i) {
