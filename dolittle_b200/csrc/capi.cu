@@ -3,6 +3,7 @@
 // src/kernels/cuda/common.cuh:57-65): unsupported dtypes and shapes are
 // rejected, never silently converted.  Exceptions become dl_status codes and
 // a thread-local message.
+#include <atomic>
 #include <climits>
 #include <cstring>
 #include <exception>
@@ -810,9 +811,12 @@ namespace {
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 int device_sms() {
+  static std::atomic<int> known[64];  // by device ordinal
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 

@@ -14,6 +14,9 @@ namespace sa {
 
 constexpr int kRows = 128;   // query rows of a tile = TMEM lanes
 constexpr int kKeys = 128;   // keys of a tile
+constexpr int kMaxSplits = 32;  // key ranges of a row tile
+constexpr int kMaxSuffixSplits = 8;
+constexpr int kFewRows = 32;    // rows of a unit (new tokens x group) that the few-row kernels take
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -24,12 +27,14 @@ struct RowNorm {
 };
 
 // Workspace: FP32 partial outputs of key ranges, one 128-row tile per (range,
-// tile) stored row by row with 16-byte pieces permuted (piece c of row r lies
-// at c ^ (r & 7)), their running maximum (base 2) and sum, the rows' norms
-// [tokens][Hq] and, for the weights, the suffix scores of the few-row kernel.
+// split task, row tile of it) in the layout of part_offset, their running
+// maximum (base 2) and sum, the rows' norms [tokens][Hq] and, for the weights,
+// the suffix scores of the few-row kernel.
 struct Workspace {
-  float* part_o;    // [splits][tiles][128][D]
-  float2* part_ml;  // [splits][tiles][128]
+  float* part_o;    // [splits][tasks - full][per_cta][128 x D]
+  float2* part_ml;  // [splits][tasks - full][per_cta][128]
+  float* suffix_o;    // [suffix splits][B][Hkv][rows x group][D]
+  float2* suffix_ml;  // [suffix splits][B][Hkv][rows x group]
   RowNorm* norm;    // [tokens * Hq]
   float* scores;    // [B][Hq * rows][scap]
 };
@@ -38,17 +43,20 @@ struct Workspace {
 struct Plan {
   bool pooled;    // row tiles hold tokens of several sequences and cover the prefix; the few-row kernel adds the suffixes
   int per_tile;   // tokens of a row tile: 128 / group
-  int tiles;      // row tiles of a unit
-  int units;      // KV heads (pooled) or sequences x KV heads
-  bool wide;      // two row tiles per CTA share its key tiles; otherwise one row tile, key tiles in two interleaved streams
-  int splits;     // key ranges of a row tile (0: no tile kernel)
-  int suffix_splits;  // CTAs (one cluster) per sequence and KV head in the few-row kernel
+  int tiles;      // row tiles of a unit: a KV head (pooled) or a sequence's KV head
+  int per_cta;    // 2: two row tiles share a CTA's key tiles; 1: one row tile, key tiles in two interleaved streams
+  int groups;     // CTA tasks of a unit: tiles / per_cta, rounded up
+  int tasks;      // groups x units
+  int full;       // tasks done whole, by the first CTAs; the rest are cut into key ranges
+  int splits;     // key ranges of the rest (0: no tile kernel; the few-row kernel reads the prefix too)
+  int suffix_splits;  // CTAs (a cluster if there is no tile kernel) per sequence and KV head in the few-row kernel
   int weight_ranks;   // CTAs (one cluster) per key tile in the weights kernel
 };
 
 cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 
 // Launch configuration of a programmatic dependent launch (every kernel here
@@ -74,7 +82,9 @@ struct DependentLaunch {
   }
 };
 
-// Dynamic shared memory above 48 KB, allowed once per kernel and device.
+// Dynamic shared memory above 48 KB, allowed once per kernel and device; with
+// the whole of the SM's memory as shared memory, or blocks of two kernels
+// would not fit side by side (the split follows the kernel that came first).
 template <auto Kernel>
 cudaError_t allow_smem(int bytes) {
   static std::atomic<uint64_t> done{0};  // devices 0 .. 63
@@ -84,6 +94,8 @@ cudaError_t allow_smem(int bytes) {
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
   e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
@@ -118,6 +130,15 @@ __device__ __forceinline__ int suffix_len(const SharedAttnArgs& a, int b) {
 }
 // Suffix keys that row i sees of a suffix of n keys.
 __device__ __forceinline__ int suffix_seen(int n, int rows, int i) { return max(0, n - (rows - 1 - i)); }
+
+// Feature f of row r within a partial tile: two halves of the features, row by
+// row, 16-byte piece c of a row's half at c ^ (r & 7) (so that neither the
+// staging of rows by threads nor the bulk copy meets bank conflicts).
+template <int D>
+__device__ __forceinline__ int part_offset(int r, int f) {
+  const int half = f / (D / 2), c = f % (D / 2) / 4;
+  return (half * kRows + r) * (D / 2) + ((c ^ (r & 7)) << 2) + (f & 3);
+}
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;

@@ -1,11 +1,15 @@
-// Few-row kernel of the shared-prefix attention: at most 32 query rows (the
-// new tokens of one sequence x the query heads of one KV head) against that
-// sequence's suffix, joined with the prefix ranges the tile kernel left.
+// Few-row kernels of the shared-prefix attention: at most 32 query rows (the
+// new tokens of one sequence x the query heads of one KV head).
 //
-// Bound by reading the suffix caches once, so the products run on the warp
-// tensor instructions, whose small fragments fit a few rows: a warp takes 16
-// keys at a time, with the keys as the 16-row operand of both products and the
-// query rows as the 8-wide one,
+// shared_rows_kernel streams that sequence's suffix beside the tile kernel's
+// prefix and leaves the part of each key range; shared_join_kernel joins the
+// prefix and suffix parts.  For small calls (SOLO) it streams prefix and suffix
+// both and ends the rows itself, one launch in all.
+//
+// Bound by reading the caches once, so the products run on the warp tensor
+// instructions, whose small fragments fit a few rows: a warp takes 16 keys at
+// a time, with the keys as the 16-row operand of both products and the query
+// rows as the 8-wide one,
 //
 //   S^T [16 keys x 8 rows] = K Q^T,   O^T [features x 8 rows] += V^T P^T,
 //
@@ -13,10 +17,11 @@
 // and V fragments are read once for all row blocks.  Warps do not meet until
 // the end: each streams its own keys through a private ring of three 16-row
 // slots (K, V, K, ...; cp.async, two slots ahead) and keeps its own running
-// maximum and sum.  The four warps of a CTA, the CTAs of a cluster (one key
-// range each, over distributed shared memory) and the tile kernel's ranges
-// are then joined in a fixed order.  Rows past the length are loaded as zeros.
+// maximum and sum.  The four warps of a CTA, then the CTAs that share a row
+// are joined in a fixed order.  Rows past the length are loaded as zeros.
 #include "shared_attention.cuh"
+
+#include <algorithm>
 
 namespace dl {
 namespace sa {
@@ -26,6 +31,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStep = 16;  // keys of a warp's step
 constexpr int kSlots = 3;
 constexpr float kRescale = 8.f;
+constexpr int kMaxParts = kMaxSplits + kMaxSuffixSplits;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
   const int bytes = real ? 16 : 0;  // 0: zero fill, nothing read
@@ -82,42 +88,114 @@ struct RowsShape {
   static constexpr int smem = ring > join ? ring : join;
 };
 
-template <int D, int NB>
-__global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnArgs a, const Plan pl,
-                                                              const Workspace ws, const float scale_log2) {
+// The whole softmax of one row from its parts' (maximum, sum), by one warp:
+// lanes hold two parts each, joined by a fixed tree.  factor[s]: of part s in
+// the normalised output.
+struct RowJoin {
+  float m, inv, lse;
+};
+template <class Part>
+__device__ __forceinline__ RowJoin join_row(int parts, Part&& part, float* factor) {
+  const int lane = threadIdx.x & 31;
+  float m[2], l[2], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int s = lane + 32 * u;
+    const float2 ml = s < parts ? part(s) : make_float2(-INFINITY, 0.f);
+    m[u] = ml.x;
+    l[u] = ml.y;
+    top = fmaxf(top, m[u]);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    m[u] = m[u] == -INFINITY ? 0.f : exp2_approx(m[u] - top);
+    sum = fmaf(l[u], m[u], sum);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 32 * u < parts) factor[lane + 32 * u] = m[u] * inv;
+  return {sum == 0.f ? 0.f : top, inv, sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2};
+}
+
+// out += y * f; a part of factor 0 may be undefined.
+__device__ __forceinline__ void add_part(float4& out, float4 y, float f) {
+  if (f == 0.f) return;
+  out.x = fmaf(y.x, f, out.x);
+  out.y = fmaf(y.y, f, out.y);
+  out.z = fmaf(y.z, f, out.z);
+  out.w = fmaf(y.w, f, out.w);
+}
+
+// Row `row` (new token * group + query head of the group) of unit (b, h).
+__device__ __forceinline__ size_t row_index(const SharedAttnArgs& a, int b, int h, int row) {
+  return (size_t(b) * a.rows + row / a.group) * a.query_heads + h * a.group + row % a.group;
+}
+template <int D>
+__device__ __forceinline__ void store_piece(const SharedAttnArgs& a, int b, int h, int row, int piece, float4 v) {
+  bf16* out = a.out + (size_t(b) * a.rows + row / a.group) * a.ldo + size_t(h * a.group + row % a.group) * D + piece * 4;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+// Adds the weights of suffix keys [j0, j1) of unit (b, h) to their sums, from
+// the stored scores and the rows' norms in shared memory.
+__device__ __forceinline__ void add_suffix_weights(const SharedAttnArgs& a, const Workspace& ws, float scale_log2, int b,
+                                                   int h, int n, int j0, int j1, const float* row_m,
+                                                   const float* row_r) {
+  const int live = a.rows * a.group;
+  float* sums = a.sw + (size_t(b) * a.kv_heads + h) * a.scap;
+  const float* scores = ws.scores + (size_t(b) * a.kv_heads + h) * live * a.scap;
+  for (int j = j0 + int(threadIdx.x); j < j1; j += blockDim.x) {
+    float w = 0.f;
+    for (int row = 0; row < live; ++row)
+      if (j < suffix_seen(n, a.rows, row / a.group))
+        w = fmaf(exp2_approx(fmaf(scores[size_t(row) * a.scap + j], scale_log2, -row_m[row])), row_r[row], w);
+    sums[j] += w;
+  }
+}
+
+template <int D, int NB, bool SOLO>
+__global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(const SharedAttnArgs a, const Plan pl,
+                                                                               const Workspace ws,
+                                                                               const float scale_log2) {
   constexpr int R = 8 * NB;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float warp_m[kWarps][R], warp_l[kWarps][R], cta_m[R], cta_l[R], row_m[R], row_r[R];
+  __shared__ float part_f[R][kMaxSuffixSplits];
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int g4 = lane >> 2, c2 = (lane & 3) * 2;
   const int live = a.rows * a.group;  // row = new token * group + query head of the group
-  // The suffix and the queries come from before the tile kernel, whose blocks
-  // have all waited for them; its own results are waited for below.
-  if (pl.splits == 0) {
-    wait_prior();
-    allow_next();
-  }
-  const int n = suffix_len(a, b);
-  const int per = ((n + pl.suffix_splits - 1) / pl.suffix_splits + kStep - 1) / kStep * kStep;
-  const int j0 = min(n, split * per), j1 = min(n, j0 + per);
-  const int steps = (j1 - j0 + kStep * kWarps - 1) / (kStep * kWarps);
-  // Step i of this warp: keys j0 + (i * kWarps + warp) * 16 ...
-  auto key0 = [&](int i) { return j0 + (i * kWarps + warp) * kStep; };
+  // Beside the tile kernel: the suffix and the queries come from before it, and
+  // its blocks, which had to start before this kernel could, have waited for them.
+  if (SOLO) wait_prior();
+  allow_next();
+  // Keys in steps of 16: the prefix's (SOLO), then the suffix's; this CTA has
+  // the steps [g0, g1), its warps every fourth.
+  const int np = SOLO ? prefix_len(a, b) : 0, n = suffix_len(a, b);
+  const int ps = (np + kStep - 1) / kStep, all = ps + (n + kStep - 1) / kStep;
+  const int g0 = int((long long)all * split / pl.suffix_splits), g1 = int((long long)all * (split + 1) / pl.suffix_splits);
+  const int steps = (g1 - g0 + kWarps - 1) / kWarps;
 
   const uint32_t ring = smem_addr(smem) + warp * (kSlots * kStep * D * 2);
-  const bf16* base_k = a.sk + size_t(b) * a.s_seq + size_t(h) * D;
-  const bf16* base_v = a.sv + size_t(b) * a.s_seq + size_t(h) * D;
   constexpr int P = D / 8;  // 16-byte pieces of a row; piece c of row k lies at c ^ (k & 7)
   auto load = [&](int item) {  // items: K of step 0, V of step 0, K of step 1, ...
-    const int i = item >> 1, slot = item % kSlots;
-    if (i < steps) {
-      const bf16* src = item & 1 ? base_v : base_k;
+    const int i = item >> 1, slot = item % kSlots, g = g0 + i * kWarps + warp;
+    if (g < g1) {
+      const bool pre = g < ps;
+      const bf16* base = item & 1 ? (pre ? a.pv : a.sv) : (pre ? a.pk : a.sk);
+      const bf16* src = base + (pre ? 0 : size_t(b) * a.s_seq) + size_t(h) * D;
+      const int j0 = (pre ? g : g - ps) * kStep, end = pre ? np : n;
+      const size_t stride = pre ? a.p_row : a.s_row;
       const uint32_t dst = ring + slot * (kStep * D * 2);
 #pragma unroll
       for (int u = 0; u < kStep * P / 32; ++u) {
-        const int idx = u * 32 + lane, k = idx / P, c = idx % P, j = key0(i) + k;
-        const bool real = j < j1;
-        cp16(dst + k * (D * 2) + ((c ^ (k & 7)) << 4), src + size_t(real ? j : 0) * a.s_row + c * 8, real);
+        const int idx = u * 32 + lane, k = idx / P, c = idx % P, j = j0 + k;
+        const bool real = j < end;
+        cp16(dst + k * (D * 2) + ((c ^ (k & 7)) << 4), src + size_t(real ? j : 0) * stride + c * 8, real);
       }
     }
     cp_commit();
@@ -137,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
       q[nb][kk][1] = row < live ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 + c2) : 0u;
     }
   }
-  // Rows 8 nb + c2, + 1 of the score fragments: how many keys they see.
+  // Rows 8 nb + c2, + 1 of the score fragments: how many suffix keys they see.
   int seen[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -158,6 +236,8 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
 
 #pragma unroll 1
   for (int i = 0; i < steps; ++i) {
+    const int g = g0 + i * kWarps + warp;
+    const bool pre = g < ps;
     load(2 * i + 2);
     cp_wait<2>();
     __syncwarp();
@@ -176,7 +256,8 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
       }
     }
     __syncwarp();  // every lane has read the slot that the next load refills
-    const int ka = key0(i) + g4, kb = ka + 8;
+    if (g >= g1) continue;  // this warp's last turn may be empty
+    const int ka = (pre ? g : g - ps) * kStep + g4, kb = ka + 8;
     uint32_t p_hi[NB][2], p_lo[NB][2];
     bool grow = false;
     float top[NB][2];
@@ -184,10 +265,10 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int end = min(seen[nb][u], j1), row = 8 * nb + c2 + u;
-        if (scores && row < live) {
-          if (ka < j1) scores[size_t(row) * a.scap + ka] = s[nb][u];
-          if (kb < j1) scores[size_t(row) * a.scap + kb] = s[nb][2 + u];
+        const int row = 8 * nb + c2 + u, end = row < live ? (pre ? np : seen[nb][u]) : 0;
+        if (scores && row < live && !pre) {
+          if (ka < n) scores[size_t(row) * a.scap + ka] = s[nb][u];
+          if (kb < n) scores[size_t(row) * a.scap + kb] = s[nb][2 + u];
         }
         if (ka >= end) s[nb][u] = -INFINITY;
         if (kb >= end) s[nb][2 + u] = -INFINITY;
@@ -310,105 +391,149 @@ __global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttnA
       v.z = fmaf(y.z, f, v.z);
       v.w = fmaf(y.w, f, v.w);
     }
-    cta_o[i] = v;
+    if (SOLO) {
+      cta_o[i] = v;
+    } else {
+      const size_t part = ((size_t(split) * a.batch + b) * a.kv_heads + h) * live + row;
+      reinterpret_cast<float4*>(ws.suffix_o + part * D)[(i % (D / 4)) ^ (row & 7)] = v;
+    }
   }
-  if (pl.splits) {
-    wait_prior();  // the prefix ranges are complete
-    allow_next();
+  if constexpr (!SOLO) {
+    if (t < live)
+      ws.suffix_ml[((size_t(split) * a.batch + b) * a.kv_heads + h) * live + t] = make_float2(cta_m[t], cta_l[t]);
+    // One block outlasts the tile kernel, so that this kernel's end, which the
+    // join waits for, is the end of both; the others make room at once.
+    if (split == int(gridDim.x) - 1 && h == int(gridDim.y) - 1 && b == int(gridDim.z) - 1) wait_prior();
+    return;
   }
-  const unsigned ctas = pl.suffix_splits;
+  const int ctas = pl.suffix_splits;
   if (ctas > 1) tc::cluster_sync();
   else __syncthreads();
-
-  // The row's whole softmax, the same in every CTA of the cluster: the
-  // cluster's ranges in order, then the prefix ranges in order.
-  auto part_of = [&](int row, int s) {
-    const int token = b * a.rows + row / a.group;
-    return ((size_t(s) * pl.units + h) * pl.tiles + token / pl.per_tile) * kRows +
-           token % pl.per_tile * a.group + row % a.group;
-  };
-  if (t < live) {
-    float top = -INFINITY, sum = 0.f;
-    for (unsigned r = 0; r < ctas; ++r) top = fmaxf(top, remote_f32(&cta_m[t], r));
-    for (int s = 0; s < pl.splits; ++s) top = fmaxf(top, ws.part_ml[part_of(t, s)].x);
-    for (unsigned r = 0; r < ctas; ++r) {
-      const float x = remote_f32(&cta_m[t], r);
-      if (x != -INFINITY) sum = fmaf(remote_f32(&cta_l[t], r), exp2_approx(x - top), sum);
-    }
-    for (int s = 0; s < pl.splits; ++s) {
-      const float2 ml = ws.part_ml[part_of(t, s)];
-      sum = fmaf(ml.y, ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top), sum);
-    }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-    row_m[t] = sum == 0.f ? 0.f : top;
-    row_r[t] = inv;
-    if (split == 0) {
-      const size_t row = (size_t(b) * a.rows + t / a.group) * a.query_heads + h * a.group + t % a.group;
-      if (a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-      if (a.pw) ws.norm[row] = RowNorm{row_m[t], inv};
+  for (int row = warp; row < live; row += kWarps) {
+    const RowJoin j = join_row(
+        ctas, [&](int s) { return make_float2(remote_f32(&cta_m[row], s), remote_f32(&cta_l[row], s)); }, part_f[row]);
+    if (lane == 0) {
+      row_m[row] = j.m;
+      row_r[row] = j.inv;
+      if (split == 0) {
+        if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
+        if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+      }
     }
   }
   __syncthreads();
-  for (int i = split * kThreads + t; i < live * (D / 4); i += int(ctas) * kThreads) {
-    const int row = i / (D / 4), c = i % (D / 4);  // c: where the piece lies, c ^ (row & 7): the piece
-    const float mr = row_m[row], inv = row_r[row];
+  for (int i = split * kThreads + t; i < live * (D / 4); i += ctas * kThreads) {
+    const int row = i / (D / 4);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float4 y, float f) {
-      v.x = fmaf(y.x, f, v.x);
-      v.y = fmaf(y.y, f, v.y);
-      v.z = fmaf(y.z, f, v.z);
-      v.w = fmaf(y.w, f, v.w);
-    };
-    for (unsigned r = 0; r < ctas; ++r) {
-      const float x = remote_f32(&cta_m[row], r);
-      if (x != -INFINITY) add(remote_f32x4(joined + i * 4, r), exp2_approx(x - mr));
-    }
-    const int feature = (c ^ (row & 7)) * 4;
-#pragma unroll 4
-    for (int s = 0; s < pl.splits; ++s) {
-      const size_t part = part_of(row, s);
-      const float x = ws.part_ml[part].x;
-      const int r = int(part % kRows);
-      if (x != -INFINITY)
-        add(reinterpret_cast<const float4*>(ws.part_o + part * D)[(feature >> 2) ^ (r & 7)], exp2_approx(x - mr));
-    }
-    bf16* out = a.out + (size_t(b) * a.rows + row / a.group) * a.ldo + size_t(h * a.group + row % a.group) * D + feature;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+    for (int r = 0; r < ctas; ++r) add_part(v, remote_f32x4(joined + i * 4, r), part_f[row][r]);
+    store_piece<D>(a, b, h, row, (i % (D / 4)) ^ (row & 7), v);
   }
-  if (a.sw) {
-    float* sums = a.sw + (size_t(b) * a.kv_heads + h) * a.scap;
-    for (int j = j0 + t; j < j1; j += kThreads) {
-      float w = 0.f;
-      for (int row = 0; row < live; ++row)
-        if (j < suffix_seen(n, a.rows, row / a.group))
-          w = fmaf(exp2_approx(fmaf(scores[size_t(row) * a.scap + j], scale_log2, -row_m[row])), row_r[row], w);
-      sums[j] += w;
-    }
-  }
+  if (a.sw)  // of this CTA's suffix keys
+    add_suffix_weights(a, ws, scale_log2, b, h, n, max(0, g0 - ps) * kStep, min(n, max(0, g1 - ps) * kStep), row_m, row_r);
   if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, int NB>
-cudaError_t launch_shape(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  constexpr int smem = RowsShape<D, NB>::smem;
-  const cudaError_t e = allow_smem<shared_rows_kernel<D, NB>>(smem);
-  if (e != cudaSuccess) return e;
-  DependentLaunch d(dim3(p.suffix_splits, a.kv_heads, a.batch), kThreads, smem, stream, p.suffix_splits);
-  return cudaLaunchKernelEx(&d.cfg, shared_rows_kernel<D, NB>, a, p, ws, attention_scale(D) * kLog2e);
+// Joins the prefix ranges and the suffix ranges of the rows of unit (b, h);
+// with weights, blockIdx.x is a chunk of the suffix keys whose sums it adds.
+template <int D>
+__global__ void __launch_bounds__(kThreads) shared_join_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws,
+                                                              const float scale_log2) {
+  constexpr int kBatch = 16;  // parts in flight per thread
+  __shared__ float factor[kFewRows][kMaxParts], row_m[kFewRows], row_r[kFewRows];
+  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int live = a.rows * a.group, parts = pl.splits + pl.suffix_splits;
+  const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;               // rows between two prefix ranges
+  const size_t suffix_stride = size_t(a.batch) * a.kv_heads * live;          // and two suffix ranges
+  const size_t suffix_first = (size_t(b) * a.kv_heads + h) * live;
+  auto prefix_row = [&](int row) {  // within range 0; modulo 128: the row of its tile
+    const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
+    return (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows +
+           token % pl.per_tile * a.group + row % a.group;
+  };
+  auto load = [&](int i, int s0, float4* y) {  // piece i % (D / 4) of row i / (D / 4), parts s0 ..
+    const int row = i / (D / 4), piece = i % (D / 4);
+    const size_t first = prefix_row(row);
+    const float* pre = ws.part_o + first / kRows * kRows * D + part_offset<D>(int(first % kRows), piece * 4);
+    const float* suf = ws.suffix_o + (suffix_first + row) * D + piece * 4;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int s = s0 + u;
+      if (s < parts)
+        y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
+                                                              : suf + (s - pl.splits) * suffix_stride * D);
+    }
+  };
+  wait_prior();
+  allow_next();
+  const int pieces = chunk == 0 ? live * (D / 4) : 0;
+  float4 y[kBatch];
+  if (t < pieces) load(t, 0, y);  // on their way while the factors are made
+  for (int row = warp; row < live; row += kWarps) {
+    const RowJoin j = join_row(
+        parts,
+        [&](int s) {
+          return s < pl.splits ? ws.part_ml[prefix_row(row) + s * stride]
+                               : ws.suffix_ml[suffix_first + row + (s - pl.splits) * suffix_stride];
+        },
+        factor[row]);
+    if (lane == 0) {
+      row_m[row] = j.m;
+      row_r[row] = j.inv;
+      if (chunk == 0) {
+        if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
+        if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = t; i < pieces; i += kThreads) {
+    const int row = i / (D / 4);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < parts; s0 += kBatch) {
+      if (i != t || s0) load(i, s0, y);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (s0 + u < parts) add_part(v, y[u], factor[row][s0 + u]);
+    }
+    store_piece<D>(a, b, h, row, i % (D / 4), v);
+  }
+  if (a.sw) {
+    const int n = suffix_len(a, b), chunks = gridDim.x;
+    add_suffix_weights(a, ws, scale_log2, b, h, n, int((long long)n * chunk / chunks),
+                       int((long long)n * (chunk + 1) / chunks), row_m, row_r);
+  }
 }
 
-template <int D>
+template <int D, int NB, bool SOLO>
+cudaError_t launch_shape(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+  constexpr int smem = RowsShape<D, NB>::smem;
+  const cudaError_t e = allow_smem<shared_rows_kernel<D, NB, SOLO>>(smem);
+  if (e != cudaSuccess) return e;
+  DependentLaunch d(dim3(p.suffix_splits, a.kv_heads, a.batch), kThreads, smem, stream, SOLO ? p.suffix_splits : 1);
+  return cudaLaunchKernelEx(&d.cfg, shared_rows_kernel<D, NB, SOLO>, a, p, ws, attention_scale(D) * kLog2e);
+}
+
+template <int D, bool SOLO>
 cudaError_t launch_width(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
   const int live = a.rows * a.group;
-  return live <= 8    ? launch_shape<D, 1>(a, p, ws, stream)
-         : live <= 16 ? launch_shape<D, 2>(a, p, ws, stream)
-                      : launch_shape<D, 4>(a, p, ws, stream);
+  return live <= 8    ? launch_shape<D, 1, SOLO>(a, p, ws, stream)
+         : live <= 16 ? launch_shape<D, 2, SOLO>(a, p, ws, stream)
+                      : launch_shape<D, 4, SOLO>(a, p, ws, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  return a.width == 64 ? launch_width<64>(a, p, ws, stream) : launch_width<128>(a, p, ws, stream);
+  if (p.splits == 0) return a.width == 64 ? launch_width<64, true>(a, p, ws, stream) : launch_width<128, true>(a, p, ws, stream);
+  return a.width == 64 ? launch_width<64, false>(a, p, ws, stream) : launch_width<128, false>(a, p, ws, stream);
+}
+
+cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+  const int chunks = a.sw ? std::min(16, (a.scap + 1023) / 1024) : 1;
+  DependentLaunch d(dim3(chunks, a.kv_heads, a.batch), kThreads, 0, stream);
+  const float scale = attention_scale(a.width) * kLog2e;
+  return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_join_kernel<64>, a, p, ws, scale)
+                       : cudaLaunchKernelEx(&d.cfg, shared_join_kernel<128>, a, p, ws, scale);
 }
 
 }  // namespace sa

@@ -37,11 +37,16 @@ constexpr int kAtom = kRows * 128;  // [128 rows][64 BF16]
 constexpr uint32_t kTmemCols = 512;  // S0, S1, O0, O1
 constexpr float kRescale = 8.f;     // base-2 growth of the maximum that moves the reference
 
-template <int D, bool WIDE>
+// BESIDE: a CTA that leaves room for one of the few-row kernel on its SM (65 KB
+// of shared memory, a quarter of the registers), which then streams the
+// suffixes while this one is busy with products.
+template <int D, bool WIDE, bool BESIDE>
 struct Shape {
   static constexpr int slot = D / 64 * kAtom;  // a K, V or Q tile
-  static constexpr int stages = D == 64 ? 8 : WIDE ? 5 : 4;
-  static constexpr int smem = (WIDE ? 2 : 1) * slot + stages * slot + 1024;
+  static constexpr int queries = WIDE ? 2 : 1;
+  static constexpr int stages = D == 64 ? 8 : !WIDE ? 4 : BESIDE ? 3 : 5;
+  static constexpr int smem = (queries + stages) * slot + 1024;
+  static constexpr int bound = BESIDE ? 512 : kThreads;  // threads that the registers are shared out for
 };
 
 struct alignas(64) TileArgs {
@@ -73,14 +78,16 @@ __device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uin
   for (int i = 0; i < 4; ++i) {
     const int kk = 4 * half + i;
     const uint64_t v = smem_desc_sw128_mn(v_tile + uint32_t(kk * 2048), kAtom);
-    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kk * 8), v, idesc, (accumulate || i) ? 1u : 0u);
-    mma_bf16_ts(tmem_o, tmem_p + uint32_t(kKeys / 2 + kk * 8), v, idesc, 1u);
+    const uint32_t p = tmem_p + uint32_t((kk >> 1) * 32 + (kk & 1) * 8);  // 32 keys: 16 columns hi, 16 lo
+    mma_bf16_ts(tmem_o, p, v, idesc, (accumulate || i) ? 1u : 0u);
+    mma_bf16_ts(tmem_o, p + 16, v, idesc, 1u);
   }
 }
 
-template <int D, bool WIDE>
-__global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_constant__ TileArgs t) {
-  using S = Shape<D, WIDE>;
+template <int D, bool WIDE, bool BESIDE>
+__global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
+    shared_tile_kernel(const __grid_constant__ TileArgs t) {
+  using S = Shape<D, WIDE, BESIDE>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_half[2], p_full[2], o_full[2];
   __shared__ uint64_t dirty, clean, drained;
@@ -88,23 +95,21 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
   __shared__ uint32_t tmem_slot;
   __shared__ int most[2];  // keys of the prefix / suffix that any row sees
   __shared__ int failed_s;
-  __shared__ float2 other[kRows];  // second stream's (m, l)
+  __shared__ float2 stream_ml[2][kRows];
   volatile int* failed = &failed_s;
   const SharedAttnArgs& a = t.a;
   const Plan& pl = t.plan;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ring = base + (WIDE ? 2 : 1) * S::slot;
-  float* stage = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)));
+  const uint32_t ring = base + S::queries * S::slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // Work of this CTA: row tiles fastest, so CTAs side by side read the same keys.
-  const int per_cta = WIDE ? 2 : 1, groups = (pl.tiles + per_cta - 1) / per_cta;
-  int at = blockIdx.x;
-  const int tile0 = at % groups * per_cta;
-  at /= groups;
-  const int split = at % pl.splits;
-  at /= pl.splits;
-  const int h = at % a.kv_heads, seq = at / a.kv_heads;  // seq = 0 when pooled
+  // Task of this CTA (row tiles fastest, so CTAs side by side read the same
+  // keys), whole or one of its key ranges.
+  const int cta = blockIdx.x, rest = pl.tasks - pl.full;
+  const int task = cta < pl.full ? cta : pl.full + (cta - pl.full) % rest;
+  const int split = cta < pl.full ? 0 : (cta - pl.full) / rest, splits = cta < pl.full ? 1 : pl.splits;
+  const int tile0 = task % pl.groups * pl.per_cta, h = task / pl.groups % a.kv_heads;
+  const int seq = task / pl.groups / a.kv_heads;  // 0 when pooled
   const int unit_tokens = pl.pooled ? a.batch * a.rows : a.rows;
   const int streams = WIDE && tile0 + 1 >= pl.tiles ? 1 : 2;
 
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
   fence_after_sync();
   const uint32_t tmem = tmem_slot;
   const int np = (most[0] + kKeys - 1) / kKeys, nt = np + (most[1] + kKeys - 1) / kKeys;
-  const int k0 = int((long long)nt * split / pl.splits), n = int((long long)nt * (split + 1) / pl.splits) - k0;
+  const int k0 = int((long long)nt * split / splits), n = int((long long)nt * (split + 1) / splits) - k0;
   // Key tiles of stream s, and the i-th one's place among the n.
   auto count = [&](int s) { return WIDE ? (s < streams ? n : 0) : (n + 1 - s) / 2; };
   auto nth = [&](int s, int i) { return WIDE ? i : 2 * i + s; };
@@ -328,24 +333,45 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
       ok = role_wait_warp(&s_full[x], i & 1, failed);
       if (!ok) break;
       fence_after_sync();
-      uint32_t s[kKeys];
+      // All 128 scores in registers, or (BESIDE, for fewer registers) two
+      // passes over them, 32 at a time with the next 32 on their way.
+      const bool masked = __any_sync(0xffffffffu, lim < kKeys);
+      constexpr int held = BESIDE ? 2 : 4;
+      uint32_t s[held][32];
+      auto fetch = [&](int j) { tmem_ld32_async(t_s + 32 * j, s[j % held]); };
+      auto mask = [&](int j) {
+        if (masked) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tmem_ld32_async(t_s + 32 * j, s + 32 * j);
+          for (int k = 0; k < 32; ++k)
+            if (32 * j + k >= lim) s[j % held][k] = 0xff800000u;  // -infinity
+        }
+      };
+      auto turn = [&](int j) {
+        tmem_ld_wait32(s[j % held]);
+        if (j < 3) fetch(j + 1);
+        mask(j);
+      };
+      if constexpr (BESIDE) {
+        fetch(0);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tmem_ld_wait32(s + 32 * j);
-      if (__any_sync(0xffffffffu, lim < kKeys)) {
+        for (int j = 0; j < 4; ++j) fetch(j);
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j)
-          if (j >= lim) s[j] = 0xff800000u;  // -infinity
+        for (int j = 0; j < 4; ++j) {
+          tmem_ld_wait32(s[j]);
+          mask(j);
+        }
       }
-      float mx[8];
+      float mx[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mx[j] = fmaxf(__uint_as_float(s[j]), __uint_as_float(s[8 + j]));
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (BESIDE) turn(j);
 #pragma unroll
-      for (int j = 16; j < kKeys; j += 16)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[j + k]), __uint_as_float(s[j + 8 + k])));
+        for (int k = 0; k < 16; ++k)
+          mx[k & 7] =
+              fmaxf(mx[k & 7], fmaxf(__uint_as_float(s[j % held][k]), __uint_as_float(s[j % held][16 + k])));
+      }
+      if constexpr (BESIDE) fetch(0);
       const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
                               fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
       const bool grow = (top - m) * c > kRescale;  // also from -infinity
@@ -370,18 +396,19 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
       uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if constexpr (BESIDE) turn(j);
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float x0, x1;
-          unpair(fma2(pair(__uint_as_float(s[32 * j + 2 * k]), __uint_as_float(s[32 * j + 2 * k + 1])), c2, shift2),
+          unpair(fma2(pair(__uint_as_float(s[j % held][2 * k]), __uint_as_float(s[j % held][2 * k + 1])), c2, shift2),
                  x0, x1);
           const uint64_t e = pair(exp2_approx(x0), exp2_approx(x1));
           sum[k & 3] = add2(sum[k & 3], e);
           split_bf16(e, hi[k], lo[k]);
         }
-        tmem_st16(t_s + 16 * j, hi);
-        tmem_st16(t_s + kKeys / 2 + 16 * j, lo);
+        tmem_st16(t_s + 32 * j, hi);  // over the 32 scores just used
+        tmem_st16(t_s + 32 * j + 16, lo);
         if (j & 1) {  // 64 keys are there: their products may begin
           tmem_st_wait();
           fence_before_sync();
@@ -393,109 +420,91 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
       unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
       l += s0 + s1;
     }
-    // Both streams' products must be over before the ring becomes scratch.
+    // Both streams' products must be over before the operands become scratch.
     for (int s = 0; s < 2; ++s)
       if (count(s) > 0) ok = role_wait_warp(&o_full[s], 0, failed) && ok;
     fence_after_sync();
-    float m2 = m == -INFINITY ? -INFINITY : m * c, mine_f = 1.f, other_f = 0.f;
-    auto piece = [&](int i, int row) { return stage + (WIDE ? x * kRows * D : 0) + row * D + ((i ^ (row & 7)) << 2); };
+    // A wide stream ends its own row; the two narrow ones hold parts of one
+    // row, and each thread ends half of its features.
+    float m2 = m == -INFINITY ? -INFINITY : m * c, f[2] = {1.f, 0.f};
     if constexpr (!WIDE) {
-      if (x == 1) {
-        other[r] = make_float2(m2, l);
-        if (mine > 0 && ok) {
-#pragma unroll 1
-          for (int j = 0; j < D / 32; ++j) {
-            uint32_t o[32];
-            __syncwarp();
-            tmem_ld32_async(t_o + 32 * j, o);
-            tmem_ld_wait32(o);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              *reinterpret_cast<uint4*>(piece(8 * j + k, r)) =
-                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-          }
-        }
-      }
+      stream_ml[x][r] = make_float2(m2, l);
       named_sync(1, 2 * kRows);
-      if (x == 0 && count(1) > 0) {
-        const float2 ml = other[r];
-        const float top = fmaxf(m2, ml.x);
-        mine_f = m2 == -INFINITY ? 0.f : exp2_approx(m2 - top);
-        other_f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-        l = l * mine_f + ml.y * other_f;
-        m2 = top;
-      }
+      const float2 p = stream_ml[0][r], q = stream_ml[1][r];
+      m2 = fmaxf(p.x, q.x);
+      f[0] = p.x == -INFINITY ? 0.f : exp2_approx(p.x - m2);
+      f[1] = q.x == -INFINITY ? 0.f : exp2_approx(q.x - m2);
+      l = p.y * f[0] + q.y * f[1];
+    } else if (m == -INFINITY) {
+      f[0] = 0.f;
     }
     ok = ok && !*failed;
     if (!ok) l = NAN;
-    if (WIDE || x == 0) {
-      const bool has = mine > 0 && ok;
-      if (!pl.pooled && pl.splits == 1) {  // the whole softmax of the row
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
-        const int hq = h * a.group + r % a.group;
-        bf16* out = a.out + size_t(token) * a.ldo + size_t(hq) * D;
+    constexpr int columns = WIDE ? D : D / 2;
+    const int from = WIDE ? 0 : x * columns;
+    const uint32_t t_o0 = tmem + lanes + 256 + (WIDE ? x * 128 : 0) + from;
+    auto features = [&](int j, float* v) {  // features from + 32 j ..
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld32_async(t_o0 + 32 * j, o);
+      tmem_ld_wait32(o);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = f[0] != 0.f ? __uint_as_float(o[k]) * f[0] : 0.f;
+      if constexpr (!WIDE) {
+        __syncwarp();
+        tmem_ld32_async(t_o0 + 128 + 32 * j, o);
+        tmem_ld_wait32(o);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = f[1] != 0.f ? fmaf(__uint_as_float(o[k]), f[1], v[k]) : v[k];
+      }
+    };
+    if (!BESIDE && splits == 1) {  // the whole softmax of the row
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+      const int hq = h * a.group + r % a.group;
+      bf16* out = a.out + size_t(token) * a.ldo + size_t(hq) * D + from;
 #pragma unroll 1
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t o[32];
-          __syncwarp();
-          tmem_ld32_async(t_o + 32 * j, o);
-          tmem_ld_wait32(o);
-          if (!live) continue;
-#pragma unroll
-          for (int k = 0; k < 8; k += 2) {
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = has ? __uint_as_float(o[4 * k + u]) * mine_f : 0.f;
-            if (!WIDE && other_f != 0.f) {
-              const float4 y = *reinterpret_cast<const float4*>(piece(8 * j + k, r));
-              const float4 z = *reinterpret_cast<const float4*>(piece(8 * j + k + 1, r));
-              const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
-#pragma unroll
-              for (int u = 0; u < 8; ++u) v[u] = fmaf(w[u], other_f, v[u]);
-            }
-            reinterpret_cast<uint4*>(out)[4 * j + k / 2] =
-                make_uint4(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv),
-                           pack_bf16(v[4] * inv, v[5] * inv), pack_bf16(v[6] * inv, v[7] * inv));
-          }
-        }
+      for (int j = 0; j < columns / 32; ++j) {
+        float v[32];
+        features(j, v);
         if (live) {
-          const size_t row = size_t(token) * a.query_heads + hq;
-          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * kLn2;
-          if (t.norms) t.ws.norm[row] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{m2, inv};
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            reinterpret_cast<uint4*>(out)[4 * j + k / 8] =
+                make_uint4(pack_bf16(v[k] * inv, v[k + 1] * inv), pack_bf16(v[k + 2] * inv, v[k + 3] * inv),
+                           pack_bf16(v[k + 4] * inv, v[k + 5] * inv), pack_bf16(v[k + 6] * inv, v[k + 7] * inv));
         }
-      } else if (tile < pl.tiles) {
-        const size_t part = (size_t(split) * pl.units + seq * a.kv_heads + h) * pl.tiles + tile;
-        t.ws.part_ml[part * kRows + r] = make_float2(m2, l);
+      }
+      if (live && (WIDE || x == 0)) {
+        const size_t row = size_t(token) * a.query_heads + hq;
+        if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m2 + log2f(l)) * kLn2;
+        if (t.norms) t.ws.norm[row] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{m2, inv};
+      }
+    } else if (tile < pl.tiles) {
+      // One range's part, staged in shared memory and copied out in bulk.
+      const size_t part = (size_t(split) * rest + task - pl.full) * pl.per_cta + (WIDE ? x : 0);
+      const uint32_t stage = base + uint32_t((WIDE ? x * D : from) * kRows * 4);
+      if (WIDE || x == 0) t.ws.part_ml[part * kRows + r] = make_float2(m2, l);
 #pragma unroll 1
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t o[32];
-          __syncwarp();
-          tmem_ld32_async(t_o + 32 * j, o);
-          tmem_ld_wait32(o);
+      for (int j = 0; j < columns / 32; ++j) {
+        float v[32];
+        features(j, v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = has ? __uint_as_float(o[4 * k + u]) * mine_f : 0.f;
-            if (!WIDE && other_f != 0.f) {
-              const float4 y = *reinterpret_cast<const float4*>(piece(8 * j + k, r));
-              v[0] = fmaf(y.x, other_f, v[0]);
-              v[1] = fmaf(y.y, other_f, v[1]);
-              v[2] = fmaf(y.z, other_f, v[2]);
-              v[3] = fmaf(y.w, other_f, v[3]);
-            }
-            *reinterpret_cast<float4*>(piece(8 * j + k, r)) = make_float4(v[0], v[1], v[2], v[3]);
-          }
-        }
-        fence_proxy_async_smem();
-        named_sync(2 + x, kRows);
-        if (r == 0) {
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(t.ws.part_o +
-                                                                                            part * kRows * D),
-                       "r"(smem_addr(stage + (WIDE ? x * kRows * D : 0))), "r"(kRows * D * 4)
+        for (int k = 0; k < 8; ++k) {
+          const int i = 8 * j + k, half = i / (D / 8);
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           stage + uint32_t((half * kRows + r) * (D * 2) + (((i % (D / 8)) ^ (r & 7)) << 4))),
+                       "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
                        : "memory");
-          asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
         }
+      }
+      fence_proxy_async_smem();
+      named_sync(2 + x, kRows);
+      if (r == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(t.ws.part_o +
+                                                                                          (part * D + from) * kRows),
+                     "r"(stage), "r"(kRows * columns * 4)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       }
     }
     fence_before_sync();
@@ -504,38 +513,36 @@ __global__ void __launch_bounds__(kThreads, 1) shared_tile_kernel(const __grid_c
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the key ranges of each (token, query head): one warp per row, the
-// ranges in order.
+// Joins the key ranges of the split tasks: one warp per (token, query head),
+// the ranges in order.
 template <int D>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws,
                                                            bool norms) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = row % kRows;
   wait_prior();
   allow_next();
-  if (row >= a.batch * a.rows * a.query_heads) return;
-  const int token = row / a.query_heads, hq = row % a.query_heads, h = hq / a.group, g = hq % a.group;
-  const int seq = pl.pooled ? 0 : token / a.rows, local = pl.pooled ? token : token % a.rows;
-  const int r = local % pl.per_tile * a.group + g;
-  const size_t first = size_t(seq * a.kv_heads + h) * pl.tiles + local / pl.per_tile;
-  const size_t stride = size_t(pl.units) * pl.tiles;
+  const int rest = pl.tasks - pl.full, task = pl.full + row / kRows / pl.per_cta;
+  const int tile = task % pl.groups * pl.per_cta + row / kRows % pl.per_cta, h = task / pl.groups % a.kv_heads;
+  const int local = tile * pl.per_tile + r / a.group;
+  if (r / a.group >= pl.per_tile || local >= a.rows) return;
+  const int token = task / pl.groups / a.kv_heads * a.rows + local, hq = h * a.group + r % a.group;
+  const size_t stride = size_t(rest) * pl.per_cta * kRows;  // rows between two ranges
   float top = -INFINITY;
-  for (int s = 0; s < pl.splits; ++s) top = fmaxf(top, ws.part_ml[(first + s * stride) * kRows + r].x);
+  for (int s = 0; s < pl.splits; ++s) top = fmaxf(top, ws.part_ml[row + s * stride].x);
   constexpr int F = D / 32;  // consecutive features of a lane
-  const int where = ((lane * F / 4) ^ (r & 7)) * 4 + lane * F % 4;
+  const float* src = ws.part_o + size_t(row / kRows) * kRows * D + part_offset<D>(r, lane * F);
   float l = 0.f, o[F] = {};
+#pragma unroll 4
   for (int s = 0; s < pl.splits; ++s) {
-    const size_t part = (first + s * stride) * kRows + r;
-    const float2 ml = ws.part_ml[part];
+    const float2 ml = ws.part_ml[row + s * stride];
     const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
     l = fmaf(ml.y, f, l);
-    if (f == 0.f) continue;
-    const float* src = ws.part_o + part * D + where;
     float v[F];
     if constexpr (F == 4) {
-      const float4 y = *reinterpret_cast<const float4*>(src);
+      const float4 y = *reinterpret_cast<const float4*>(src + s * stride * D);
       v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
     } else {
-      const float2 y = *reinterpret_cast<const float2*>(src);
+      const float2 y = *reinterpret_cast<const float2*>(src + s * stride * D);
       v[0] = y.x, v[1] = y.y;
     }
 #pragma unroll
@@ -546,20 +553,29 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnArgs 
 #pragma unroll
   for (int c = 0; c < F; c += 2) out[c / 2] = pack_bf16(o[c] * inv, o[c + 1] * inv);
   if (lane == 0) {
-    if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
-    if (norms) ws.norm[row] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{top, inv};
+    const size_t at = size_t(token) * a.query_heads + hq;
+    if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    if (norms) ws.norm[at] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{top, inv};
   }
 }
 
-template <int D, bool WIDE>
+template <int D, bool WIDE, bool BESIDE>
 cudaError_t launch_tiles_shape(const TileArgs& t, cudaStream_t stream) {
-  using S = Shape<D, WIDE>;
-  cudaError_t e = allow_smem<shared_tile_kernel<D, WIDE>>(S::smem);
+  constexpr int smem = Shape<D, WIDE, BESIDE>::smem;
+  const cudaError_t e = allow_smem<shared_tile_kernel<D, WIDE, BESIDE>>(smem);
   if (e != cudaSuccess) return e;
-  const int per_cta = WIDE ? 2 : 1;
-  const unsigned grid = unsigned((t.plan.tiles + per_cta - 1) / per_cta) * t.plan.splits * t.plan.units;
-  DependentLaunch d(dim3(grid), kThreads, S::smem, stream);
-  return cudaLaunchKernelEx(&d.cfg, shared_tile_kernel<D, WIDE>, t);
+  const unsigned grid = unsigned(t.plan.full + (t.plan.tasks - t.plan.full) * t.plan.splits);
+  DependentLaunch d(dim3(grid), kThreads, smem, stream);
+  return cudaLaunchKernelEx(&d.cfg, shared_tile_kernel<D, WIDE, BESIDE>, t);
+}
+
+template <int D>
+cudaError_t launch_tiles_width(const TileArgs& t, cudaStream_t stream) {
+  if (t.plan.pooled)
+    return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, true>(t, stream)
+                               : launch_tiles_shape<D, false, true>(t, stream);
+  return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, false>(t, stream)
+                             : launch_tiles_shape<D, false, false>(t, stream);
 }
 
 }  // namespace
@@ -575,13 +591,11 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace
   if (a.pcap && !(encode_prefix_map(&t.pk, a, a.pk) && encode_prefix_map(&t.pv, a, a.pv))) return cudaErrorInvalidValue;
   if (a.scap && !p.pooled && !(encode_suffix_map(&t.sk, a, a.sk) && encode_suffix_map(&t.sv, a, a.sv)))
     return cudaErrorInvalidValue;
-  if (a.width == 64) return p.wide ? launch_tiles_shape<64, true>(t, stream) : launch_tiles_shape<64, false>(t, stream);
-  return p.wide ? launch_tiles_shape<128, true>(t, stream) : launch_tiles_shape<128, false>(t, stream);
+  return a.width == 64 ? launch_tiles_width<64>(t, stream) : launch_tiles_width<128>(t, stream);
 }
 
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  const int rows = a.batch * a.rows * a.query_heads;
-  DependentLaunch d(dim3((rows + 7) / 8), 256, 0, stream);
+  DependentLaunch d(dim3(unsigned(p.tasks - p.full) * p.per_cta * (kRows / 8)), 256, 0, stream);
   const bool norms = a.pw || a.sw;
   return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<64>, a, p, ws, norms)
                        : cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<128>, a, p, ws, norms);

@@ -11,39 +11,67 @@ strides raise ValueError, refusals of the library DolittleError.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
 
-
-def _cache(t, name: str, dims: int):
-    """(row stride, outer stride) of a cache tensor [..., positions, heads, width]."""
-    if t.dtype != torch.bfloat16 or t.dim() != dims or not t.is_cuda:
-        raise ValueError(f"{name} must be a bfloat16 CUDA tensor of {dims} dimensions")
-    s = t.stride()
-    if (s[-1] != 1 and t.shape[-1] > 1) or (s[-2] != t.shape[-1] and t.shape[-2] > 1):
-        raise ValueError(f"{name}: the heads of a position must be contiguous")
-    row = t.shape[-1] * t.shape[-2]
-    # A stride torch left arbitrary (one position, one cache) is not used.
-    inner = s[-3] if t.shape[-3] > 1 else row
-    return inner, (s[0] if dims == 4 and t.shape[0] > 1 else inner * t.shape[-3])
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+# The stream's address without building a Stream object (a decode step makes
+# one call per block).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _flat(t, name: str, dtype, shape, device):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}")
+def _pair(key, value, name: str, dims: int, device: int):
+    """(shape, row stride, outer stride) of key and value caches [..., positions, heads, width]."""
+    shape, stride = key.shape, key.stride()
+    if (key.dtype is not _BF16 or value.dtype is not _BF16 or len(shape) != dims or value.shape != shape or
+            key.get_device() != device or value.get_device() != device):
+        raise ValueError(f"{name}_key and {name}_value must be bfloat16 tensors of one shape and {dims} dimensions, "
+                         "on the query's device")
+    width, heads, positions = shape[-1], shape[-2], shape[-3]
+    # torch leaves the stride of a dimension of size 1 arbitrary; it is not used.
+    row = stride[-3] if positions > 1 else heads * width
+    outer = stride[0] if dims == 4 and shape[0] > 1 else row * positions
+    if (stride[-1] != 1 and width > 1) or (stride[-2] != width and heads > 1):
+        raise ValueError(f"{name}_key: the heads of a position must be contiguous")
+    if value.stride() != stride and any(a != b for a, b, n in zip(value.stride(), stride, shape) if n > 1):
+        raise ValueError(f"{name}_key and {name}_value must have the same strides")
+    return shape, row, outer
+
+
+def _flat(t, name: str, dtype, shape: tuple, device: int) -> int:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on the query's device")
     return t.data_ptr()
 
 
-def _pair(key, value, name: str, dims: int, device):
-    row, outer = _cache(key, f"{name}_key", dims)
-    if value.shape != key.shape or value.device != device or key.device != device:
-        raise ValueError(f"{name}_key and {name}_value must have one shape, on the query's device")
-    if _cache(value, f"{name}_value", dims) != (row, outer):
-        raise ValueError(f"{name}_key and {name}_value must have the same strides")
-    return row, outer
+def _on(device: int, call):
+    """call(stream) with `device` current."""
+    if torch.cuda.current_device() == device:
+        return check(call(_raw_stream(device)))
+    with torch.cuda.device(device):
+        return check(call(_raw_stream(device)))
+
+
+@functools.lru_cache(maxsize=512)
+def _attention_workspace(device: int, batch, rows, heads, kv_heads, width, prefix, suffix, weights: bool) -> int:
+    # The size depends on the shapes alone; the pointers only have to be plausible here.
+    a = _lib.SharedAttention(batch, rows, heads, kv_heads, width, 0, 0, 16, 16, prefix, kv_heads * width, 16, 16, 16,
+                             suffix, kv_heads * width, kv_heads * width * suffix, 16)
+    with torch.cuda.device(device):
+        return lib().dl_attention_shared_workspace_bytes(C.byref(a), weights)
+
+
+@functools.lru_cache(maxsize=512)
+def _evict_workspace(device: int, caches, kv_heads, width, capacity, budget) -> int:
+    e = _lib.CacheEviction(caches=caches, kv_heads=kv_heads, width=width, capacity=capacity, budget=budget,
+                           row_stride=kv_heads * width, out_row_stride=kv_heads * width, out_capacity=capacity)
+    with torch.cuda.device(device):
+        return lib().dl_cache_evict_workspace_bytes(C.byref(e))
 
 
 def attention_shared(query, prefix_key, prefix_value, suffix_key, suffix_value, prefix_lengths, suffix_lengths, *,
@@ -56,54 +84,52 @@ def attention_shared(query, prefix_key, prefix_value, suffix_key, suffix_value, 
     float32); a row without keys gives zeros and -inf.  prefix_weights
     [Hkv, P] and suffix_weights [B, Hkv, S] (float32) are added to: the softmax
     weight each key received from every row and query head."""
-    if query.dtype != torch.bfloat16 or query.dim() != 4 or not query.is_cuda:
+    shape, inner, device = query.shape, query.stride(), query.get_device()
+    if query.dtype is not _BF16 or len(shape) != 4 or device < 0:
         raise ValueError("query must be a bfloat16 CUDA tensor [batch, rows, heads, width]")
-    device = query.device
-    batch, rows, heads, width = query.shape
-    token, inner = heads * width, query.stride()
-    stride = inner[1] if rows > 1 else inner[0] if batch > 1 else token
-    if ((width > 1 and inner[3] != 1) or (heads > 1 and inner[2] != width) or
+    batch, rows, heads, width = shape
+    stride = inner[1] if rows > 1 else inner[0] if batch > 1 else heads * width
+    if ((inner[3] != 1 and width > 1) or (inner[2] != width and heads > 1) or
             (rows > 1 and batch > 1 and inner[0] != rows * stride)):
         raise ValueError("query: heads contiguous, one stride between tokens")
-    a = _lib.SharedAttention(batch=batch, rows=rows, query_heads=heads, width=width, query_stride=stride)
+    kv_heads = pk = pv = pl = sk = sv = sl = None
+    prefix = p_row = suffix = s_row = s_seq = 0
     if prefix_key is not None:
-        a.prefix_row_stride, _ = _pair(prefix_key, prefix_value, "prefix", 3, device)
-        a.prefix_capacity, a.kv_heads = prefix_key.shape[0], prefix_key.shape[1]
-        if prefix_key.shape[2] != width:
+        (prefix, kv_heads, w), p_row, _ = _pair(prefix_key, prefix_value, "prefix", 3, device)
+        if w != width:
             raise ValueError("prefix caches must have the query's head width")
-        a.prefix_key, a.prefix_value = prefix_key.data_ptr(), prefix_value.data_ptr()
-        a.prefix_lengths = _flat(prefix_lengths, "prefix_lengths", torch.int64, (batch,), device)
+        pk, pv = prefix_key.data_ptr(), prefix_value.data_ptr()
+        pl = _flat(prefix_lengths, "prefix_lengths", _I64, (batch,), device)
     if suffix_key is not None:
-        a.suffix_row_stride, a.suffix_sequence_stride = _pair(suffix_key, suffix_value, "suffix", 4, device)
-        if suffix_key.shape[0] != batch or suffix_key.shape[3] != width or (
-                prefix_key is not None and suffix_key.shape[2] != a.kv_heads):
+        (n, suffix, h, w), s_row, s_seq = _pair(suffix_key, suffix_value, "suffix", 4, device)
+        if n != batch or w != width or (kv_heads is not None and h != kv_heads):
             raise ValueError("suffix caches must be [batch, positions, the prefix's KV heads, the query's head width]")
-        a.suffix_capacity, a.kv_heads = suffix_key.shape[1], suffix_key.shape[2]
-        a.suffix_key, a.suffix_value = suffix_key.data_ptr(), suffix_value.data_ptr()
-        a.suffix_lengths = _flat(suffix_lengths, "suffix_lengths", torch.int64, (batch,), device)
-    if prefix_key is None and suffix_key is None:
+        kv_heads = h
+        sk, sv = suffix_key.data_ptr(), suffix_value.data_ptr()
+        sl = _flat(suffix_lengths, "suffix_lengths", _I64, (batch,), device)
+    if kv_heads is None:
         raise ValueError("a prefix or a suffix cache is required")
     pw = sw = None
     if prefix_weights is not None:
-        pw = _flat(prefix_weights, "prefix_weights", torch.float32, (a.kv_heads, a.prefix_capacity), device)
+        pw = _flat(prefix_weights, "prefix_weights", _F32, (kv_heads, prefix), device)
     if suffix_weights is not None:
-        sw = _flat(suffix_weights, "suffix_weights", torch.float32, (batch, a.kv_heads, a.suffix_capacity), device)
+        sw = _flat(suffix_weights, "suffix_weights", _F32, (batch, kv_heads, suffix), device)
     if out is None:
-        out = torch.empty((batch, rows, heads, width), dtype=torch.bfloat16, device=device)
+        out = torch.empty(shape, dtype=_BF16, device=query.device)
     else:
-        _flat(out, "out", torch.bfloat16, query.shape, device)
+        _flat(out, "out", _BF16, shape, device)
     if lse is None:
-        lse = torch.empty((batch, rows, heads), dtype=torch.float32, device=device)
+        lse = torch.empty((batch, rows, heads), dtype=_F32, device=query.device)
     else:
-        _flat(lse, "lse", torch.float32, (batch, rows, heads), device)
-    with torch.cuda.device(device):
-        ref = C.byref(a)
-        need = lib().dl_attention_shared_workspace_bytes(ref, pw is not None or sw is not None)
-        if not need:
-            raise _lib.DolittleError(_lib.DL_INVALID_ARGUMENT, lib().dl_last_error().decode())
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        check(lib().dl_attention_shared(ref, query.data_ptr(), out.data_ptr(), lse.data_ptr(), pw, sw,
-                                        workspace.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        _flat(lse, "lse", _F32, (batch, rows, heads), device)
+    a = _lib.SharedAttention(batch, rows, heads, kv_heads, width, stride, 0, pk, pv, prefix, p_row, pl, sk, sv, suffix,
+                             s_row, s_seq, sl)
+    # 0 when the library refuses the shape: the call below then says why.
+    need = _attention_workspace(device, batch, rows, heads, kv_heads, width, prefix, suffix,
+                                pw is not None or sw is not None)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+    _on(device, lambda stream: lib().dl_attention_shared(C.byref(a), query.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                                         pw, sw, workspace.data_ptr(), stream))
     return out, lse
 
 
@@ -117,31 +143,28 @@ def cache_evict(key, value, weights, positions, lengths, budget: int, *, first: 
     place, kept slots beyond it move into the vacated ones.  out = (key, value,
     weights, positions, lengths) receives the result, None evicts in place.
     Returns the five tensors that hold it."""
-    device = key.device
-    row, outer = _pair(key, value, "cache", 4, device)
-    n, capacity, heads, width = key.shape
-    e = _lib.CacheEviction(caches=n, kv_heads=heads, width=width, capacity=capacity, budget=budget, first=first,
-                           recent=recent, row_stride=row, cache_stride=outer)
-    e.key, e.value = key.data_ptr(), value.data_ptr()
-    e.weights = _flat(weights, "weights", torch.float32, (n, heads, capacity), device)
-    e.positions = _flat(positions, "positions", torch.int32, (n, heads, capacity), device)
-    e.lengths = _flat(lengths, "lengths", torch.int64, (n,), device)
+    device = key.get_device()
+    if device < 0:
+        raise ValueError("the caches must be CUDA tensors")
+    (n, capacity, heads, width), row, outer = _pair(key, value, "cache", 4, device)
     if out is None:
         out = (key, value, weights, positions, lengths)
-    key_out, value_out, weights_out, positions_out, lengths_out = out
-    e.out_row_stride, e.out_cache_stride = _pair(key_out, value_out, "out", 4, device)
-    room = key_out.shape[1]
-    if tuple(key_out.shape) != (n, room, heads, width):
-        raise ValueError("the output caches must be [caches, positions, heads, width] like the inputs")
-    e.key_out, e.value_out, e.out_capacity = key_out.data_ptr(), value_out.data_ptr(), room
-    e.weights_out = _flat(weights_out, "weights (output)", torch.float32, (n, heads, room), device)
-    e.positions_out = _flat(positions_out, "positions (output)", torch.int32, (n, heads, room), device)
-    e.lengths_out = _flat(lengths_out, "lengths (output)", torch.int64, (n,), device)
-    with torch.cuda.device(device):
-        ref = C.byref(e)
-        need = lib().dl_cache_evict_workspace_bytes(ref)
-        if not need:
-            raise _lib.DolittleError(_lib.DL_INVALID_ARGUMENT, lib().dl_last_error().decode())
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        check(lib().dl_cache_evict(ref, workspace.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        room, out_row, out_outer = capacity, row, outer
+    else:
+        (m, room, h, w), out_row, out_outer = _pair(out[0], out[1], "out", 4, device)
+        if m != n or h != heads or w != width:
+            raise ValueError("the output caches must be [caches, positions, heads, width] like the inputs")
+    slots, out_slots = (n, heads, capacity), (n, heads, room)
+    if budget < 0 or first < 0 or recent < 0:
+        raise ValueError("budget, first and recent must not be negative")
+    e = _lib.CacheEviction(n, heads, width, capacity, budget, first, recent, key.data_ptr(), value.data_ptr(), row,
+                           outer, _flat(weights, "weights", _F32, slots, device),
+                           _flat(positions, "positions", _I32, slots, device),
+                           _flat(lengths, "lengths", _I64, (n,), device), out[0].data_ptr(), out[1].data_ptr(), room,
+                           out_row, out_outer, _flat(out[2], "weights (output)", _F32, out_slots, device),
+                           _flat(out[3], "positions (output)", _I32, out_slots, device),
+                           _flat(out[4], "lengths (output)", _I64, (n,), device))
+    need = _evict_workspace(device, n, heads, width, capacity, budget)
+    workspace = torch.empty(need, dtype=torch.uint8, device=key.device)
+    _on(device, lambda stream: lib().dl_cache_evict(C.byref(e), workspace.data_ptr(), stream))
     return out
