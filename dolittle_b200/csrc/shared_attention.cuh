@@ -82,9 +82,10 @@ struct DependentLaunch {
   }
 };
 
-// Dynamic shared memory above 48 KB, allowed once per kernel and device; with
-// the whole of the SM's memory as shared memory, or blocks of two kernels
-// would not fit side by side (the split follows the kernel that came first).
+// Dynamic shared memory above 48 KB, allowed once per kernel and device; and
+// the same split of the SM's memory for every kernel here, all of it shared
+// memory: blocks of two kernels fit side by side only within one split, and an
+// SM changes its split only when it is empty.
 template <auto Kernel>
 cudaError_t allow_smem(int bytes) {
   static std::atomic<uint64_t> done{0};  // devices 0 .. 63
@@ -209,6 +210,9 @@ struct RingPos {
   }
 };
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "

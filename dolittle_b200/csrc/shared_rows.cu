@@ -169,17 +169,8 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int g4 = lane >> 2, c2 = (lane & 3) * 2;
   const int live = a.rows * a.group;  // row = new token * group + query head of the group
-  // Beside the tile kernel: the suffix and the queries come from before it, and
-  // its blocks, which had to start before this kernel could, have waited for them.
-  if (SOLO) wait_prior();
-  allow_next();
-  // Keys in steps of 16: the prefix's (SOLO), then the suffix's; this CTA has
-  // the steps [g0, g1), its warps every fourth.
-  const int np = SOLO ? prefix_len(a, b) : 0, n = suffix_len(a, b);
-  const int ps = (np + kStep - 1) / kStep, all = ps + (n + kStep - 1) / kStep;
-  const int g0 = int((long long)all * split / pl.suffix_splits), g1 = int((long long)all * (split + 1) / pl.suffix_splits);
-  const int steps = (g1 - g0 + kWarps - 1) / kWarps;
-
+  int np, n, ps, g0, g1, steps;  // keys of prefix and suffix; steps of 16: prefix steps, this CTA's [g0, g1), per warp
+  float o[NB][D / 16][4], m[NB][2], l[NB][2];
   const uint32_t ring = smem_addr(smem) + warp * (kSlots * kStep * D * 2);
   constexpr int P = D / 8;  // 16-byte pieces of a row; piece c of row k lies at c ^ (k & 7)
   auto load = [&](int item) {  // items: K of step 0, V of step 0, K of step 1, ...
@@ -200,143 +191,162 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
     }
     cp_commit();
   };
-  load(0);
-  load(1);
-
-  // Query fragments: row 8 nb + g4 (zero past the live rows), features 16 kk + c2, + 8.
-  uint32_t q[NB][D / 16][2];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int row = 8 * nb + g4;
-    const bf16* src = a.q + (size_t(b) * a.rows + row / a.group) * a.ldq + size_t(h * a.group + row % a.group) * D;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      q[nb][kk][0] = row < live ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + c2) : 0u;
-      q[nb][kk][1] = row < live ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 + c2) : 0u;
-    }
-  }
-  // Rows 8 nb + c2, + 1 of the score fragments: how many suffix keys they see.
-  int seen[NB][2];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = 8 * nb + c2 + u;
-      seen[nb][u] = row < live ? suffix_seen(n, a.rows, row / a.group) : 0;
-    }
-  float o[NB][D / 16][4], m[NB][2], l[NB][2];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m[nb][0] = m[nb][1] = -INFINITY;  // unscaled references
-    l[nb][0] = l[nb][1] = 0.f;        // this lane's keys only
-#pragma unroll
-    for (int f = 0; f < D / 16; ++f) o[nb][f][0] = o[nb][f][1] = o[nb][f][2] = o[nb][f][3] = 0.f;
-  }
-  float* scores = a.sw ? ws.scores + (size_t(b) * a.kv_heads + h) * live * a.scap : nullptr;
-
+  // Turn -1 (SOLO) runs one step on no keys while the kernel before this one
+  // ends, which brings the loop's code in: a small call runs it only a few
+  // times.  Beside the tile kernel nothing has to be waited for: the suffix and
+  // the queries come from before it, and its blocks, which had to start before
+  // this kernel could, have waited for them.
 #pragma unroll 1
-  for (int i = 0; i < steps; ++i) {
-    const int g = g0 + i * kWarps + warp;
-    const bool pre = g < ps;
-    load(2 * i + 2);
-    cp_wait<2>();
-    __syncwarp();
-    float s[NB][4];
+  for (int turn = SOLO ? -1 : 0; turn < 1; ++turn) {
+    const int rows = turn < 0 ? 0 : live;
+    if (SOLO && turn == 0) wait_prior();
+    if (turn == 0) allow_next();
+    // Keys in steps of 16: the prefix's (SOLO), then the suffix's; this CTA has
+    // the steps [g0, g1), its warps every fourth.
+    np = SOLO && rows ? prefix_len(a, b) : 0;
+    n = rows ? suffix_len(a, b) : 0;
+    ps = (np + kStep - 1) / kStep;
+    const int all = ps + (n + kStep - 1) / kStep;
+    g0 = int((long long)all * split / pl.suffix_splits);
+    g1 = int((long long)all * (split + 1) / pl.suffix_splits);
+    steps = rows ? (g1 - g0 + kWarps - 1) / kWarps : 1;
+    load(0);
+    load(1);
+
+    // Query fragments: row 8 nb + g4 (zero past the live rows), features 16 kk + c2, + 8.
+    uint32_t q[NB][D / 16][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-    {
-      const uint32_t slot = ring + (2 * i) % kSlots * (kStep * D * 2);
-      const int k = lane & 15;
+    for (int nb = 0; nb < NB; ++nb) {
+      const int row = 8 * nb + g4;
+      const bf16* src = a.q + (size_t(b) * a.rows + row / a.group) * a.ldq + size_t(h * a.group + row % a.group) * D;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t ka[4];
-        ldsm4(ka, slot + k * (D * 2) + (((2 * kk + (lane >> 4)) ^ (k & 7)) << 4));
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma16816(s[nb], ka, q[nb][kk][0], q[nb][kk][1]);
+        q[nb][kk][0] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + c2) : 0u;
+        q[nb][kk][1] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 + c2) : 0u;
       }
     }
-    __syncwarp();  // every lane has read the slot that the next load refills
-    if (g >= g1) continue;  // this warp's last turn may be empty
-    const int ka = (pre ? g : g - ps) * kStep + g4, kb = ka + 8;
-    uint32_t p_hi[NB][2], p_lo[NB][2];
-    bool grow = false;
-    float top[NB][2];
+    // Rows 8 nb + c2, + 1 of the score fragments: how many suffix keys they see.
+    int seen[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = 8 * nb + c2 + u, end = row < live ? (pre ? np : seen[nb][u]) : 0;
-        if (scores && row < live && !pre) {
-          if (ka < n) scores[size_t(row) * a.scap + ka] = s[nb][u];
-          if (kb < n) scores[size_t(row) * a.scap + kb] = s[nb][2 + u];
-        }
-        if (ka >= end) s[nb][u] = -INFINITY;
-        if (kb >= end) s[nb][2 + u] = -INFINITY;
-        float x = fmaxf(s[nb][u], s[nb][2 + u]);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        top[nb][u] = x;
-        grow = grow || (x - m[nb][u]) * scale_log2 > kRescale;
+        const int row = 8 * nb + c2 + u;
+        seen[nb][u] = row < rows ? suffix_seen(n, a.rows, row / a.group) : 0;
       }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float alpha[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bool up = (top[nb][u] - m[nb][u]) * scale_log2 > kRescale;
-          alpha[u] = up ? exp2_approx((m[nb][u] - top[nb][u]) * scale_log2) : 1.f;
-          if (up) m[nb][u] = top[nb][u];
-          l[nb][u] *= alpha[u];
-        }
-#pragma unroll
-        for (int f = 0; f < D / 16; ++f) {
-          o[nb][f][0] *= alpha[0];
-          o[nb][f][1] *= alpha[1];
-          o[nb][f][2] *= alpha[0];
-          o[nb][f][3] *= alpha[1];
-        }
-      }
-    }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float e[4];
+      m[nb][0] = m[nb][1] = -INFINITY;  // unscaled references
+      l[nb][0] = l[nb][1] = 0.f;        // this lane's keys only
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float shift = m[nb][u] == -INFINITY ? 0.f : -m[nb][u] * scale_log2;
-        e[u] = exp2_approx(fmaf(s[nb][u], scale_log2, shift));
-        e[2 + u] = exp2_approx(fmaf(s[nb][2 + u], scale_log2, shift));
-        l[nb][u] += e[u] + e[2 + u];
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t hi, lo;
-        split_bf16(pair(e[2 * u], e[2 * u + 1]), hi, lo);
-        p_hi[nb][u] = transpose8(hi);
-        p_lo[nb][u] = transpose8(lo);
-      }
+      for (int f = 0; f < D / 16; ++f) o[nb][f][0] = o[nb][f][1] = o[nb][f][2] = o[nb][f][3] = 0.f;
     }
-    load(2 * i + 3);
-    cp_wait<2>();
-    __syncwarp();
-    {
-      const uint32_t slot = ring + (2 * i + 1) % kSlots * (kStep * D * 2);
-      const int k = (lane & 7) + ((lane >> 4) & 1) * 8;
+    float* scores = a.sw ? ws.scores + (size_t(b) * a.kv_heads + h) * live * a.scap : nullptr;
+
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      const int g = g0 + i * kWarps + warp;
+      const bool pre = g < ps;
+      load(2 * i + 2);
+      cp_wait<2>();
+      __syncwarp();
+      float s[NB][4];
 #pragma unroll
-      for (int f = 0; f < D / 16; ++f) {
-        uint32_t va[4];
-        ldsm4_trans(va, slot + k * (D * 2) + (((2 * f + ((lane >> 3) & 1)) ^ (k & 7)) << 4));
+      for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+      {
+        const uint32_t slot = ring + (2 * i) % kSlots * (kStep * D * 2);
+        const int k = lane & 15;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          mma16816(o[nb][f], va, p_hi[nb][0], p_hi[nb][1]);
-          mma16816(o[nb][f], va, p_lo[nb][0], p_lo[nb][1]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t ka[4];
+          ldsm4(ka, slot + k * (D * 2) + (((2 * kk + (lane >> 4)) ^ (k & 7)) << 4));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16816(s[nb], ka, q[nb][kk][0], q[nb][kk][1]);
         }
       }
+      __syncwarp();  // every lane has read the slot that the next load refills
+      if (g >= g1 && rows) continue;  // this warp's last step may be empty
+      const int ka = (pre ? g : g - ps) * kStep + g4, kb = ka + 8;
+      uint32_t p_hi[NB][2], p_lo[NB][2];
+      bool grow = false;
+      float top[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 8 * nb + c2 + u, end = row < rows ? (pre ? np : seen[nb][u]) : 0;
+          if (scores && row < rows && !pre) {
+            if (ka < n) scores[size_t(row) * a.scap + ka] = s[nb][u];
+            if (kb < n) scores[size_t(row) * a.scap + kb] = s[nb][2 + u];
+          }
+          if (ka >= end) s[nb][u] = -INFINITY;
+          if (kb >= end) s[nb][2 + u] = -INFINITY;
+          float x = fmaxf(s[nb][u], s[nb][2 + u]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          top[nb][u] = x;
+          grow = grow || (x - m[nb][u]) * scale_log2 > kRescale;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float alpha[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bool up = (top[nb][u] - m[nb][u]) * scale_log2 > kRescale;
+            alpha[u] = up ? exp2_approx((m[nb][u] - top[nb][u]) * scale_log2) : 1.f;
+            if (up) m[nb][u] = top[nb][u];
+            l[nb][u] *= alpha[u];
+          }
+#pragma unroll
+          for (int f = 0; f < D / 16; ++f) {
+            o[nb][f][0] *= alpha[0];
+            o[nb][f][1] *= alpha[1];
+            o[nb][f][2] *= alpha[0];
+            o[nb][f][3] *= alpha[1];
+          }
+        }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float e[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float shift = m[nb][u] == -INFINITY ? 0.f : -m[nb][u] * scale_log2;
+          e[u] = exp2_approx(fmaf(s[nb][u], scale_log2, shift));
+          e[2 + u] = exp2_approx(fmaf(s[nb][2 + u], scale_log2, shift));
+          l[nb][u] += e[u] + e[2 + u];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t hi, lo;
+          split_bf16(pair(e[2 * u], e[2 * u + 1]), hi, lo);
+          p_hi[nb][u] = transpose8(hi);
+          p_lo[nb][u] = transpose8(lo);
+        }
+      }
+      load(2 * i + 3);
+      cp_wait<2>();
+      __syncwarp();
+      {
+        const uint32_t slot = ring + (2 * i + 1) % kSlots * (kStep * D * 2);
+        const int k = (lane & 7) + ((lane >> 4) & 1) * 8;
+#pragma unroll
+        for (int f = 0; f < D / 16; ++f) {
+          uint32_t va[4];
+          ldsm4_trans(va, slot + k * (D * 2) + (((2 * f + ((lane >> 3) & 1)) ^ (k & 7)) << 4));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            mma16816(o[nb][f], va, p_hi[nb][0], p_hi[nb][1]);
+            mma16816(o[nb][f], va, p_lo[nb][0], p_lo[nb][1]);
+          }
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
+    cp_wait<0>();
   }
-  cp_wait<0>();
 
   // This warp's maxima (base 2) and sums, then its outputs over the ring.
 #pragma unroll
@@ -435,67 +445,80 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
 
 // Joins the prefix ranges and the suffix ranges of the rows of unit (b, h);
 // with weights, blockIdx.x is a chunk of the suffix keys whose sums it adds.
+// Bound by latency (a few KB per block), so the work is spread thin: four warps
+// share a row, each every fourth part with all its loads in flight, lane =
+// 16-byte piece of the row; every one of them makes the row's factors itself.
+constexpr int kJoinThreads = 512, kJoinWarps = 4;  // warps of a row
+constexpr int kInFlight = 5;                       // parts that a warp has in flight
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) shared_join_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws,
-                                                              const float scale_log2) {
-  constexpr int kBatch = 16;  // parts in flight per thread
-  __shared__ float factor[kFewRows][kMaxParts], row_m[kFewRows], row_r[kFewRows];
-  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int live = a.rows * a.group, parts = pl.splits + pl.suffix_splits;
-  const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;               // rows between two prefix ranges
-  const size_t suffix_stride = size_t(a.batch) * a.kv_heads * live;          // and two suffix ranges
-  const size_t suffix_first = (size_t(b) * a.kv_heads + h) * live;
-  auto prefix_row = [&](int row) {  // within range 0; modulo 128: the row of its tile
-    const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
-    return (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows +
-           token % pl.per_tile * a.group + row % a.group;
-  };
-  auto load = [&](int i, int s0, float4* y) {  // piece i % (D / 4) of row i / (D / 4), parts s0 ..
-    const int row = i / (D / 4), piece = i % (D / 4);
-    const size_t first = prefix_row(row);
-    const float* pre = ws.part_o + first / kRows * kRows * D + part_offset<D>(int(first % kRows), piece * 4);
-    const float* suf = ws.suffix_o + (suffix_first + row) * D + piece * 4;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int s = s0 + u;
-      if (s < parts)
-        y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
-                                                              : suf + (s - pl.splits) * suffix_stride * D);
-    }
-  };
+__global__ void __launch_bounds__(kJoinThreads, 2) shared_join_kernel(const SharedAttnArgs a, const Plan pl,
+                                                                  const Workspace ws, const float scale_log2) {
+  constexpr int kAtOnce = kJoinThreads / 32 / kJoinWarps;  // rows of a pass
+  __shared__ float row_m[kFewRows], row_r[kFewRows], factors[kJoinThreads / 32][kMaxParts];
+  __shared__ float4 sums[kJoinThreads / 32][D / 4];
+  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = warp % kJoinWarps, live = a.rows * a.group, parts = pl.splits + pl.suffix_splits;
+  const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;       // rows between two prefix ranges
+  const size_t suffix_stride = size_t(a.batch) * a.kv_heads * live;  // and two suffix ranges
   wait_prior();
   allow_next();
-  const int pieces = chunk == 0 ? live * (D / 4) : 0;
-  float4 y[kBatch];
-  if (t < pieces) load(t, 0, y);  // on their way while the factors are made
-  for (int row = warp; row < live; row += kWarps) {
-    const RowJoin j = join_row(
-        parts,
-        [&](int s) {
-          return s < pl.splits ? ws.part_ml[prefix_row(row) + s * stride]
-                               : ws.suffix_ml[suffix_first + row + (s - pl.splits) * suffix_stride];
-        },
-        factor[row]);
-    if (lane == 0) {
-      row_m[row] = j.m;
-      row_r[row] = j.inv;
-      if (chunk == 0) {
-        if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
-        if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+#pragma unroll 1
+  for (int row0 = 0; row0 < live; row0 += kAtOnce) {
+    const int row = row0 + warp / kJoinWarps;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < live) {
+      const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
+      const int r = token % pl.per_tile * a.group + row % a.group;
+      const size_t first = (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows;
+      const size_t suffix_row = (size_t(b) * a.kv_heads + h) * live + row;
+      const float* pre = ws.part_o + first * D + part_offset<D>(r, lane * 4);
+      const float* suf = ws.suffix_o + suffix_row * D + lane * 4;
+      float4 y[kInFlight];
+      auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+          const int s = s0 + u * kJoinWarps;
+          if (s < parts && lane < D / 4)
+            y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
+                                                                  : suf + (s - pl.splits) * suffix_stride * D);
+        }
+      };
+      load(sub);
+      const RowJoin j = join_row(
+          parts,
+          [&](int s) {
+            return s < pl.splits ? ws.part_ml[first + r + s * stride]
+                                 : ws.suffix_ml[suffix_row + (s - pl.splits) * suffix_stride];
+          },
+          factors[warp]);
+      __syncwarp();
+#pragma unroll 1
+      for (int s0 = sub; s0 < parts; s0 += kInFlight * kJoinWarps) {
+        if (s0 != sub) load(s0);
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+          const int s = s0 + u * kJoinWarps;
+          if (s < parts) add_part(v, y[u], factors[warp][s]);
+        }
+      }
+      if (lane == 0 && sub == 0) {
+        row_m[row] = j.m;
+        row_r[row] = j.inv;
+        if (chunk == 0) {
+          if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
+          if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+        }
       }
     }
-  }
-  __syncthreads();
-  for (int i = t; i < pieces; i += kThreads) {
-    const int row = i / (D / 4);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < parts; s0 += kBatch) {
-      if (i != t || s0) load(i, s0, y);
+    if (lane < D / 4) sums[warp][lane] = v;
+    __syncthreads();
+    if (row < live && sub == 0 && chunk == 0 && lane < D / 4) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (s0 + u < parts) add_part(v, y[u], factor[row][s0 + u]);
+      for (int w = 1; w < kJoinWarps; ++w) add_part(v, sums[warp + w][lane], 1.f);
+      store_piece<D>(a, b, h, row, lane, v);
     }
-    store_piece<D>(a, b, h, row, i % (D / 4), v);
+    __syncthreads();
   }
   if (a.sw) {
     const int n = suffix_len(a, b), chunks = gridDim.x;
@@ -530,8 +553,10 @@ cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace&
 
 cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
   const int chunks = a.sw ? std::min(16, (a.scap + 1023) / 1024) : 1;
-  DependentLaunch d(dim3(chunks, a.kv_heads, a.batch), kThreads, 0, stream);
+  DependentLaunch d(dim3(chunks, a.kv_heads, a.batch), kJoinThreads, 0, stream);
   const float scale = attention_scale(a.width) * kLog2e;
+  const cudaError_t e = a.width == 64 ? allow_smem<shared_join_kernel<64>>(0) : allow_smem<shared_join_kernel<128>>(0);
+  if (e != cudaSuccess) return e;
   return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_join_kernel<64>, a, p, ws, scale)
                        : cudaLaunchKernelEx(&d.cfg, shared_join_kernel<128>, a, p, ws, scale);
 }

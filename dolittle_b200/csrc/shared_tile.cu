@@ -133,36 +133,45 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     fence_barrier_init();
   }
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kTmemCols);
-  wait_prior();
-  allow_next();  // after the wait: the next kernel may read what this one's inputs are before it waits itself
-  __syncthreads();
-
-  // Rows of the softmax threads.
-  const int x = (warp >> 2) & 1, r = threadIdx.x & (kRows - 1);
-  const int tile = WIDE ? tile0 + x : tile0;
-  const int local = tile * pl.per_tile + r / a.group;  // token within the unit
-  const bool live = warp < kTmaWarp && r / a.group < pl.per_tile && local < unit_tokens && tile < pl.tiles;
-  const int token = pl.pooled ? local : seq * a.rows + local;
-  const int seen_p = live ? prefix_len(a, token / a.rows) : 0;
-  const int seen_s = live && !pl.pooled ? suffix_seen(suffix_len(a, seq), a.rows, local) : 0;
-  if (warp < kTmaWarp) {
-    const int p = __reduce_max_sync(0xffffffffu, seen_p), s = __reduce_max_sync(0xffffffffu, seen_s);
-    if (lane == 0) {
-      atomicMax(&most[0], p);
-      atomicMax(&most[1], s);
-    }
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_map(&t.q);
+    if (a.pcap) prefetch_map(&t.pk), prefetch_map(&t.pv);
+    if (a.scap && !BESIDE) prefetch_map(&t.sk), prefetch_map(&t.sv);
   }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int np = (most[0] + kKeys - 1) / kKeys, nt = np + (most[1] + kKeys - 1) / kKeys;
-  const int k0 = int((long long)nt * split / splits), n = int((long long)nt * (split + 1) / splits) - k0;
+
+  // Row of a softmax thread.
+  const int x = (warp >> 2) & 1, r = threadIdx.x & (kRows - 1);
+  const int tile = WIDE ? tile0 + x : tile0;
+  const int local = tile * pl.per_tile + r / a.group;  // token within the unit
+  const bool live = warp < kTmaWarp && r / a.group < pl.per_tile && local < unit_tokens && tile < pl.tiles;
+  const int token = pl.pooled ? local : seq * a.rows + local;
+  int seen_p = 0, seen_s = 0, np = 0, k0 = 0, n = 0;  // keys the row sees; prefix tiles, the range's tiles
+  // Every role calls this before it touches what other kernels wrote.
+  auto begin = [&] {
+    wait_prior();
+    allow_next();  // after the wait: the next kernel may read what this one's inputs are before it waits itself
+    if (warp < kTmaWarp) {
+      seen_p = live ? prefix_len(a, token / a.rows) : 0;
+      seen_s = live && !pl.pooled ? suffix_seen(suffix_len(a, seq), a.rows, local) : 0;
+      const int p = __reduce_max_sync(0xffffffffu, seen_p), s = __reduce_max_sync(0xffffffffu, seen_s);
+      if (lane == 0) {
+        atomicMax(&most[0], p);
+        atomicMax(&most[1], s);
+      }
+    }
+    __syncthreads();
+    np = (most[0] + kKeys - 1) / kKeys;
+    const int nt = np + (most[1] + kKeys - 1) / kKeys;
+    k0 = int((long long)nt * split / splits);
+    n = int((long long)nt * (split + 1) / splits) - k0;
+  };
   // Key tiles of stream s, and the i-th one's place among the n.
   auto count = [&](int s) { return WIDE ? (s < streams ? n : 0) : (n + 1 - s) / 2; };
   auto nth = [&](int s, int i) { return WIDE ? i : 2 * i + s; };
-  const int steps = count(0);  // count(1) is at most that
-
   // Keys of the i-th tile that exist; a tile that holds fewer than 128 ends its side.
   auto filled = [&](int i) {
     const int g = k0 + i;
@@ -170,6 +179,8 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   };
 
   if (warp == kTmaWarp) {
+    begin();
+    const int steps = count(0);  // count(1) is at most that
     if (n > 0 && elect_one()) {
       const int boxes = D / 64, q_bytes = pl.per_tile * a.group * 128 * boxes;
       RingPos<S::stages> at;
@@ -211,6 +222,8 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    begin();
+    const int steps = count(0);
     if (n > 0 && elect_one()) {
       RingPos<S::stages> at;
       unsigned cleared = 0;
@@ -308,6 +321,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   } else if (warp == kClearWarp) {
     // Value rows past every length hold anything: times a weight of zero they
     // would still count, so the products wait until they are zeros.
+    begin();
     unsigned events = 0;
     for (int i = 0; i < n; ++i) events += filled(i) < kKeys;
     for (unsigned e = 0; e < events; ++e) {
@@ -322,23 +336,37 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   } else if (warp < kTmaWarp) {
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + x * kKeys, t_o = tmem + lanes + 256 + x * 128;
-    const int mine = count(x);
     const float c = t.scale_log2;
     float m = -INFINITY, l = 0.f;  // m: unscaled reference of the row
     bool ok = true;
+    // Turn -1 (BESIDE) runs the code once on whatever the scores' columns hold,
+    // while the kernel before this one ends: a decode step has only a few turns,
+    // and fetching the loop from memory that other kernels' data went through
+    // took longer than they do (batch 32 on 8192 keys: 4900 and 3400 cycles for
+    // the two passes of the first turn, 720 and 2400 after it).
 #pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
+    for (int i = BESIDE ? -1 : 0;; ++i) {
+      if (i == 0) {
+        begin();
+        m = -INFINITY;
+        l = 0.f;
+      }
+      if (i >= 0 && i >= count(x)) break;
       const int g = k0 + nth(x, i);
-      const int lim = g < np ? seen_p - g * kKeys : seen_s - (g - np) * kKeys;  // keys of the tile this row sees
-      ok = role_wait_warp(&s_full[x], i & 1, failed);
-      if (!ok) break;
-      fence_after_sync();
-      // All 128 scores in registers, or (BESIDE, for fewer registers) two
-      // passes over them, 32 at a time with the next 32 on their way.
+      int lim = kKeys;  // keys of the tile this row sees
+      if (i >= 0) {
+        lim = g < np ? seen_p - g * kKeys : seen_s - (g - np) * kKeys;
+        ok = role_wait_warp(&s_full[x], i & 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+      }
       const bool masked = __any_sync(0xffffffffu, lim < kKeys);
-      constexpr int held = BESIDE ? 2 : 4;
+      // BESIDE: two rolled passes over the scores, 32 at a time, for a quarter of
+      // the registers and of the code (a decode step runs each loop only a few
+      // times, so fetching unrolled code would take longer than running it).
+      // Otherwise all 128 scores in registers, unrolled.
+      constexpr int held = BESIDE ? 1 : 4;
       uint32_t s[held][32];
-      auto fetch = [&](int j) { tmem_ld32_async(t_s + 32 * j, s[j % held]); };
       auto mask = [&](int j) {
         if (masked) {
 #pragma unroll
@@ -346,36 +374,35 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
             if (32 * j + k >= lim) s[j % held][k] = 0xff800000u;  // -infinity
         }
       };
-      auto turn = [&](int j) {
-        tmem_ld_wait32(s[j % held]);
-        if (j < 3) fetch(j + 1);
-        mask(j);
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto raise = [&](int j) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          mx[k & 3] =
+              fmaxf(mx[k & 3], fmaxf(__uint_as_float(s[j % held][k]), __uint_as_float(s[j % held][16 + k])));
       };
       if constexpr (BESIDE) {
-        fetch(0);
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          tmem_ld32_async(t_s + 32 * j, s[0]);
+          tmem_ld_wait32(s[0]);
+          mask(j);
+          raise(j);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fetch(j);
+        for (int j = 0; j < 4; ++j) tmem_ld32_async(t_s + 32 * j, s[j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           tmem_ld_wait32(s[j]);
           mask(j);
         }
-      }
-      float mx[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (BESIDE) turn(j);
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          mx[k & 7] =
-              fmaxf(mx[k & 7], fmaxf(__uint_as_float(s[j % held][k]), __uint_as_float(s[j % held][16 + k])));
+        for (int j = 0; j < 4; ++j) raise(j);
       }
-      if constexpr (BESIDE) fetch(0);
-      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                              fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grow = (top - m) * c > kRescale;  // also from -infinity
-      if (i == 0) {
+      if (i <= 0) {
         m = top;
       } else if (__any_sync(0xffffffffu, grow)) {
         const float alpha = grow ? exp2_approx((m - top) * c) : 1.f;
@@ -394,9 +421,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
       const float shift = m == -INFINITY ? 0.f : -m * c;
       const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift);
       uint64_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (BESIDE) turn(j);
+      auto weights = [&](int j) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -413,8 +438,20 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
           tmem_st_wait();
           fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(j == 1 ? &p_half[x] : &p_full[x]);
+          if (lane == 0 && i >= 0) mbar_arrive(j == 1 ? &p_half[x] : &p_full[x]);
         }
+      };
+      if constexpr (BESIDE) {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          tmem_ld32_async(t_s + 32 * j, s[0]);
+          tmem_ld_wait32(s[0]);
+          mask(j);
+          weights(j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) weights(j);
       }
       float s0, s1;
       unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
@@ -597,6 +634,9 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
   DependentLaunch d(dim3(unsigned(p.tasks - p.full) * p.per_cta * (kRows / 8)), 256, 0, stream);
   const bool norms = a.pw || a.sw;
+  const cudaError_t e =
+      a.width == 64 ? allow_smem<shared_merge_kernel<64>>(0) : allow_smem<shared_merge_kernel<128>>(0);
+  if (e != cudaSuccess) return e;
   return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<64>, a, p, ws, norms)
                        : cudaLaunchKernelEx(&d.cfg, shared_merge_kernel<128>, a, p, ws, norms);
 }
