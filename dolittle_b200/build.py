@@ -1,4 +1,5 @@
-"""Build the sm_100a shared library in-tree: dolittle_b200/libdolittle_b200.so.
+"""Build the sm_100a shared library in-tree, dolittle_b200/libdolittle_b200.so,
+and the torch-side calls of dolittle_b200/shared.py, dolittle_b200/_torch_shared.so.
 
     python -m dolittle_b200.build [--verbose-ptxas]
 
@@ -17,10 +18,13 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdolittle_b200.so")
+TORCH_SRC = os.path.join(CSRC, "torch_shared.cpp")
+TORCH_OUT = os.path.join(HERE, "_torch_shared.so")
 BUILD = os.path.join(HERE, "_build")
 ROOT = os.path.dirname(HERE)
 
 NVCC = os.environ.get("NVCC", "nvcc")
+CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "--fmad=false",
          "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-I", os.path.join(ROOT, "include")]
@@ -41,6 +45,28 @@ def _stale(target, deps):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_torch_calls(force: bool = False) -> str:
+    """The extension module that shared.py calls (host code only; torch's own
+    libraries are already loaded when it is imported)."""
+    header = os.path.join(ROOT, "include", "dolittle_b200.h")
+    if not force and not _stale(TORCH_OUT, [TORCH_SRC, header]):
+        return TORCH_OUT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(root, "include"),
+           "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(CUDA_HOME, "include"), TORCH_SRC,
+           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", TORCH_OUT]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("torch calls failed to build:\n" + r.stdout + r.stderr)
+    return TORCH_OUT
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:
@@ -75,6 +101,7 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
+    build_torch_calls(force)
     return OUT
 
 
