@@ -1,16 +1,20 @@
 // Eviction from KV caches by accumulated attention weight (see
 // dl_cache_evict in the public header for the definition).
 //
-// Two launches.  evict_select_kernel: one cluster of 1-8 CTAs per (cache, KV
-// head) orders the slots by a 32-bit key (protected highest, then the weight's
-// order-preserving bits, NaN lowest), finds the budget-th largest key by radix
-// selection over 11-, 11- and 10-bit digits, and ranks ties, vacated slots
-// ("holes", below the kept count) and kept slots beyond it ("movers") with
-// prefix sums in slot order; hole i receives mover i.  evict_move_kernel
-// copies the rows of the resulting (destination, source) list.  Sources lie
-// at or above the kept count and destinations below it, so moving in place
-// needs no order between rows.  Counts and integer prefix sums only: results
-// do not depend on scheduling.
+// evict_select_kernel: one cluster of 1-8 CTAs per (cache, KV head) gives each
+// slot a 32-bit key (protected highest, then the weight's order-preserving
+// bits, NaN lowest) and finds the last slot that stays: histograms of 11, 11
+// and 10 bits narrow the keys down until at most 256 slots share the bits found
+// so far, those are ranked against one another by (key, slot); only more than
+// 256 equal keys need the ties counted in slot order.  Then a slot stays if its
+// (key, slot) is at least the cut's, and prefix sums in slot order pair vacated
+// slots ("holes", below the kept count) with kept slots beyond it ("movers"):
+// hole i receives mover i.  Weights and positions move with the pairing; rows
+// are copied by the same CTAs when that is little work, and by
+// evict_move_kernel, spread over all SMs, otherwise.  Sources lie at or above
+// the kept count and destinations below it, so moving in place needs no order
+// between rows.  Integer counts and prefix sums only: results do not depend on
+// scheduling.
 #include <algorithm>
 #include <climits>
 
@@ -20,9 +24,11 @@
 namespace dl {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kMaxCached = 40 * 1024;  // keys held in shared memory per CTA
+constexpr int kRanked = 256;       // slots of a unit ranked one against all
+constexpr int kMostTiles = 1024;   // runs of kThreads slots per CTA
+constexpr int kMaxCtas = 8;
 
 // dst, src and mover lists of one unit, then the entry count of every unit.
 __host__ __device__ __forceinline__ int* list_of(int* ws, int unit, int budget) { return ws + size_t(unit) * 3 * budget; }
@@ -41,13 +47,13 @@ __device__ __forceinline__ T block_scan(T v, T* warp_sums, T* total) {
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    T s = warp_sums[lane], e = s;
+    T s = lane < kWarps ? warp_sums[lane] : T(0), e = s;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const T y = __shfl_up_sync(0xffffffffu, e, o);
       if (lane >= o) e += y;
     }
-    warp_sums[lane] = e - s;
+    if (lane < kWarps) warp_sums[lane] = e - s;
     if (lane == 31) warp_sums[32] = e;
   }
   __syncthreads();
@@ -57,22 +63,22 @@ __device__ __forceinline__ T block_scan(T v, T* warp_sums, T* total) {
   return r;
 }
 
-__device__ __forceinline__ unsigned remote_u32(const unsigned* p, unsigned rank) {
-  unsigned v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(tc::mapa_shared(smem_addr(p), rank)) : "memory");
+__device__ __forceinline__ uint4 remote_u32x4(const unsigned* p, unsigned rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(tc::mapa_shared(smem_addr(p), rank)));
   return v;
 }
-
-// Sum of *p over the cluster's CTAs before this one; *total over all.
-__device__ __forceinline__ unsigned cluster_offset(const unsigned* p, unsigned rank, unsigned ctas, unsigned* total) {
-  unsigned before = 0, all = 0;
-  for (unsigned r = 0; r < ctas; ++r) {
-    const unsigned v = remote_u32(p, r);
-    before += r < rank ? v : 0;
-    all += v;
-  }
-  *total = all;
-  return before;
+__device__ __forceinline__ unsigned remote_u32(const unsigned* p, unsigned rank) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(tc::mapa_shared(smem_addr(p), rank)));
+  return v;
+}
+// The word at p in every CTA of the cluster (0 past the last), loads in flight together.
+__device__ __forceinline__ void remote_all(const unsigned* p, unsigned ctas, unsigned (&v)[kMaxCtas]) {
+#pragma unroll
+  for (int r = 0; r < kMaxCtas; ++r) v[r] = r < ctas ? remote_u32(p, r) : 0u;
 }
 
 // Larger = kept first.  -0 counts as +0, NaN below -infinity.
@@ -83,140 +89,321 @@ __device__ __forceinline__ unsigned slot_key(float w, int position, int first, l
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs a, int* ws, int cached_max) {
-  extern __shared__ unsigned cached[];
-  __shared__ unsigned hist[3][kBins];
-  __shared__ unsigned scan_u[33], found[2], tie_total, hole_total, mover_total, newest_s;
-  __shared__ unsigned long long scan_l[33];
+__device__ __forceinline__ void move_sums(const EvictArgs& a, int unit, int from, int to) {
+  a.weights_out[size_t(unit) * a.out_capacity + to] = a.weights[size_t(unit) * a.capacity + from];
+  a.positions_out[size_t(unit) * a.out_capacity + to] = a.positions[size_t(unit) * a.capacity + from];
+}
+
+// TILES: runs of kThreads slots per CTA, a slot per thread, their keys in
+// registers; 0: any number, keys made again from global memory each time.
+// Dynamic shared memory: counts [tiles * kWarps] (64 bits), then, with TILES,
+// the movers of the CTA [tiles * kThreads] and, to move, the slots that its rows come from.
+template <int TILES>
+__global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kernel(const EvictArgs a, int* ws, int tiles_by_capacity,
+                                                               bool move) {
+  extern __shared__ __align__(16) unsigned long long counts[];
+  int* const own_movers = reinterpret_cast<int*>(counts + tiles_by_capacity * kWarps);
+  int* const from_slot = own_movers + tiles_by_capacity * kThreads;
+  __shared__ __align__(16) unsigned hist[kBins];
+  __shared__ unsigned long long near_order[kRanked], scan_l[33], cut_s;
+  __shared__ unsigned scan_u[33], found[3], newest_s, listed, hole_total, mover_total;
+  static_assert(sizeof(hist) >= sizeof(near_order), "the histogram's memory takes the unit's list afterwards");
   const unsigned ctas = gridDim.x / (a.caches * a.kv_heads), rank = tc::cluster_ctarank();
-  const int unit = blockIdx.x / ctas, cache = unit / a.kv_heads, t = threadIdx.x;
-  allow_next();
+  const int unit = blockIdx.x / ctas, cache = unit / a.kv_heads, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  for (int i = t; i < kBins; i += kThreads) hist[i] = 0;
+  if (t == 0) {
+    newest_s = 0;
+    listed = 0;
+    cut_s = 0;
+  }
   wait_prior();
+  allow_next();
   const long long len = a.lengths[cache];
   const int n = int(len < 0 ? 0 : len > a.capacity ? a.capacity : len);
   const int keep = min(n, a.budget);
-  const int chunk = (n + ctas - 1) / ctas;
+  const int chunk = (n + ctas - 1) / ctas, tiles = (chunk + kThreads - 1) / kThreads;
   const int s0 = min(n, int(rank) * chunk), s1 = min(n, s0 + chunk);
   const float* weights = a.weights + size_t(unit) * a.capacity;
   const int* positions = a.positions + size_t(unit) * a.capacity;
   const bool all = n <= a.budget;  // nothing is evicted
-  const bool use_cache = chunk <= cached_max;
   auto sync = [&] {
     if (ctas > 1) tc::cluster_sync();
     else __syncthreads();
   };
-
-  long long recent_from = 0;
-  unsigned threshold = 0, need = 0;
-  if (!all) {
-    for (int i = t; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
-    int newest = INT_MIN;
-    for (int s = s0 + t; s < s1; s += kThreads) newest = max(newest, positions[s]);
-    newest = __reduce_max_sync(0xffffffffu, newest);
-    if (t == 0) newest_s = unsigned(INT_MIN);
-    __syncthreads();
-    if ((t & 31) == 0) atomicMax(reinterpret_cast<int*>(&newest_s), newest);
-    sync();
-    for (unsigned r = 0; r < ctas; ++r) newest = max(newest, int(remote_u32(&newest_s, r)));
-    recent_from = (long long)newest - a.recent;
-  }
-  auto key_at = [&](int s) {
-    return use_cache ? cached[s - s0] : slot_key(weights[s], positions[s], a.first, recent_from);
+  // f(e, slot) for this thread's slot of tile e, in slot order; with TILES also
+  // for tiles past the last one, whose slots are at or beyond s1.
+  auto each = [&](auto f) {
+    if constexpr (TILES > 0) {
+#pragma unroll
+      for (int e = 0; e < TILES; ++e) f(e, s0 + e * kThreads + t);
+    } else {
+      for (int e = 0; e < tiles; ++e) f(e, s0 + e * kThreads + t);
+    }
   };
+
+  constexpr int held = TILES ? TILES : 1;
+  unsigned keys[held];
+  long long recent_from = 0;
+  unsigned long long cut = 0;  // order of the last slot that stays
+  auto key_at = [&](int e, int s) {
+    return TILES ? keys[TILES ? e : 0] : slot_key(weights[s], positions[s], a.first, recent_from);
+  };
+  // Slots from first kept to first evicted: by key, then the lowest slot.
+  auto order = [](unsigned k, int s) { return (unsigned long long)k << 32 | (0xffffffffu - unsigned(s)); };
+  auto cut_of_all = [&] {  // one CTA of the cluster found it
+    unsigned v[kMaxCtas], u[kMaxCtas];
+    remote_all(reinterpret_cast<const unsigned*>(&cut_s), ctas, u);
+    remote_all(reinterpret_cast<const unsigned*>(&cut_s) + 1, ctas, v);
+    unsigned long long c = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCtas; ++r) c = max(c, (unsigned long long)v[r] << 32 | u[r]);
+    return c;
+  };
+  __syncthreads();
   if (!all) {
-    if (use_cache)
-      for (int s = s0 + t; s < s1; s += kThreads)
-        cached[s - s0] = slot_key(weights[s], positions[s], a.first, recent_from);
-    unsigned mask = 0;
-    need = keep;
+    // Positions as unsigned with the order of int, 0 where there is none.
+    unsigned newest = 0;
+    float w[held];
+    int pos[held];
+    each([&](int e, int s) {
+      if (s >= s1) return;
+      const int p = positions[s];
+      newest = max(newest, unsigned(p) ^ 0x80000000u);
+      if constexpr (TILES > 0) {
+        pos[e] = p;
+        w[e] = weights[s];
+      }
+    });
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) atomicMax(&newest_s, newest);
+    sync();
+    unsigned v[kMaxCtas];
+    remote_all(&newest_s, ctas, v);
+    for (int r = 0; r < kMaxCtas; ++r) newest = max(newest, v[r]);
+    recent_from = (long long)int(newest ^ 0x80000000u) - a.recent;
+    if constexpr (TILES > 0)
+      each([&](int e, int s) { keys[e] = s < s1 ? slot_key(w[e], pos[e], a.first, recent_from) : 0u; });
+
+    unsigned mask = 0, prefix = 0, need = keep, near = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const unsigned bins = pass == 2 ? 1024 : 2048;
-      for (int s = s0 + t; s < s1; s += kThreads) {  // its own cached keys: no barrier needed before
-        const unsigned k = key_at(s);
-        if ((k & mask) == threshold) atomicAdd(&hist[pass][(k >> shift) & (bins - 1)], 1u);
-      }
+      each([&](int e, int s) {
+        const unsigned k = s < s1 ? key_at(e, s) : 0u;
+        const bool in = s < s1 && (k & mask) == prefix;
+        // The two keys that many slots share, never looked at and protected,
+        // are counted per warp: adds to one word queue up.
+        const unsigned none = __ballot_sync(0xffffffffu, in && k == 0x80000000u);
+        const unsigned safe = __ballot_sync(0xffffffffu, in && k == 0xffffffffu);
+        if (in && (k != 0x80000000u || lane == __ffs(none) - 1) && (k != 0xffffffffu || lane == __ffs(safe) - 1))
+          atomicAdd(&hist[(k >> shift) & (bins - 1)],
+                    k == 0x80000000u ? __popc(none) : k == 0xffffffffu ? __popc(safe) : 1);
+      });
       sync();
-      // Bins from the top, two per thread; the bin where the count reaches `need`.
-      unsigned v[2] = {};
+      // Bins from the top, four per thread (one load from each CTA); the bin
+      // where the count reaches `need`.
+      unsigned c[4] = {};
+      const int top = int(bins) - 4 - 4 * t;
+      if (top >= 0) {
+        uint4 y[kMaxCtas];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (unsigned(2 * t + j) < bins)
-          for (unsigned r = 0; r < ctas; ++r) v[j] += remote_u32(&hist[pass][bins - 1 - (2 * t + j)], r);
-      unsigned total, before = block_scan(v[0] + v[1], scan_u, &total);
+        for (int r = 0; r < kMaxCtas; ++r) y[r] = r < ctas ? remote_u32x4(&hist[top], r) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (before < need && need <= before + v[j]) {
-          found[0] = bins - 1 - (2 * t + j);
-          found[1] = need - before;
+        for (int r = 0; r < kMaxCtas; ++r) {
+          c[0] += y[r].w;
+          c[1] += y[r].z;
+          c[2] += y[r].y;
+          c[3] += y[r].x;
         }
-        before += v[j];
       }
-      __syncthreads();
-      threshold |= found[0] << shift;
+      unsigned total, before = block_scan(c[0] + c[1] + c[2] + c[3], scan_u, &total);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before < need && need <= before + c[j]) {
+          found[0] = top + 3 - j;
+          found[1] = need - before;
+          found[2] = c[j];
+        }
+        before += c[j];
+      }
+      sync();  // also: every CTA has read every histogram
+      prefix |= found[0] << shift;
       need = found[1];
+      near = found[2];
       mask |= (bins - 1) << shift;
+      if (near <= kRanked || pass == 2) break;
+      for (int i = t; i < kBins; i += kThreads) hist[i] = 0;
       __syncthreads();
     }
+    if (near <= kRanked) {
+      each([&](int e, int s) {
+        if (s >= s1) return;
+        const unsigned k = key_at(e, s);
+        if ((k & mask) == prefix) near_order[atomicAdd(&listed, 1u)] = order(k, s);  // their ranks do not depend on it
+      });
+      sync();
+      // Every CTA ranks its own against the unit's.
+      unsigned long long* list = reinterpret_cast<unsigned long long*>(hist);
+      remote_all(&listed, ctas, v);
+      for (unsigned i = t; i < near; i += kThreads) {
+        unsigned j = i, r = 0;
+#pragma unroll
+        for (unsigned u = 0; u + 1 < kMaxCtas; ++u)
+          if (r == u && j >= v[u]) {
+            j -= v[u];
+            r = u + 1;
+          }
+        const unsigned* word = reinterpret_cast<const unsigned*>(&near_order[j]);
+        list[i] = (unsigned long long)remote_u32(word + 1, r) << 32 | remote_u32(word, r);
+      }
+      __syncthreads();
+      for (unsigned i = warp; i < listed; i += kWarps) {
+        const unsigned long long mine = near_order[i];
+        unsigned better = 0;
+        for (unsigned j = lane; j < near; j += 32) better += list[j] > mine;
+        better = __reduce_add_sync(0xffffffffu, better);
+        if (lane == 0 && better == need - 1) cut_s = mine;
+      }
+      sync();
+      cut = cut_of_all();
+    } else {  // more than kRanked equal keys: the need-th of them in slot order
+      each([&](int e, int s) {
+        const unsigned m = __ballot_sync(0xffffffffu, s < s1 && key_at(e, s) == prefix);
+        if (lane == 0 && e < tiles) counts[e * kWarps + warp] = __popc(m);
+      });
+      __syncthreads();
+      unsigned long long run = 0;
+      for (int i0 = 0; i0 < tiles * kWarps; i0 += kThreads) {
+        const int i = i0 + t;
+        unsigned long long total;
+        const unsigned long long x = block_scan(i < tiles * kWarps ? counts[i] : 0ull, scan_l, &total);
+        if (i < tiles * kWarps) counts[i] = run + x;
+        run += total;
+      }
+      if (t == 0) listed = unsigned(run);
+      sync();
+      remote_all(&listed, ctas, v);
+      unsigned before = 0;
+      for (unsigned r = 0; r < rank; ++r) before += remote_u32(&listed, r);
+      each([&](int e, int s) {
+        const bool tie = s < s1 && key_at(e, s) == prefix;
+        const unsigned m = __ballot_sync(0xffffffffu, tie);
+        if (tie && before + unsigned(counts[e * kWarps + warp]) + __popc(m & ((1u << lane) - 1)) == need - 1)
+          cut_s = order(prefix, s);
+      });
+      sync();
+      cut = cut_of_all();
+    }
   }
-  // Slot order from here on: thread t owns the slots [b0, b1); an odd count
-  // spreads neighbouring threads over the shared memory banks.
-  const int own = max(1, (chunk + kThreads - 1) / kThreads) | 1;
-  const int b0 = min(s1, s0 + t * own), b1 = min(s1, b0 + own);
-  unsigned ties = 0;
-  if (!all)
-    for (int s = b0; s < b1; ++s) ties += key_at(s) == threshold;
-  unsigned cta_ties, tie0 = block_scan(ties, scan_u, &cta_ties);
-  if (t == 0) tie_total = cta_ties;
-  sync();
-  unsigned unused;
-  tie0 += cluster_offset(&tie_total, rank, ctas, &unused);
-  // kept(s) for s walking upward; `tie` counts the ties passed.
-  auto kept = [&](int s, unsigned& tie) {
-    if (all) return true;
-    const unsigned k = key_at(s);
-    return k > threshold || (k == threshold && tie++ < need);
-  };
-  unsigned long long both = 0;  // holes, movers << 32
-  unsigned tie = tie0;
-  for (int s = b0; s < b1; ++s) {
-    const bool k = kept(s, tie);
-    if (s < keep) both += !k;
-    else both += (unsigned long long)(k) << 32;
+  auto stays = [&](int e, int s) { return all || order(key_at(e, s), s) >= cut; };
+  // Ranks of holes and movers: counts per (tile, warp), summed in slot order.
+  const int used = tiles * kWarps;
+  each([&](int e, int s) {
+    const bool in = s < s1, k = in && stays(e, s);
+    const unsigned h = __ballot_sync(0xffffffffu, in && s < keep && !k);
+    const unsigned m = __ballot_sync(0xffffffffu, in && s >= keep && k);
+    if (lane == 0 && e < tiles) counts[e * kWarps + warp] = __popc(h) | (unsigned long long)(__popc(m)) << 32;
+  });
+  __syncthreads();
+  unsigned long long run = 0;
+  for (int i0 = 0; i0 < used; i0 += kThreads) {
+    const int i = i0 + t;
+    unsigned long long total;
+    const unsigned long long x = block_scan(i < used ? counts[i] : 0ull, scan_l, &total);
+    if (i < used) counts[i] = run + x;
+    run += total;
   }
-  unsigned long long cta_both, rank0 = block_scan(both, scan_l, &cta_both);
   if (t == 0) {
-    hole_total = unsigned(cta_both);
-    mover_total = unsigned(cta_both >> 32);
+    hole_total = unsigned(run);
+    mover_total = unsigned(run >> 32);
   }
   sync();
-  unsigned holes, movers;
-  unsigned hole = unsigned(rank0) + cluster_offset(&hole_total, rank, ctas, &holes);
-  unsigned mover = unsigned(rank0 >> 32) + cluster_offset(&mover_total, rank, ctas, &movers);
-  int* dst = list_of(ws, unit, a.budget);
-  int *src = dst + a.budget, *mov = src + a.budget;
-  tie = tie0;
-  for (int s = b0; s < b1; ++s)
-    if (kept(s, tie) && s >= keep) mov[mover++] = s;
-  __threadfence();
-  sync();  // every mover of the unit is listed; no CTA reads another's shared memory after this
-  float* weights_out = a.weights_out + size_t(unit) * a.out_capacity;
-  int* positions_out = a.positions_out + size_t(unit) * a.out_capacity;
-  tie = tie0;
-  for (int s = b0; s < b1 && s < keep; ++s) {
-    const bool stays = kept(s, tie);
-    const int from = stays ? s : __ldcg(mov + hole);
-    const int entry = a.in_place ? int(hole) : s;
-    hole += !stays;
-    if (stays && a.in_place) continue;
-    dst[entry] = s;
-    src[entry] = from;
-    weights_out[s] = weights[from];
-    positions_out[s] = positions[from];
+  unsigned hole0 = 0, mover0 = 0, holes = 0, movers[kMaxCtas];
+  {
+    unsigned h[kMaxCtas];
+    remote_all(&hole_total, ctas, h);
+    remote_all(&mover_total, ctas, movers);
+#pragma unroll
+    for (unsigned r = 0; r < kMaxCtas; ++r) {
+      hole0 += r < rank ? h[r] : 0;
+      mover0 += r < rank ? movers[r] : 0;
+      holes += h[r];
+    }
   }
-  if (rank == 0 && t == 0)
-    list_of(ws, a.caches * a.kv_heads, a.budget)[unit] = a.in_place ? int(holes) : keep;
+  // Movers in slot order: each CTA's in its shared memory (with TILES), or the
+  // unit's in global memory.
+  int* dst = list_of(ws, unit, a.budget);
+  int *src = dst + a.budget, *mov = TILES ? own_movers : src + a.budget + mover0;
+  each([&](int e, int s) {
+    const bool mover = s < s1 && s >= keep && stays(e, s);
+    const unsigned m = __ballot_sync(0xffffffffu, mover);
+    if (mover) mov[unsigned(counts[e * kWarps + warp] >> 32) + __popc(m & ((1u << lane) - 1))] = s;
+  });
+  if (!TILES) __threadfence();
+  sync();  // every mover of the unit is listed
+  auto mover_at = [&](unsigned i) {
+    if constexpr (TILES > 0) {
+      unsigned r = 0;
+#pragma unroll
+      for (unsigned u = 0; u + 1 < kMaxCtas; ++u)
+        if (r == u && i >= movers[u]) {
+          i -= movers[u];
+          r = u + 1;
+        }
+      return int(remote_u32(reinterpret_cast<const unsigned*>(own_movers) + i, r));
+    } else {
+      return *reinterpret_cast<volatile int*>(src + a.budget + i);
+    }
+  };
+  each([&](int e, int s) {
+    const bool in = s < s1 && s < keep, k = in && stays(e, s);
+    const unsigned h = __ballot_sync(0xffffffffu, in && !k);
+    if (!in) return;
+    const unsigned hole = hole0 + unsigned(counts[e * kWarps + warp]) + __popc(h & ((1u << lane) - 1));
+    const int from = k ? s : mover_at(hole);
+    if (move) {
+      from_slot[s - s0] = k && a.in_place ? -1 : from;
+    } else if (!k && a.in_place) {
+      dst[hole] = s;
+      src[hole] = from;
+    } else if (!a.in_place) {
+      src[s] = from;  // its destination is s
+    }
+  });
+  if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
+  if (!move) {
+    if (rank == 0 && t == 0)
+      list_of(ws, a.caches * a.kv_heads, a.budget)[unit] = a.in_place ? int(holes) : keep;
+    return;
+  }
+  const int h = unit % a.kv_heads;
+  if (rank == 0 && h == 0 && t == 0) a.lengths_out[cache] = keep;  // not the input lengths: see the launch
+  __syncthreads();
+  const int rows = max(0, min(s1, keep) - s0), pieces = a.width / 4;  // 16-byte pieces of a row's key, then its value
+  constexpr int kAhead = 4;
+  for (int row = t; row < rows; row += kThreads)
+    if (from_slot[row] >= 0) move_sums(a, unit, from_slot[row], s0 + row);
+#pragma unroll 1
+  for (int i0 = 0; i0 < rows * pieces; i0 += kAhead * kThreads) {
+    uint4 v[kAhead];
+    uint4* to[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kThreads + t, row = i / pieces, p = i % pieces, c = p % (pieces / 2);
+      const bool val = p >= pieces / 2;
+      to[j] = nullptr;
+      if (i >= rows * pieces || from_slot[row] < 0) continue;
+      const size_t from = size_t(cache) * a.cache_stride + size_t(from_slot[row]) * a.row_stride + size_t(h) * a.width;
+      const size_t into =
+          size_t(cache) * a.out_cache_stride + size_t(s0 + row) * a.out_row_stride + size_t(h) * a.width;
+      v[j] = reinterpret_cast<const uint4*>((val ? a.value : a.key) + from)[c];
+      to[j] = reinterpret_cast<uint4*>((val ? a.value_out : a.key_out) + into) + c;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (to[j]) *to[j] = v[j];
+  }
 }
 
 // Block (KV head fastest, then a run of entries, then the cache): the heads'
@@ -237,6 +424,12 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
   const long long count = (long long)list_of(ws, a.caches * a.kv_heads, a.budget)[unit] * pieces;
   const int* dst = list_of(ws, unit, a.budget);
   const int* src = dst + a.budget;
+  // The weights and positions of the entries whose first piece is this block's.
+  constexpr int span = kPieces * kMoveThreads;
+  const long long e1 = ((long long)(run + 1) * span + pieces - 1) / pieces;
+  for (long long e = ((long long)run * span + pieces - 1) / pieces + threadIdx.x; e < e1 && e * pieces < count;
+       e += kMoveThreads)
+    move_sums(a, unit, src[e], a.in_place ? dst[e] : int(e));
   uint4 v[kPieces];
   uint4* to[kPieces];
 #pragma unroll
@@ -246,8 +439,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
     if (i >= count) continue;
     const int e = int(i / pieces), p = int(i % pieces), c = p % (pieces / 2);
     const bool val = p >= pieces / 2;
-    const size_t from = size_t(cache) * a.cache_stride + size_t(src[e]) * a.row_stride + size_t(h) * a.width;
-    const size_t into = size_t(cache) * a.out_cache_stride + size_t(dst[e]) * a.out_row_stride + size_t(h) * a.width;
+    const int source = src[e], slot = a.in_place ? dst[e] : e;
+    const size_t from = size_t(cache) * a.cache_stride + size_t(source) * a.row_stride + size_t(h) * a.width;
+    const size_t into = size_t(cache) * a.out_cache_stride + size_t(slot) * a.out_row_stride + size_t(h) * a.width;
     v[j] = reinterpret_cast<const uint4*>((val ? a.value : a.key) + from)[c];
     to[j] = reinterpret_cast<uint4*>((val ? a.value_out : a.key_out) + into) + c;
   }
@@ -262,43 +456,62 @@ size_t cache_evict_workspace_bytes(int caches, int kv_heads, int budget) {
   return size_t(caches) * kv_heads * (3 * size_t(budget) + 1) * 4;
 }
 
-cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, cudaStream_t stream) {
+int cache_evict_most_slots() { return kMaxCtas * kMostTiles * kThreads; }
+
+cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cudaStream_t stream) {
   const int units = a.caches * a.kv_heads;
   int ctas = 1;
-  while (ctas < 8 && a.capacity > 4096 * ctas) ctas *= 2;
-  const int cached = std::min((a.capacity + ctas - 1) / ctas, kMaxCached);
-  if (cached > 4096) {  // beyond the 48 KB that need no opt-in (a setting of the current device)
-    const cudaError_t s = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kMaxCached * 4);
-    if (s != cudaSuccess) return s;
-  }
+  while (ctas < kMaxCtas && a.capacity > 8 * kThreads * ctas) ctas *= 2;
+  const int tiles = (a.capacity + ctas * kThreads - 1) / (ctas * kThreads);
+  // Moving in the selecting CTAs saves the second kernel's start (2 us) while
+  // they are few rows each and one wave; not when the lengths are updated in
+  // place, since a CTA of another head may still have to read them.
+  const int own_rows = std::min(a.budget, tiles * kThreads);
+  const size_t bytes = size_t(own_rows) * a.width * 4;
+  const bool move =
+      tiles <= 8 && bytes <= (size_t(256) << 10) && units * ctas <= 2 * sms && a.lengths_out != a.lengths;
+  const size_t smem = size_t(tiles) * kWarps * 8 + (tiles <= 32 ? size_t(tiles) * kThreads * 4 : 0) +
+                      (move ? size_t(own_rows) * 4 : 0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units * ctas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = size_t(cached) * 4;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int* ws = static_cast<int*>(workspace);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a, ws, cached);
-  if (e != cudaSuccess) return e;
-  const int pieces = 2 * (a.width / 8);
-  const int runs = int((size_t(a.budget) * pieces + kMoveThreads * kPieces - 1) / (kMoveThreads * kPieces));
-  cudaLaunchConfig_t mv = {};
-  mv.gridDim = dim3(unsigned(units) * runs);
-  mv.blockDim = dim3(kMoveThreads);
-  mv.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  mv.attrs = attr;
-  mv.numAttrs = 1;
-  if (a.width == 128) return cudaLaunchKernelEx(&mv, evict_move_kernel<16>, a, ws, runs);
-  if (a.width == 64) return cudaLaunchKernelEx(&mv, evict_move_kernel<8>, a, ws, runs);
-  return cudaLaunchKernelEx(&mv, evict_move_kernel<0>, a, ws, runs);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  int* ws = static_cast<int*>(workspace);
+  cudaError_t e;
+  if (tiles <= 1) {
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<1>, a, ws, tiles, move);
+  } else if (tiles <= 8) {
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a, ws, tiles, move);
+  } else if (tiles <= 32) {  // up to 68 KB: an opt-in of the current device
+    e = cudaFuncSetAttribute(evict_select_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             32 * (kWarps * 8 + kThreads * 4));
+    if (e != cudaSuccess) return e;
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<32>, a, ws, tiles, move);
+  } else {
+    e = cudaFuncSetAttribute(evict_select_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMostTiles * kWarps * 8);
+    if (e != cudaSuccess) return e;
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<0>, a, ws, tiles, move);
+  }
+  if (e != cudaSuccess || move) return e;
+  const int pieces = 2 * (a.width / 8);
+  const int runs = int((size_t(a.budget) * pieces + kMoveThreads * kPieces - 1) / (kMoveThreads * kPieces));
+  cfg.gridDim = dim3(unsigned(units) * runs);
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  if (a.width == 128) return cudaLaunchKernelEx(&cfg, evict_move_kernel<16>, a, ws, runs);
+  if (a.width == 64) return cudaLaunchKernelEx(&cfg, evict_move_kernel<8>, a, ws, runs);
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel<0>, a, ws, runs);
 }
 
 }  // namespace dl

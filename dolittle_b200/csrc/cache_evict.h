@@ -23,6 +23,7 @@ struct EvictArgs {
 };
 
 size_t cache_evict_workspace_bytes(int caches, int kv_heads, int budget);
-cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, cudaStream_t stream);
+int cache_evict_most_slots();  // of one (cache, KV head)
+cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cudaStream_t stream);
 
 }  // namespace dl

@@ -888,7 +888,9 @@ dl_status evict_args(const dl_cache_eviction* e, dl::EvictArgs* o) {
   if (e->width % 8 || (e->row_stride | e->cache_stride | e->out_row_stride | e->out_cache_stride) % 8)
     return fail(DL_UNSUPPORTED, "cache evict: width and strides must be multiples of 8");
   const size_t most = size_t(1) << 30;
-  if (e->width > 1024 || e->caches > most / e->kv_heads || e->capacity > most || e->out_capacity > most ||
+  if (e->capacity > size_t(dl::cache_evict_most_slots()))
+    return fail(DL_UNSUPPORTED, "cache evict: more than 4194304 slots");
+  if (e->width > 1024 || e->caches > most / e->kv_heads || e->out_capacity > most ||
       e->caches * e->kv_heads > most / (budget * e->width / 4096 + 1))
     return fail(DL_UNSUPPORTED, "cache evict: size out of range");
   if (e->row_stride < e->kv_heads * e->width || e->out_row_stride < e->kv_heads * e->width)
@@ -974,7 +976,7 @@ DL_API dl_status dl_cache_evict(const dl_cache_eviction* e, void* workspace, voi
         overlap(e->weights_out, out4, e->weights, in4) || overlap(e->positions_out, out4, e->positions, in4))
       return fail(DL_INVALID_ARGUMENT, "cache evict: outputs overlap the inputs without being them");
   }
-  return cuda_status(dl::launch_cache_evict(o, workspace, st(stream)), "cache evict");
+  return cuda_status(dl::launch_cache_evict(o, workspace, device_sms(), st(stream)), "cache evict");
 }
 
 }  // extern "C"

@@ -378,6 +378,9 @@ EVICTIONS = [
     (3, 100, None, 200, 2, 2, 2, 64),        # a budget above the capacity evicts nothing
     (2, 64, None, 7, 0, 7, 2, 24),           # every kept slot protected, an unusual width
     (2, 130, [1 << 40, -5], 100, 3, 10, 2, 64),
+    (1, 9000, [4097], 2048, 0, 0, 2, 8),     # a cluster whose last blocks hold few slots
+    (1, 70000, None, 30000, 2, 3, 1, 8),
+    (1, 200000, [150001], 66000, 0, 9, 1, 8),
 ]
 
 
@@ -398,6 +401,33 @@ def test_eviction_of_ties_and_special_weights(in_place):
     w[:, 4::7], w[:, 5::7], w[:, 6::7] = -math.inf, 1e-40, -2.5
     c["weights"][2] = torch.randint(0, 4, (2, 700), device="cuda").float()
     check_eviction(c, 300, 5, 40, in_place)
+
+
+@pytest.mark.parametrize("n,capacity,budget", [(2, 1000, 600), (1, 4000, 999), (1, 20000, 12345), (1, 80000, 40001),
+                                               (1, 140000, 70001)])
+def test_eviction_of_equal_weights(n, capacity, budget):
+    """More equal keys than are ranked one by one: the lowest slots stay."""
+    c = make_caches(n, capacity, 1, 8, seed=capacity)
+    c["weights"][:] = 0.5
+    c["weights"][:, :, capacity // 2::3] = 0.25
+    check_eviction(c, budget, 0, 17, True)
+
+
+def test_eviction_in_place_with_lengths_of_its_own():
+    """In place for the caches, the new lengths elsewhere; then both out of place."""
+    for in_place in (True, False):
+        c = make_caches(3, 300, 4, 64, seed=8, lengths=[300, 200, 129])
+        d = {k: v.clone() for k, v in c.items()}
+        want = shared.cache_evict(*[d[k] for k in ("key", "value", "weights", "positions", "lengths")], 128, recent=9)
+        fresh = torch.zeros_like(c["lengths"])
+        args = [c[k] for k in ("key", "value", "weights", "positions")]
+        out = [x if in_place else torch.zeros_like(x) for x in args]
+        got = shared.cache_evict(*args, c["lengths"], 128, recent=9, out=[*out, fresh])
+        assert c["lengths"].tolist() == [300, 200, 129] and fresh.tolist() == [128, 128, 128]
+        for x, y in zip(got[:2], want[:2]):
+            assert torch.equal(x[:, :128], y[:, :128])
+        for x, y in zip(got[2:4], want[2:4]):
+            assert torch.equal(x[..., :128], y[..., :128])
 
 
 def test_eviction_drops_nan_only_when_it_must():
