@@ -134,6 +134,7 @@ SIGNATURES = {
     "dl_engine_set_reconstruction_head": (C.c_int, [vp, u16p]),
     "dl_engine_reconstruct": (C.c_int, [vp, u32p, sz, u16p]),
     "dl_engine_read_kv": (C.c_int, [vp, sz, C.c_int, sz, sz, u16p]),
+    "dl_engine_kv_device": (C.c_int, [vp, sz, C.c_int, C.POINTER(vp), C.POINTER(sz)]),
     "dl_engine_generate": (C.c_int, [vp, u32p, sz, sz, C.POINTER(Sampling), C.c_uint64, u32p, sz, C.c_int,
                                      u32p, C.POINTER(sz), u16p, C.POINTER(GenerationStats)]),
     "dl_engine_start": (C.c_int, [vp, u32p, sz, sz, C.POINTER(Sampling), C.c_uint64, u32p, sz, C.c_int]),

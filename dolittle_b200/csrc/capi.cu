@@ -586,6 +586,11 @@ DL_API dl_status dl_engine_read_kv(dl_engine* e, size_t layer, int values, size_
                                    uint16_t* host) {
   DL_ENGINE_CALL(e->impl->read_kv(layer, values, first, count, host));
 }
+DL_API dl_status dl_engine_kv_device(dl_engine* e, size_t layer, int values, const void** device_ptr,
+                                     size_t* row_stride) {
+  if (!device_ptr) return fail(DL_INVALID_ARGUMENT, "kv_device: null output");
+  DL_ENGINE_CALL(*device_ptr = e->impl->kv_device(layer, values, row_stride));
+}
 DL_API dl_status dl_engine_generate(dl_engine* e, const uint32_t* prompt, size_t n_prompt, size_t max_new,
                                     const dl_sampling* settings, uint64_t seed, const uint32_t* stop_ids,
                                     size_t n_stop, int prefill_mode, uint32_t* tokens_out, size_t* n_out,
@@ -812,10 +817,11 @@ bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0
 
 int device_sms() {
   static std::atomic<int> known[64];  // by device ordinal
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64) sms = known[dev].load(std::memory_order_relaxed);
+  if (sms > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return 148;
   if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }

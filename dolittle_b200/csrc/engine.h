@@ -66,6 +66,11 @@ class Engine {
   void read_capture(size_t first, size_t count, uint16_t* host);
   void set_observation(void* device_rows, size_t positions);
   void set_intervention(int layer, size_t selected, float strength, const float* direction);
+  const void* kv_device(size_t layer, int values, size_t* row_stride) const {
+    if (layer >= layers_.size()) throw std::invalid_argument("kv layer");
+    if (row_stride) *row_stride = size_t(cfg_.kv_heads) * cfg_.head_width;
+    return values ? vcache_[layer] : kcache_[layer];
+  }
   void read_kv(size_t layer, int values, size_t first, size_t count, uint16_t* host);
   void set_injection(long long position, const uint16_t* source_bits, float scale);
   void set_reconstruction_head(const uint16_t* host_bits);

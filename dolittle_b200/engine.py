@@ -203,6 +203,13 @@ class Engine:
         check(lib().dl_engine_read_kv(self._h, layer, int(values), first, count, out.ctypes.data_as(_lib.u16p)))
         return out
 
+    def kv_device(self, layer: int, values: bool) -> tuple:
+        """(device address, elements between positions) of a block's key or
+        value cache [capacity][Hkv][d]."""
+        p, s = C.c_void_p(), C.c_size_t()
+        check(lib().dl_engine_kv_device(self._h, layer, int(values), C.byref(p), C.byref(s)))
+        return int(p.value), int(s.value)
+
     # ---- device-side sequence loop (DeviceSequence) ---------------------
     def start(self, prompt, max_new: int, settings: Settings | None = None, seed: int = 0, stop_ids=(),
               prefill: int = _lib.DL_PREFILL_PARITY) -> None:

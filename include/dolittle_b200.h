@@ -337,6 +337,13 @@ DL_API dl_status dl_engine_set_reconstruction_head(dl_engine* e, const uint16_t*
 DL_API dl_status dl_engine_reconstruct(dl_engine* e, const uint32_t* tokens, size_t n, uint16_t* out_bits);
 DL_API dl_status dl_engine_read_kv(dl_engine* e, size_t layer, int values, size_t first,
                                    size_t count, uint16_t* host);
+/* Device address of block `layer`'s key (values = 0) or value cache,
+ * [capacity][Hkv][d] with *row_stride elements between positions; rows below
+ * dl_engine_position() are valid once the stream work that wrote them (a
+ * finished consume or generate call) is complete.  A prefix for
+ * dl_attention_shared as it stands. */
+DL_API dl_status dl_engine_kv_device(dl_engine* e, size_t layer, int values, const void** device_ptr,
+                                     size_t* row_stride);
 /* Live generation: prompt pass, first selection, then decode steps replayed
  * from one captured CUDA graph per step until max_new tokens or a stop ID.
  * tokens_out receives the generated IDs (host); logits_out (optional, host,

@@ -1,0 +1,101 @@
+"""Branches of one prompt against an engine that runs each branch by itself,
+and caches cut by accumulated weight against what the definition keeps."""
+import numpy as np
+import pytest
+import torch
+
+import dolittle_b200 as dl
+from dolittle_b200.branches import Branches
+from tests import numerics as nm
+
+pytestmark = pytest.mark.gpu
+
+CONFIG = dl.Qwen3Config(hidden=512, query_heads=8, kv_heads=2, head_width=128, mlp_width=1024, vocabulary=1024, layers=3,
+                        theta=1e6)
+
+
+def engine(capacity=512):
+    e = dl.Engine(CONFIG, capacity=capacity, max_rows=64)
+    e.init_random(3, 0.05)
+    return e
+
+
+def close(got, bits, what):
+    """BF16 logits within the tolerance that the fast paths are held to elsewhere."""
+    ours = got.float().cpu().numpy()
+    theirs = nm.bf16_bits_to_f32(bits)
+    peak = float(np.max(np.abs(theirs)))
+    r = nm.compare_values(theirs, ours, max(1e-4, 0.0625 * peak), 0.03)
+    assert r["passed"] and nm.cosine(theirs, ours) > 0.999, (what, r)
+
+
+@pytest.mark.parametrize("batch,prompt,turns", [(1, 40, [1, 1]), (3, 150, [1, 5, 1]), (16, 64, [1] * 6), (2, 300, [40, 1])])
+def test_branches_match_separate_sequences(batch, prompt, turns):
+    rng = np.random.default_rng(batch)
+    ids = rng.integers(0, CONFIG.vocabulary, prompt)
+    e, alone = engine(), engine()
+    e.consume_view(ids)
+    b = Branches(e, batch, sum(turns) + 3, weights=batch == 3)
+    new = rng.integers(0, CONFIG.vocabulary, (batch, sum(turns)))
+    at = 0
+    for rows in turns:
+        logits = b.step(torch.from_numpy(new[:, at:at + rows]).cuda())
+        at += rows
+        for s in range(batch):
+            alone.reset()
+            close(logits[s], alone.consume_view(np.concatenate([ids, new[s, :at]])), (at, s))
+    if batch == 3:  # every row's weights sum to one
+        total = sum(w.sum().item() for w in b.prefix_weights) + b.suffix_weights.sum().item()
+        assert abs(total - CONFIG.layers * batch * at * CONFIG.query_heads) < 1e-3 * total
+
+
+def test_evicted_branches_attend_what_is_left():
+    """A cut of the prompt and of the branches' own caches keeps exactly the
+    slots the definition names, and steps go on over what is left."""
+    rng = np.random.default_rng(1)
+    batch, prompt = 4, 200
+    ids = rng.integers(0, CONFIG.vocabulary, prompt)
+    e = engine()
+    e.consume_view(ids)
+    b = Branches(e, batch, 64, weights=True)
+    for _ in range(24):
+        b.step(torch.from_numpy(rng.integers(0, CONFIG.vocabulary, batch)).cuda())
+    sums = [w.clone() for w in b.prefix_weights]
+    own = b.suffix_weights.clone()
+    keys = [(k.clone(), v.clone()) for k, v in b._prefix]
+    b.evict_prefix(64, first=4, recent=16)
+    b.evict_suffix(12, recent=4)
+    assert b.prefix == 64 and b.length == 12 and b.position == prompt + 24
+    assert b._suffix_lengths.tolist() == [12] * batch
+    for layer in range(CONFIG.layers):
+        for h in range(CONFIG.kv_heads):
+            held = b._prefix_positions[layer][0, h].long()
+            middle = sums[layer][h, 4:184].topk(64 - 20).indices + 4
+            assert set(held.tolist()) == set(range(4)) | set(range(184, 200)) | set(middle.tolist())
+            assert torch.equal(b._prefix[layer][0][:, h], keys[layer][0][held, h])
+            assert torch.equal(b._prefix[layer][1][:, h], keys[layer][1][held, h])
+            for s in range(batch):
+                held = b._suffix_positions[layer, s, h, :12].long() - prompt
+                best = own[layer, s, h, :20].topk(8).indices
+                assert set(held.tolist()) == set(range(20, 24)) | set(best.tolist()), (layer, h, s)
+    logits = b.step(torch.from_numpy(rng.integers(0, CONFIG.vocabulary, batch)).cuda())
+    assert bool(torch.isfinite(logits.float()).all()) and b.length == 13
+    # The prompt's cut is the branches' own copy: the engine's cache is untouched.
+    again = Branches(e, 1, 4)
+    assert all(torch.equal(x[0], y[0]) and torch.equal(x[1], y[1]) for x, y in zip(again._prefix, keys))
+
+
+def test_refusals():
+    e = engine(64)
+    with pytest.raises(ValueError):
+        Branches(e, 2, 8)  # nothing consumed yet
+    e.consume_view([1, 2, 3])
+    b = Branches(e, 2, 2)
+    with pytest.raises(ValueError):
+        b.step(torch.zeros(3, 1, dtype=torch.int64).cuda())
+    with pytest.raises(ValueError):
+        b.step(torch.zeros(2, 3, dtype=torch.int64).cuda())
+    with pytest.raises(ValueError):
+        b.evict_prefix(2)  # no weights were summed
+    with pytest.raises(dl.DolittleError):
+        e.kv_device(99, False)
