@@ -73,9 +73,10 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
   p.suffix_splits = p.pooled ? suffix_splits(units, unit_keys, 3 * sms) : 1;
   p.weight_ranks = 1;
   if (weights) {
-    const long long key_units = (long long)(prefix_tiles + (p.pooled ? 0 : suffix_tiles * a.batch)) * a.kv_heads;
+    const long long key_units =  // pairs of key tiles
+        ((prefix_tiles + 1) / 2 + (long long)(p.pooled ? 0 : (suffix_tiles + 1) / 2) * a.batch) * a.kv_heads;
     const int row_tiles = (tokens + p.per_tile - 1) / p.per_tile;
-    while (p.weight_ranks < 8 && key_units * p.weight_ranks < sms && row_tiles >= 2 * p.weight_ranks)
+    while (p.weight_ranks < 8 && key_units * p.weight_ranks * 2 <= sms && row_tiles >= 2 * p.weight_ranks)
       p.weight_ranks *= 2;
   }
   return p;
@@ -119,7 +120,7 @@ cudaError_t launch_shared_attention(const SharedAttnArgs& a, void* workspace, in
   if (e == cudaSuccess && p.pooled) e = launch_rows(a, p, ws, stream);
   if (e == cudaSuccess && p.pooled && p.splits) e = launch_join(a, p, ws, stream);
   if (e == cudaSuccess && !p.pooled && p.full < p.tasks) e = launch_merge(a, p, ws, stream);
-  if (e == cudaSuccess && (a.pw || (a.sw && !p.pooled))) e = launch_weights(a, p, ws, stream);
+  if (e == cudaSuccess && (a.pw || (a.sw && !p.pooled))) e = launch_weights(a, p, ws, sms, stream);
   return e;
 }
 

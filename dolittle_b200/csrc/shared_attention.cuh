@@ -50,14 +50,14 @@ struct Plan {
   int full;       // tasks done whole, by the first CTAs; the rest are cut into key ranges
   int splits;     // key ranges of the rest (0: no tile kernel; the few-row kernel reads the prefix too)
   int suffix_splits;  // CTAs (a cluster if there is no tile kernel) per sequence and KV head in the few-row kernel
-  int weight_ranks;   // CTAs (one cluster) per key tile in the weights kernel
+  int weight_ranks;   // CTAs (one cluster) per pair of key tiles in the weights kernel
 };
 
 cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
-cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream);
 
 // Launch configuration of a programmatic dependent launch (every kernel here
 // waits for its predecessor before it touches global memory).

@@ -2,17 +2,21 @@
 //
 // The rows' norms are known by then, so a key's sum needs its scores once more
 // and nothing else: weight = exp2(s * scale - m[row]) * r[row].  One CTA takes
-// 128 keys of one KV head and walks the query rows in tiles of up to 128,
+// 256 keys of one KV head and walks the query rows in tiles of up to 128,
 //
-//   S^T [128 keys x 128 rows] = K Q^T   (tcgen05, both K-major)
+//   S^T [2 x 128 keys x 128 rows] = K Q^T   (tcgen05, both K-major)
 //
-// with the keys as TMEM lanes: a thread owns one key and adds up its row of
-// S^T in order, with no exchange between threads and no atomics.  Scores and
-// queries are double-buffered, so the next product runs under the sums.  When
-// there are few key tiles, a cluster shares the rows of one and rank 0 adds
-// the ranks' sums in order.  The keys were just read by the attention, so they
-// come from L2 while the caches fit it.
+// with the keys as TMEM lanes: two threads own a key and add up half of its row
+// of S^T each, in order, joined at the end: no exchange in between, no atomics.
+// The exponentials bound it (16 per cycle and SM): sixteen warps cover one
+// another's latencies, two key tiles share each query tile that comes through
+// L2, scores and queries are double-buffered, and the next key tiles load under
+// the sums of the ones before.  When there are few key tiles, a cluster shares
+// the rows of a pair and rank 0 adds the ranks' sums in order.  The keys were
+// just read by the attention, so they come from L2 while the caches fit it.
 #include "shared_attention.cuh"
+
+#include <algorithm>
 
 namespace dl {
 namespace sa {
@@ -20,54 +24,68 @@ namespace {
 
 using namespace tc;
 
-constexpr int kThreads = 160;  // 4 warps of keys, one that loads and issues
+constexpr int kPair = 2 * kKeys;      // keys of a unit
+constexpr int kWork = 2 * kPair;      // threads that sum, two per key
+constexpr int kThreads = kWork + 32;  // and a warp that loads and issues
+constexpr int kIssueWarp = kWork / 32;
 constexpr int kAtom = kKeys * 128;
-constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kTmemCols = 512;  // scores: [key tile][buffer]
 
 struct alignas(64) WeightArgs {
   CUtensorMap q, pk, sk;
   SharedAttnArgs a;
   const RowNorm* norm;
-  int per_tile, prefix_tiles, suffix_tiles, ranks;  // key tiles by capacity; CTAs per key tile
+  int per_tile, prefix_pairs, suffix_pairs, ranks;  // pairs of key tiles by capacity; CTAs per pair
+  int units;                                        // pairs x KV heads (x sequences)
   float scale_log2;
 };
 
+// A pair of key tiles of one KV head and the row tiles [i0, i0 + n) that this
+// CTA takes it through: of all tokens for a prefix key, of the sequence's rows
+// that can see the first tile for a suffix key.
+struct Unit {
+  bool suffix;
+  int h, b, j0, tokens, token0, i0, n, span;
+  int longest, shortest;  // prefix lengths of all sequences; a suffix's own
+};
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) shared_weights_kernel(const __grid_constant__ WeightArgs w) {
+__global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __grid_constant__ WeightArgs w) {
   constexpr int slot = D / 64 * kAtom;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t k_full, q_full[2], q_free[2], s_full[2], s_free[2];
+  __shared__ uint64_t k_full[2], q_full[2], q_free[2], s_full[2][2], s_free[2][2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed_s, whole[2][4];
-  __shared__ __align__(16) RowNorm norms[2][kRows];
-  __shared__ int seen_s[2][kRows];
-  __shared__ float sums[kKeys];
+  __shared__ int failed_s;
+  __shared__ __align__(16) RowNorm norms[2][2][kRows];
+  __shared__ int seen_s[2][2][kRows];
+  __shared__ float sums[kWork];
   volatile int* failed = &failed_s;
   const SharedAttnArgs& a = w.a;
-  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;  // K, then two query tiles
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;  // two pairs of key tiles, two query tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned rank = cluster_ctarank();
 
-  int at = blockIdx.x / w.ranks;
-  const bool suffix = at >= w.prefix_tiles * a.kv_heads;
-  if (suffix) at -= w.prefix_tiles * a.kv_heads;
-  const int h = at % a.kv_heads;
-  at /= a.kv_heads;
-  const int tile = suffix ? at % w.suffix_tiles : at, b = suffix ? at / w.suffix_tiles : 0;
-  const int j0 = tile * kKeys;
-
   if (threadIdx.x == 0) {
-    mbar_init(&k_full, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
       mbar_init(&q_full[i], 1);
       mbar_init(&q_free[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], kKeys);
+      for (int p = 0; p < 2; ++p) {
+        mbar_init(&s_full[p][i], 1);
+        mbar_init(&s_free[p][i], kPair / 32);
+      }
     }
     failed_s = 0;
     fence_barrier_init();
   }
-  if (warp == 4) tmem_alloc(&tmem_slot, kTmemCols);
+  if (warp == kIssueWarp) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    if (lane == 0) {
+      prefetch_map(&w.q);
+      if (w.prefix_pairs) prefetch_map(&w.pk);
+      if (w.suffix_pairs) prefetch_map(&w.sk);
+    }
+  }
   wait_prior();
   allow_next();
   fence_before_sync();
@@ -75,183 +93,295 @@ __global__ void __launch_bounds__(kThreads) shared_weights_kernel(const __grid_c
   fence_after_sync();
   const uint32_t tmem = tmem_slot;
 
-  // Row tiles of this CTA: all tokens for a prefix key, the sequence's rows
-  // that can see the tile for a suffix key.
-  const int tokens = suffix ? a.rows : a.batch * a.rows, token0 = suffix ? b * a.rows : 0;
-  int row_tiles = (tokens + w.per_tile - 1) / w.per_tile, first = 0;
-  if (suffix) {
-    const int n = suffix_len(a, b);
-    if (j0 >= n) row_tiles = 0;
-    first = max(0, j0 - n + a.rows) / w.per_tile;
-  } else {
-    int longest = 0;
-    for (int s = lane; s < a.batch; s += 32) longest = max(longest, prefix_len(a, s));
-    if (j0 >= __reduce_max_sync(0xffffffffu, longest)) row_tiles = 0;
+  int longest = 0, shortest = a.pcap;
+  for (int s = lane; s < a.batch; s += 32) {
+    const int l = prefix_len(a, s);
+    longest = max(longest, l);
+    shortest = min(shortest, l);
   }
-  const int span = max(0, row_tiles - first);
-  const int i0 = first + int((long long)span * rank / w.ranks);
-  const int n = first + int((long long)span * (rank + 1) / w.ranks) - i0;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  shortest = __reduce_min_sync(0xffffffffu, shortest);
+  auto unit_of = [&](int at) {
+    Unit u;
+    u.suffix = at >= w.prefix_pairs * a.kv_heads;
+    if (u.suffix) at -= w.prefix_pairs * a.kv_heads;
+    u.h = at % a.kv_heads;
+    at /= a.kv_heads;
+    u.b = u.suffix ? at / w.suffix_pairs : 0;
+    u.j0 = (u.suffix ? at % w.suffix_pairs : at) * kPair;
+    u.tokens = u.suffix ? a.rows : a.batch * a.rows;
+    u.token0 = u.suffix ? u.b * a.rows : 0;
+    u.longest = u.suffix ? suffix_len(a, u.b) : longest;
+    u.shortest = shortest;
+    const int first = u.suffix ? max(0, u.j0 - u.longest + a.rows) / w.per_tile : 0;
+    u.span = u.j0 >= u.longest ? 0 : max(0, (u.tokens + w.per_tile - 1) / w.per_tile - first);
+    u.i0 = first + int((long long)u.span * rank / w.ranks);
+    u.n = first + int((long long)u.span * (rank + 1) / w.ranks) - u.i0;
+    return u;
+  };
+  // The units of this CTA (of its cluster: one) that have row tiles.
+  const int step = gridDim.x / w.ranks;
+  auto next = [&](int& at, Unit& u) {
+    for (; at < w.units; at += step) {
+      u = unit_of(at);
+      if (u.n > 0) {
+        at += step;
+        return true;
+      }
+    }
+    return false;
+  };
+  auto active = [](const Unit& u, int p) { return u.j0 + p * kKeys < u.longest; };
 
-  float sum = 0.f;
-  if (warp == 4) {
-    if (n > 0 && elect_one()) {
+  if (warp == kIssueWarp) {
+    if (elect_one()) {
       auto mem = [&](uint32_t off) { return smem_raw + (base + off - smem_addr(smem_raw)); };
       const unsigned q_bytes = unsigned(w.per_tile * a.group * 128 * (D / 64));
-      auto load_q = [&](int i) {
-        mbar_arrive_expect_tx(&q_full[i & 1], q_bytes);
-        for (int c = 0; c < D / 64; ++c)
-          tma_3d(mem((1 + (i & 1)) * slot + c * kAtom), &w.q, 64 * c, h * a.group, token0 + (i0 + i) * w.per_tile,
-                 &q_full[i & 1]);
+      // Row tiles issued and loaded, of all units in turn; scores issued per key
+      // tile; units whose keys were loaded.  The x-th use of a pair of buffers is
+      // of buffer x & 1, for its (x >> 1)-th time.
+      unsigned x = 0, loaded = 0, scored[2] = {0, 0}, unit = 0, keys = 0;
+      bool ok = true;
+      auto load_keys = [&](const Unit& u) {
+        uint64_t* bar = &k_full[keys & 1];
+        const int tiles = active(u, 1) ? 2 : 1;
+        mbar_arrive_expect_tx(bar, unsigned(tiles * slot));
+        for (int p = 0; p < tiles; ++p)
+          for (int c = 0; c < D / 64; ++c) {
+            unsigned char* dst = mem(((keys & 1) * 2 + p) * slot + c * kAtom);
+            if (u.suffix) tma_4d(dst, &w.sk, 64 * c, u.h, u.j0 + p * kKeys, u.b, bar);
+            else tma_3d(dst, &w.pk, 64 * c, u.h, u.j0 + p * kKeys, bar);
+          }
+        ++keys;
       };
-      mbar_arrive_expect_tx(&k_full, unsigned(slot));
-      for (int c = 0; c < D / 64; ++c) {
-        if (suffix) tma_4d(mem(c * kAtom), &w.sk, 64 * c, h, j0, b, &k_full);
-        else tma_3d(mem(c * kAtom), &w.pk, 64 * c, h, j0, &k_full);
+      auto load_query = [&](const Unit& u, int i) {
+        const int s = loaded & 1;
+        if (loaded >= 2 && !role_wait(&q_free[s], ((loaded >> 1) + 1) & 1, failed)) return false;
+        mbar_arrive_expect_tx(&q_full[s], q_bytes);
+        for (int c = 0; c < D / 64; ++c)
+          tma_3d(mem((4 + s) * slot + c * kAtom), &w.q, 64 * c, u.h * a.group, u.token0 + (u.i0 + i) * w.per_tile,
+                 &q_full[s]);
+        ++loaded;
+        return true;
+      };
+      Unit u, v;
+      int at = blockIdx.x / w.ranks, li = 0;  // li: next row tile to load, of u or (ahead) of v
+      bool have = next(at, u), more = false, ahead = false;
+      if (have) {
+        load_keys(u);
+        more = next(at, v);
       }
-      load_q(0);
-      int loaded = 1;
-      if (n > 1) {
-        load_q(1);
-        loaded = 2;
-      }
-      bool ok = role_wait(&k_full, 0, failed);
-      int issued = 0;
-      for (int i = 0; i < n && ok; ++i) {
-        ok = role_wait(&q_full[i & 1], (i >> 1) & 1, failed) &&
-             (i < 2 || role_wait(&s_free[i & 1], ((i >> 1) + 1) & 1, failed));
-        if (!ok) break;
-        fence_after_sync();
-        const uint32_t kt = base, qt = base + (1 + (i & 1)) * slot;
+      auto load_more = [&] {  // two row tiles ahead of the products, into the next unit if need be
+        while (ok && loaded < x + 2) {
+          if (!ahead && li >= u.n) {
+            if (!more) return;
+            ahead = true;
+            li = 0;
+          }
+          if (ahead && li >= v.n) return;
+          ok = load_query(ahead ? v : u, li++);
+        }
+      };
+      while (have && ok) {
+        load_more();
+        ok = ok && role_wait(&k_full[unit & 1], (unit >> 1) & 1, failed);
+        for (int i = 0; i < u.n && ok; ++i) {
+          const int s = x & 1;
+          ok = role_wait(&q_full[s], (x >> 1) & 1, failed);
+          for (int p = 0; p < 2 && ok; ++p) {
+            if (!active(u, p)) continue;
+            const int sb = scored[p] & 1;
+            if (scored[p] >= 2) ok = role_wait(&s_free[p][sb], ((scored[p] >> 1) + 1) & 1, failed);
+            if (!ok) break;
+            fence_after_sync();
+            const uint32_t kt = base + ((unit & 1) * 2 + p) * slot, qt = base + (4 + s) * slot;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t atom = uint32_t(kk >> 2) * kAtom;
-          const uint64_t off = uint64_t((kk & 3) * 2);
-          mma_bf16(tmem + (i & 1) * kRows, smem_desc_sw128(kt + atom) + off, smem_desc_sw128(qt + atom) + off,
-                   instr_desc_bf16(kKeys, kRows), kk ? 1u : 0u);
-        }
-        mma_commit(&s_full[i & 1]);
-        mma_commit(&q_free[i & 1]);
-        issued = i + 1;
-        if (i + 2 < n) {
-          ok = role_wait(&q_free[i & 1], (i >> 1) & 1, failed);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t atom = uint32_t(kk >> 2) * kAtom;
+              const uint64_t off = uint64_t((kk & 3) * 2);
+              mma_bf16(tmem + (p * 2 + sb) * kRows, smem_desc_sw128(kt + atom) + off, smem_desc_sw128(qt + atom) + off,
+                       instr_desc_bf16(kKeys, kRows), kk ? 1u : 0u);
+            }
+            mma_commit(&s_full[p][sb]);
+            ++scored[p];
+          }
           if (!ok) break;
-          load_q(i + 2);
-          loaded = i + 3;
+          mma_commit(&q_free[s]);
+          ++x;
+          if (i == 0 && more) {  // the other keys' buffer: its last product is over
+            if (x >= 2) ok = role_wait(&q_free[x & 1], ((x - 2) >> 1) & 1, failed);
+            if (ok) load_keys(v);
+          }
+          load_more();
         }
+        if (!ok) break;
+        have = more;
+        u = v;
+        if (!ahead) li = 0;
+        ahead = false;
+        more = have && next(at, v);
+        ++unit;
       }
       if (!ok) {  // copies and products still in flight use this CTA's memory
-        mbar_wait(&k_full, 0);
-        for (int i = max(0, loaded - 2); i < loaded; ++i) mbar_wait(&q_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, issued - 2); i < issued; ++i) mbar_wait(&q_free[i & 1], (i >> 1) & 1);
+        for (unsigned k = keys > 2 ? keys - 2 : 0; k < keys; ++k) mbar_wait(&k_full[k & 1], (k >> 1) & 1);
+        for (unsigned k = loaded > 2 ? loaded - 2 : 0; k < loaded; ++k) mbar_wait(&q_full[k & 1], (k >> 1) & 1);
+        mma_commit(&q_free[x & 1]);  // completes with the products issued so far
+        if (x >= 1) mbar_wait(&q_free[(x - 1) & 1], ((x - 1) >> 1) & 1);
+        mbar_wait(&q_free[x & 1], (x >> 1) & 1);
       }
     }
     __syncwarp();
   } else {
-    const int r = threadIdx.x, key = j0 + r;
-    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
-    // Row r of row tile i: its norm and the keys it sees.
-    auto fetch = [&](int i, RowNorm& nm, int& seen) {
-      const int local = (i0 + i) * w.per_tile + r / a.group, token = token0 + local;
-      nm = RowNorm{0.f, 0.f};
-      seen = 0;
-      if (i >= n || r / a.group >= w.per_tile || local >= tokens) return;
-      nm = w.norm[size_t(token) * a.query_heads + h * a.group + r % a.group];
-      seen = suffix ? suffix_seen(suffix_len(a, b), a.rows, local) : prefix_len(a, token / a.rows);
+    // Key r of tile p, columns (rows of the queries) from half * 64 on.
+    const int r = threadIdx.x % kKeys, half = threadIdx.x / kKeys % 2, p = threadIdx.x / kPair;
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16) + p * 2 * kRows + half * (kRows / 2);
+    const uint64_t scale2 = pair(w.scale_log2, w.scale_log2);
+    // Row r of row tile i, if it exists; its norm is on its way from one turn to the next.
+    auto row_of = [&](const Unit& u, int i, int& local) {
+      local = (u.i0 + i) * w.per_tile + r / a.group;
+      return r / a.group < w.per_tile && local < u.tokens;
     };
-    RowNorm nm;
-    int seen;
-    fetch(0, nm, seen);
-    bool ok = true;
+    auto fetch = [&](const Unit& u, int i) {
+      int local;
+      RowNorm nm = {0.f, 0.f};
+      if (half == 0 && row_of(u, i, local))
+        nm = w.norm[size_t(u.token0 + local) * a.query_heads + u.h * a.group + r % a.group];
+      return nm;
+    };
+    auto next_active = [&](int& at, Unit& u) {
+      while (next(at, u))
+        if (active(u, p)) return true;
+      return false;
+    };
+    Unit u, following;
+    int at = blockIdx.x / w.ranks;
+    unsigned g = 0;
+    bool ok = true, more = next_active(at, u);
+    RowNorm nm = {0.f, 0.f};
+    if (more) nm = fetch(u, 0);
+    sums[threadIdx.x] = 0.f;
+    while (more) {
+      const int j0 = u.j0 + p * kKeys, key = j0 + r;
+      float sum = 0.f;
+      more = next_active(at, following);
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int s = i & 1;
-      norms[s][r] = RowNorm{-nm.m, nm.r};
-      seen_s[s][r] = seen;
-      const bool all = __all_sync(0xffffffffu, seen >= j0 + kKeys);
-      if (lane == 0) whole[s][warp] = all;
-      named_sync(1, kKeys);
-      fetch(i + 1, nm, seen);
-      // After a failure the remaining turns only keep the barrier above met.
-      ok = ok && role_wait_warp(&s_full[s], (i >> 1) & 1, failed);
-      if (!ok) continue;
-      fence_after_sync();
-      const bool unmasked = whole[s][0] && whole[s][1] && whole[s][2] && whole[s][3];
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < u.n; ++i, ++g) {
+        const int s = g & 1;
+        if (half == 0) norms[p][s][r] = RowNorm{-nm.m, nm.r};
+        // Does every row of the tile exist and see every key of it?
+        const int head = (u.i0 + i) * w.per_tile;
+        const bool plain = w.per_tile * a.group == kRows && head + w.per_tile <= u.tokens &&
+                           j0 + kKeys <= (u.suffix ? suffix_seen(u.longest, a.rows, head) : u.shortest);
+        if (!plain && half == 0) {
+          int local;
+          seen_s[p][s][r] = !row_of(u, i, local) ? 0
+                            : u.suffix           ? suffix_seen(u.longest, a.rows, local)
+                                                 : prefix_len(a, (u.token0 + local) / a.rows);
+        }
+        named_sync(1 + p, kPair);
+        if (i + 1 < u.n) nm = fetch(u, i + 1);
+        else if (more) nm = fetch(following, 0);
+        // After a failure the remaining turns only keep the barrier above met.
+        ok = ok && role_wait_warp(&s_full[p][s], (g >> 1) & 1, failed);
+        if (!ok) continue;
+        fence_after_sync();
+        uint64_t part[4] = {0, 0, 0, 0};
 #pragma unroll 1
-      for (int c = 0; c < kRows; c += 32) {
-        uint32_t v[32];
-        tmem_ld32_async(lanes + s * kRows + c, v);
-        tmem_ld_wait32(v);
-        const float4* nv = reinterpret_cast<const float4*>(norms[s] + c);
-        if (unmasked) {
+        for (int c = 0; c < kRows / 2; c += 32) {
+          uint32_t v[32];
+          tmem_ld32_async(lanes + s * kRows + c, v);
+          tmem_ld_wait32(v);
+          const int from = half * (kRows / 2) + c;
+          const float4* nv = reinterpret_cast<const float4*>(norms[p][s] + from);
+          if (plain) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float4 y = nv[k];
-            part[(2 * k) & 3] =
-                fmaf(exp2_approx(fmaf(__uint_as_float(v[2 * k]), w.scale_log2, y.x)), y.y, part[(2 * k) & 3]);
-            part[(2 * k + 1) & 3] =
-                fmaf(exp2_approx(fmaf(__uint_as_float(v[2 * k + 1]), w.scale_log2, y.z)), y.w, part[(2 * k + 1) & 3]);
-          }
-        } else {
+            for (int k = 0; k < 16; ++k) {
+              const float4 y = nv[k];
+              float x0, x1;
+              unpair(fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), scale2, pair(y.x, y.z)), x0,
+                     x1);
+              part[k & 3] = fma2(pair(exp2_approx(x0), exp2_approx(x1)), pair(y.y, y.w), part[k & 3]);
+            }
+          } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const RowNorm y = norms[s][c + k];
-            const float e = exp2_approx(fmaf(__uint_as_float(v[k]), w.scale_log2, y.m));
-            part[k & 3] = key < seen_s[s][c + k] ? fmaf(e, y.r, part[k & 3]) : part[k & 3];
+            for (int k = 0; k < 32; ++k) {
+              const RowNorm y = norms[p][s][from + k];
+              const float e = exp2_approx(fmaf(__uint_as_float(v[k]), w.scale_log2, y.m));
+              part[k & 3] = fma2(pair(key < seen_s[p][s][from + k] ? e : 0.f, 0.f), pair(y.r, 0.f), part[k & 3]);
+            }
           }
         }
+        float x0, x1;
+        unpair(add2(add2(part[0], part[1]), add2(part[2], part[3])), x0, x1);
+        sum += x0 + x1;
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[p][s]);
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-      fence_before_sync();
-      mbar_arrive(&s_free[s]);
+      if (!ok) sum = NAN;
+      sums[threadIdx.x] = sum;
+      if (w.ranks > 1) break;  // joined across the cluster below
+      named_sync(1 + p, kPair);
+      if (half == 0 && key < (u.suffix ? a.scap : a.pcap)) {
+        float* out = u.suffix ? a.sw + (size_t(u.b) * a.kv_heads + u.h) * a.scap : a.pw + size_t(u.h) * a.pcap;
+        out[key] += sum + sums[threadIdx.x + kKeys];
+      }
+      u = following;
     }
-    if (!ok) sum = NAN;
-    sums[r] = sum;
+    fence_before_sync();
   }
-  fence_before_sync();
-  if (w.ranks > 1) cluster_sync();
-  else __syncthreads();
-  if (warp < 4 && rank == 0 && span > 0) {
-    const int key = j0 + int(threadIdx.x), cap = suffix ? a.scap : a.pcap;
-    float total = 0.f;
-    for (int r = 0; r < w.ranks; ++r) {
-      float v;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                   : "=f"(v)
-                   : "r"(mapa_shared(smem_addr(&sums[threadIdx.x]), r))
-                   : "memory");
-      total += v;
+  if (w.ranks > 1) {
+    cluster_sync();
+    const Unit u = unit_of(blockIdx.x / w.ranks);
+    if (threadIdx.x < kPair && rank == 0 && u.span > 0) {
+      const int p = threadIdx.x / kKeys, r = threadIdx.x % kKeys, key = u.j0 + int(threadIdx.x);
+      float total = 0.f;
+      for (int x = 0; x < 2 * w.ranks; ++x) {  // ranks in order, the halves of each
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(v)
+                     : "r"(mapa_shared(smem_addr(&sums[p * kPair + (x & 1) * kKeys + r]), x >> 1))
+                     : "memory");
+        total += v;
+      }
+      if (active(u, p) && key < (u.suffix ? a.scap : a.pcap)) {
+        float* out = u.suffix ? a.sw + (size_t(u.b) * a.kv_heads + u.h) * a.scap : a.pw + size_t(u.h) * a.pcap;
+        out[key] += total;
+      }
     }
-    if (key < cap) {
-      float* out = suffix ? a.sw + (size_t(b) * a.kv_heads + h) * a.scap : a.pw + size_t(h) * a.pcap;
-      out[key] += total;
-    }
+    cluster_sync();
+  } else {
+    __syncthreads();
   }
-  if (w.ranks > 1) cluster_sync();
-  if (warp == 4) tmem_dealloc(tmem, kTmemCols);
+  if (warp == kIssueWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
 }  // namespace
 
-cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream) {
   WeightArgs w = {};
   w.a = a;
   w.norm = ws.norm;
   w.per_tile = p.per_tile;
-  w.prefix_tiles = a.pw ? (a.pcap + kKeys - 1) / kKeys : 0;
-  w.suffix_tiles = a.sw && !p.pooled ? (a.scap + kKeys - 1) / kKeys : 0;
+  w.prefix_pairs = a.pw ? (a.pcap + kPair - 1) / kPair : 0;
+  w.suffix_pairs = a.sw && !p.pooled ? (a.scap + kPair - 1) / kPair : 0;
   w.ranks = p.weight_ranks;
   w.scale_log2 = attention_scale(a.width) * kLog2e;
   if (!encode_query_map(&w.q, a, p.per_tile)) return cudaErrorInvalidValue;
-  if (w.prefix_tiles && !encode_prefix_map(&w.pk, a, a.pk)) return cudaErrorInvalidValue;
-  if (w.suffix_tiles && !encode_suffix_map(&w.sk, a, a.sk)) return cudaErrorInvalidValue;
-  const long long units = (long long)(w.prefix_tiles + (long long)w.suffix_tiles * a.batch) * a.kv_heads;
+  if (w.prefix_pairs && !encode_prefix_map(&w.pk, a, a.pk)) return cudaErrorInvalidValue;
+  if (w.suffix_pairs && !encode_suffix_map(&w.sk, a, a.sk)) return cudaErrorInvalidValue;
+  const long long units = (w.prefix_pairs + (long long)w.suffix_pairs * a.batch) * a.kv_heads;
   if (units == 0) return cudaSuccess;
-  const int smem = 3 * (a.width / 64) * kAtom + 1024;
+  if (units > (1 << 30)) return cudaErrorInvalidValue;
+  w.units = int(units);
+  // At least half of an SM's memory, so that two blocks never share an SM: each
+  // takes all of its TMEM, and blocks of two clusters could wait for one another.
+  const int smem = std::max(6 * (a.width / 64) * kAtom + 1024, 120 << 10);
   const cudaError_t e = a.width == 64 ? allow_smem<shared_weights_kernel<64>>(smem)
                                       : allow_smem<shared_weights_kernel<128>>(smem);
   if (e != cudaSuccess) return e;
-  DependentLaunch d(dim3(unsigned(units * w.ranks)), kThreads, smem, stream, w.ranks);
+  const int grid = w.ranks > 1 ? w.units * w.ranks : std::min(w.units, sms);
+  DependentLaunch d(dim3(unsigned(grid)), kThreads, smem, stream, w.ranks);
   return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<64>, w)
                        : cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<128>, w);
 }
