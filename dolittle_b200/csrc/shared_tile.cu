@@ -550,49 +550,84 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the key ranges of the split tasks: one warp per (token, query head),
-// the ranges in order.
+// Joins the key ranges of the split tasks: a warp takes four rows (token, query
+// head) of a tile at once, all their loads in flight together, lanes hold a
+// row's features; the ranges in order.
+constexpr int kMergeRows = 4, kMergeWarps = 4;
+
 template <int D>
-__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws,
-                                                           bool norms) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = row % kRows;
+__global__ void __launch_bounds__(32 * kMergeWarps) shared_merge_kernel(const SharedAttnArgs a, const Plan pl,
+                                                                       const Workspace ws, bool norms) {
+  constexpr int F = D / 32;  // consecutive features of a lane
+  const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kMergeWarps + (threadIdx.x >> 5)) * kMergeRows;
+  const int rest = pl.tasks - pl.full, task = pl.full + row0 / kRows / pl.per_cta;
+  const int tile = task % pl.groups * pl.per_cta + row0 / kRows % pl.per_cta, h = task / pl.groups % a.kv_heads;
+  const size_t stride = size_t(rest) * pl.per_cta * kRows;  // rows between two ranges
   wait_prior();
   allow_next();
-  const int rest = pl.tasks - pl.full, task = pl.full + row / kRows / pl.per_cta;
-  const int tile = task % pl.groups * pl.per_cta + row / kRows % pl.per_cta, h = task / pl.groups % a.kv_heads;
-  const int local = tile * pl.per_tile + r / a.group;
-  if (r / a.group >= pl.per_tile || local >= a.rows) return;
-  const int token = task / pl.groups / a.kv_heads * a.rows + local, hq = h * a.group + r % a.group;
-  const size_t stride = size_t(rest) * pl.per_cta * kRows;  // rows between two ranges
-  float top = -INFINITY;
-  for (int s = 0; s < pl.splits; ++s) top = fmaxf(top, ws.part_ml[row + s * stride].x);
-  constexpr int F = D / 32;  // consecutive features of a lane
-  const float* src = ws.part_o + size_t(row / kRows) * kRows * D + part_offset<D>(r, lane * F);
-  float l = 0.f, o[F] = {};
-#pragma unroll 4
-  for (int s = 0; s < pl.splits; ++s) {
-    const float2 ml = ws.part_ml[row + s * stride];
-    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-    l = fmaf(ml.y, f, l);
-    float v[F];
-    if constexpr (F == 4) {
-      const float4 y = *reinterpret_cast<const float4*>(src + s * stride * D);
-      v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
-    } else {
-      const float2 y = *reinterpret_cast<const float2*>(src + s * stride * D);
-      v[0] = y.x, v[1] = y.y;
-    }
+  const int first = row0 % kRows;
+  const float* src = ws.part_o + size_t(row0 / kRows) * kRows * D;
+  float2 ml[kMergeRows];
+  float top[kMergeRows], l[kMergeRows], o[kMergeRows][F];
 #pragma unroll
-    for (int c = 0; c < F; ++c) o[c] = fmaf(v[c], f, o[c]);
+  for (int j = 0; j < kMergeRows; ++j) {
+    ml[j] = lane < pl.splits ? ws.part_ml[row0 + j + lane * stride] : make_float2(-INFINITY, 0.f);
+    l[j] = 0.f;
+#pragma unroll
+    for (int c = 0; c < F; ++c) o[j][c] = 0.f;
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
-  uint32_t* out = reinterpret_cast<uint32_t*>(a.out + size_t(token) * a.ldo + size_t(hq) * D + lane * F);
+  auto load = [&](int s, float (&v)[kMergeRows][F]) {
 #pragma unroll
-  for (int c = 0; c < F; c += 2) out[c / 2] = pack_bf16(o[c] * inv, o[c + 1] * inv);
-  if (lane == 0) {
-    const size_t at = size_t(token) * a.query_heads + hq;
-    if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
-    if (norms) ws.norm[at] = l == 0.f ? RowNorm{0.f, 0.f} : RowNorm{top, inv};
+    for (int j = 0; j < kMergeRows; ++j) {
+      const float* p = src + s * stride * D + part_offset<D>(first + j, lane * F);
+      if constexpr (F == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(p);
+        v[j][0] = y.x, v[j][1] = y.y, v[j][2] = y.z, v[j][3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(p);
+        v[j][0] = y.x, v[j][1] = y.y;
+      }
+    }
+  };
+  float v[2][kMergeRows][F];
+  load(0, v[0]);
+#pragma unroll
+  for (int j = 0; j < kMergeRows; ++j) {
+    top[j] = ml[j].x;
+#pragma unroll
+    for (int k = 16; k; k >>= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], k));
+    ml[j].x = ml[j].x == -INFINITY ? 0.f : exp2_approx(ml[j].x - top[j]);  // now the range's factor
+  }
+  auto add = [&](int s, const float (&v)[kMergeRows][F]) {
+#pragma unroll
+    for (int j = 0; j < kMergeRows; ++j) {
+      const float f = __shfl_sync(0xffffffffu, ml[j].x, s);
+      l[j] = fmaf(__shfl_sync(0xffffffffu, ml[j].y, s), f, l[j]);
+#pragma unroll
+      for (int c = 0; c < F; ++c) o[j][c] = fmaf(v[j][c], f, o[j][c]);
+    }
+  };
+#pragma unroll 1
+  for (int s = 0; s < pl.splits; s += 2) {
+    if (s + 1 < pl.splits) load(s + 1, v[1]);
+    add(s, v[0]);
+    if (s + 2 < pl.splits) load(s + 2, v[0]);
+    if (s + 1 < pl.splits) add(s + 1, v[1]);
+  }
+#pragma unroll
+  for (int j = 0; j < kMergeRows; ++j) {
+    const int r = first + j, local = tile * pl.per_tile + r / a.group;
+    if (r / a.group >= pl.per_tile || local >= a.rows) continue;
+    const int token = task / pl.groups / a.kv_heads * a.rows + local, hq = h * a.group + r % a.group;
+    const float inv = l[j] > 0.f ? 1.f / l[j] : l[j] == 0.f ? 0.f : NAN;
+    uint32_t* out = reinterpret_cast<uint32_t*>(a.out + size_t(token) * a.ldo + size_t(hq) * D + lane * F);
+#pragma unroll
+    for (int c = 0; c < F; c += 2) out[c / 2] = pack_bf16(o[j][c] * inv, o[j][c + 1] * inv);
+    if (lane == 0) {
+      const size_t at = size_t(token) * a.query_heads + hq;
+      if (a.lse) a.lse[at] = l[j] == 0.f ? -INFINITY : (top[j] + log2f(l[j])) * kLn2;
+      if (norms) ws.norm[at] = l[j] == 0.f ? RowNorm{0.f, 0.f} : RowNorm{top[j], inv};
+    }
   }
 }
 
@@ -632,7 +667,8 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace
 }
 
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  DependentLaunch d(dim3(unsigned(p.tasks - p.full) * p.per_cta * (kRows / 8)), 256, 0, stream);
+  DependentLaunch d(dim3(unsigned(p.tasks - p.full) * p.per_cta * (kRows / (kMergeRows * kMergeWarps))),
+                    32 * kMergeWarps, 0, stream);
   const bool norms = a.pw || a.sw;
   const cudaError_t e =
       a.width == 64 ? allow_smem<shared_merge_kernel<64>>(0) : allow_smem<shared_merge_kernel<128>>(0);
