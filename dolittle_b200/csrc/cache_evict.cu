@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
   };
 
   constexpr int held = TILES ? TILES : 1;
-  unsigned keys[held];
+  unsigned keys[held] = {};
   long long recent_from = 0;
   unsigned long long cut = 0;  // order of the last slot that stays
   auto key_at = [&](int e, int s) {

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int g4 = lane >> 2, c2 = (lane & 3) * 2;
   const int live = a.rows * a.group;  // row = new token * group + query head of the group
-  int np, n, ps, g0, g1, steps;  // keys of prefix and suffix; steps of 16: prefix steps, this CTA's [g0, g1), per warp
+  int np = 0, n = 0, ps = 0, g0 = 0, g1 = 0, steps = 0;  // keys of prefix and suffix; steps of 16: prefix steps, this CTA's [g0, g1), per warp
   float o[NB][D / 16][4], m[NB][2], l[NB][2];
   const uint32_t ring = smem_addr(smem) + warp * (kSlots * kStep * D * 2);
   constexpr int P = D / 8;  // 16-byte pieces of a row; piece c of row k lies at c ^ (k & 7)

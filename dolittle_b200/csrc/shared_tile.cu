@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   using S = Shape<D, WIDE, BESIDE>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_half[2], p_full[2], o_full[2];
-  __shared__ uint64_t dirty, clean, drained;
+  __shared__ uint64_t begun, dirty, clean, drained;
   __shared__ uint32_t dirty_from, dirty_to;  // bytes of a value tile's first 64 features to clear
   __shared__ uint32_t tmem_slot;
   __shared__ int most[2];  // keys of the prefix / suffix that any row sees
@@ -125,10 +125,10 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
       mbar_init(&p_full[x], 4);
       mbar_init(&o_full[x], 1);
     }
+    mbar_init(&begun, 1);
     mbar_init(&dirty, 1);
     mbar_init(&clean, 1);
     mbar_init(&drained, 1);
-    most[0] = most[1] = 0;
     failed_s = 0;
     fence_barrier_init();
   }
@@ -149,21 +149,31 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
   const int local = tile * pl.per_tile + r / a.group;  // token within the unit
   const bool live = warp < kTmaWarp && r / a.group < pl.per_tile && local < unit_tokens && tile < pl.tiles;
   const int token = pl.pooled ? local : seq * a.rows + local;
-  int seen_p = 0, seen_s = 0, np = 0, k0 = 0, n = 0;  // keys the row sees; prefix tiles, the range's tiles
-  // Every role calls this before it touches what other kernels wrote.
+  int np = 0, k0 = 0, n = 0;  // prefix tiles; the range's tiles
+  // Every role calls this before it touches what other kernels wrote.  The
+  // loading warp finds how far the rows see, so that the first tiles are under
+  // way while the softmax warps still fetch their code.
   auto begin = [&] {
     wait_prior();
     allow_next();  // after the wait: the next kernel may read what this one's inputs are before it waits itself
-    if (warp < kTmaWarp) {
-      seen_p = live ? prefix_len(a, token / a.rows) : 0;
-      seen_s = live && !pl.pooled ? suffix_seen(suffix_len(a, seq), a.rows, local) : 0;
-      const int p = __reduce_max_sync(0xffffffffu, seen_p), s = __reduce_max_sync(0xffffffffu, seen_s);
-      if (lane == 0) {
-        atomicMax(&most[0], p);
-        atomicMax(&most[1], s);
+    if (warp == kTmaWarp) {
+      const int end = min((tile0 + (WIDE ? streams : 1)) * pl.per_tile, unit_tokens);  // the CTA's tokens
+      int p = 0, s = 0;
+      if (pl.pooled) {
+        for (int b = tile0 * pl.per_tile / a.rows + lane; b <= (end - 1) / a.rows; b += 32) p = max(p, prefix_len(a, b));
+        p = __reduce_max_sync(0xffffffffu, p);
+      } else {
+        p = prefix_len(a, seq);
+        s = suffix_seen(suffix_len(a, seq), a.rows, end - 1);
       }
+      if (lane == 0) {
+        most[0] = p;
+        most[1] = s;
+        mbar_arrive(&begun);
+      }
+      __syncwarp();
     }
-    __syncthreads();
+    if (!role_wait_warp(&begun, 0, failed)) return;  // n stays 0
     np = (most[0] + kKeys - 1) / kKeys;
     const int nt = np + (most[1] + kKeys - 1) / kKeys;
     k0 = int((long long)nt * split / splits);
@@ -335,24 +345,33 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     }
   } else if (warp < kTmaWarp) {
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + x * kKeys, t_o = tmem + lanes + 256 + x * 128;
+    const uint32_t t_o = tmem + lanes + 256 + x * 128;
     const float c = t.scale_log2;
     float m = -INFINITY, l = 0.f;  // m: unscaled reference of the row
+    int seen_p = 0, seen_s = 0;    // keys the row sees
     bool ok = true;
-    // Turn -1 (BESIDE) runs the code once on whatever the scores' columns hold,
-    // while the kernel before this one ends: a decode step has only a few turns,
-    // and fetching the loop from memory that other kernels' data went through
-    // took longer than they do (batch 32 on 8192 keys: 4900 and 3400 cycles for
-    // the two passes of the first turn, 720 and 2400 after it).
+    // Turn -1 (BESIDE) runs the code once on whatever the tensor memory holds,
+    // while the kernel before this one ends and the first tiles load: a decode
+    // step has only a few turns, and fetching the loop from memory that other
+    // kernels' data went through took longer than they do (batch 32 on 8192
+    // keys: 4900 and 3400 cycles for the two passes of the first turn, 720 and
+    // 2400 after it).
 #pragma unroll 1
     for (int i = BESIDE ? -1 : 0;; ++i) {
       if (i == 0) {
         begin();
+        if (live) {
+          seen_p = prefix_len(a, token / a.rows);
+          if (!pl.pooled) seen_s = suffix_seen(suffix_len(a, seq), a.rows, local);
+        }
         m = -INFINITY;
         l = 0.f;
       }
       if (i >= 0 && i >= count(x)) break;
       const int g = k0 + nth(x, i);
+      // The scores' columns; in turn -1 those of the output, which nothing uses
+      // before this warp has handed over its first weights.
+      const uint32_t t_s = i < 0 ? t_o : tmem + lanes + x * kKeys;
       int lim = kKeys;  // keys of the tile this row sees
       if (i >= 0) {
         lim = g < np ? seen_p - g * kKeys : seen_s - (g - np) * kKeys;
