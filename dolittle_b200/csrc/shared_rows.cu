@@ -33,7 +33,10 @@ constexpr int kSlots = 3;
 constexpr float kRescale = 8.f;
 constexpr int kMaxParts = kMaxSplits + kMaxSuffixSplits;
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool real) {
   const int bytes = real ? 16 : 0;  // 0: zero fill, nothing read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -181,12 +184,22 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
       const bf16* src = base + (pre ? 0 : size_t(b) * a.s_seq) + size_t(h) * D;
       const int j0 = (pre ? g : g - ps) * kStep, end = pre ? np : n;
       const size_t stride = pre ? a.p_row : a.s_row;
-      const uint32_t dst = ring + slot * (kStep * D * 2);
+      // Lane: piece lane % P of rows lane / P, + 32 / P, ...
+      constexpr int kApart = 32 / P;
+      const int k0 = lane / P, c = lane % P;
+      const bf16* from = src + size_t(j0 + k0) * stride + c * 8;
+      const uint32_t dst = ring + slot * (kStep * D * 2) + k0 * (D * 2);
+      const bool whole = j0 + kStep <= end;
 #pragma unroll
-      for (int u = 0; u < kStep * P / 32; ++u) {
-        const int idx = u * 32 + lane, k = idx / P, c = idx % P, j = j0 + k;
-        const bool real = j < end;
-        cp16(dst + k * (D * 2) + ((c ^ (k & 7)) << 4), src + size_t(real ? j : 0) * stride + c * 8, real);
+      for (int u = 0; u < kStep / kApart; ++u) {
+        const uint32_t to = dst + u * kApart * (D * 2) + (((c ^ k0) ^ (u * kApart & 7)) << 4);
+        if (whole) {
+          cp16(to, from);
+          from += kApart * stride;
+        } else {
+          const int j = j0 + k0 + u * kApart;
+          cp16_or_zero(to, src + size_t(j < end ? j : 0) * stride + c * 8, j < end);
+        }
       }
     }
     cp_commit();
@@ -281,12 +294,8 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
           }
           if (ka >= end) s[nb][u] = -INFINITY;
           if (kb >= end) s[nb][2 + u] = -INFINITY;
-          float x = fmaxf(s[nb][u], s[nb][2 + u]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          top[nb][u] = x;
-          grow = grow || (x - m[nb][u]) * scale_log2 > kRescale;
+          top[nb][u] = fmaxf(s[nb][u], s[nb][2 + u]);  // of this lane's keys
+          grow = grow || (top[nb][u] - m[nb][u]) * scale_log2 > kRescale;
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -294,9 +303,13 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
           float alpha[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const bool up = (top[nb][u] - m[nb][u]) * scale_log2 > kRescale;
-            alpha[u] = up ? exp2_approx((m[nb][u] - top[nb][u]) * scale_log2) : 1.f;
-            if (up) m[nb][u] = top[nb][u];
+            float x = top[nb][u];  // of the row's
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const bool up = (x - m[nb][u]) * scale_log2 > kRescale;
+            alpha[u] = up ? exp2_approx((m[nb][u] - x) * scale_log2) : 1.f;
+            if (up) m[nb][u] = x;
             l[nb][u] *= alpha[u];
           }
 #pragma unroll
