@@ -68,7 +68,8 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
   const int step = p.per_cta == 2 ? longest : (longest + 1) / 2 * 2;  // two streams share a narrow task's key tiles
   if (key_tiles) p.splits = std::min(p.splits, (key_tiles + step - 1) / step);
   if (!p.pooled && p.splits == 1) p.full = p.tasks;
-  if (p.pooled && units * size_t(a.pcap) * a.width <= kSoloElements) p.splits = 0;
+  // (Not with rows for two CTAs, which could not add a key's weight together.)
+  if (p.pooled && a.rows * a.group <= kMostRows && units * size_t(a.pcap) * a.width <= kSoloElements) p.splits = 0;
   const int unit_keys = a.scap + (p.splits ? 0 : a.pcap);
   p.suffix_splits = p.pooled ? suffix_splits(units, unit_keys, 3 * sms) : 1;
   p.weight_ranks = 1;

@@ -17,6 +17,7 @@ constexpr int kKeys = 128;   // keys of a tile
 constexpr int kMaxSplits = 32;  // key ranges of a row tile
 constexpr int kMaxSuffixSplits = 8;
 constexpr int kFewRows = 32;    // rows of a unit (new tokens x group) that the few-row kernels take
+constexpr int kMostRows = 16;   // and one CTA of them
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -86,9 +86,8 @@ __device__ __forceinline__ float4 remote_f32x4(const float* p, unsigned rank) {
 template <int D, int NB>
 struct RowsShape {
   static constexpr int rows = 8 * NB;
-  static constexpr int ring = kWarps * kSlots * kStep * D * 2;
-  static constexpr int join = kWarps * rows * D * 4;  // the warps' outputs, over the ring
-  static constexpr int smem = ring > join ? ring : join;
+  static constexpr int smem = kWarps * kSlots * kStep * D * 2;
+  static_assert(NB <= kMostRows / 8 && (kWarps + 1) * rows * D * 4 <= smem, "the outputs fit the ring");
 };
 
 // The whole softmax of one row from its parts' (maximum, sum), by one warp:
@@ -134,6 +133,23 @@ __device__ __forceinline__ void add_part(float4& out, float4 y, float f) {
   out.w = fmaf(y.w, f, out.w);
 }
 
+// The same for four rows of at most eight parts, eight lanes each: lane = 8 x
+// row + part.  Only the lane's own part is read; its factor comes back.
+template <class Part>
+__device__ __forceinline__ RowJoin join_four_rows(bool real, Part&& part, float& factor) {
+  const float2 ml = real ? part() : make_float2(-INFINITY, 0.f);
+  float top = ml.x;
+#pragma unroll
+  for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+  float sum = ml.y * f;
+#pragma unroll
+  for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+  factor = f * inv;
+  return {sum == 0.f ? 0.f : top, inv, sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2};
+}
+
 // Row `row` (new token * group + query head of the group) of unit (b, h).
 __device__ __forceinline__ size_t row_index(const SharedAttnArgs& a, int b, int h, int row) {
   return (size_t(b) * a.rows + row / a.group) * a.query_heads + h * a.group + row % a.group;
@@ -162,16 +178,17 @@ __device__ __forceinline__ void add_suffix_weights(const SharedAttnArgs& a, cons
 }
 
 template <int D, int NB, bool SOLO>
-__global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(const SharedAttnArgs a, const Plan pl,
-                                                                               const Workspace ws,
-                                                                               const float scale_log2) {
+__global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
+    shared_rows_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws, const float scale_log2) {
   constexpr int R = 8 * NB;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float warp_m[kWarps][R], warp_l[kWarps][R], cta_m[R], cta_l[R], row_m[R], row_r[R];
   __shared__ float part_f[R][kMaxSuffixSplits];
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int split = blockIdx.x, h = blockIdx.y % a.kv_heads, b = blockIdx.z;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int g4 = lane >> 2, c2 = (lane & 3) * 2;
-  const int live = a.rows * a.group;  // row = new token * group + query head of the group
+  // Row = new token * group + query head of the group; this CTA's from row0 on.
+  const int unit_rows = a.rows * a.group, row0 = blockIdx.y / a.kv_heads * R, live = min(R, unit_rows - row0);
   int np = 0, n = 0, ps = 0, g0 = 0, g1 = 0, steps = 0;  // keys of prefix and suffix; steps of 16: prefix steps, this CTA's [g0, g1), per warp
   float o[NB][D / 16][4], m[NB][2], l[NB][2];
   const uint32_t ring = smem_addr(smem) + warp * (kSlots * kStep * D * 2);
@@ -230,12 +247,13 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
     uint32_t q[NB][D / 16][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int row = 8 * nb + g4;
+      const int row = row0 + 8 * nb + g4;
+      const bool real = 8 * nb + g4 < rows;
       const bf16* src = a.q + (size_t(b) * a.rows + row / a.group) * a.ldq + size_t(h * a.group + row % a.group) * D;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        q[nb][kk][0] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + c2) : 0u;
-        q[nb][kk][1] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 + c2) : 0u;
+        q[nb][kk][0] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + c2) : 0u;
+        q[nb][kk][1] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 + c2) : 0u;
       }
     }
     // Rows 8 nb + c2, + 1 of the score fragments: how many suffix keys they see.
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int row = 8 * nb + c2 + u;
-        seen[nb][u] = row < rows ? suffix_seen(n, a.rows, row / a.group) : 0;
+        seen[nb][u] = row < rows ? suffix_seen(n, a.rows, (row0 + row) / a.group) : 0;
       }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
 #pragma unroll
       for (int f = 0; f < D / 16; ++f) o[nb][f][0] = o[nb][f][1] = o[nb][f][2] = o[nb][f][3] = 0.f;
     }
-    float* scores = a.sw ? ws.scores + (size_t(b) * a.kv_heads + h) * live * a.scap : nullptr;
+    float* scores = a.sw ? ws.scores + ((size_t(b) * a.kv_heads + h) * unit_rows + row0) * a.scap : nullptr;
 
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
@@ -376,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
       }
     }
   __syncthreads();  // all warps are done with their rings
-  float* joined = reinterpret_cast<float*>(smem);  // [warps][R][D]; piece c of row r at c ^ (r & 7)
+  float* cta_o = reinterpret_cast<float*>(smem);  // [R][D], then [warps][R][D]; piece c of row r at c ^ (r & 7)
+  float* joined = cta_o + R * D;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -400,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
   }
   __syncthreads();
   constexpr int pieces = R * D / 4;
-  float4* cta_o = reinterpret_cast<float4*>(smem);  // over warp 0's part
+  const size_t part0 = ((size_t(split) * a.batch + b) * a.kv_heads + h) * unit_rows + row0;
   for (int i = t; i < pieces; i += kThreads) {
     const int row = i / (D / 4);
     if (row >= live) break;
@@ -414,16 +433,11 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
       v.z = fmaf(y.z, f, v.z);
       v.w = fmaf(y.w, f, v.w);
     }
-    if (SOLO) {
-      cta_o[i] = v;
-    } else {
-      const size_t part = ((size_t(split) * a.batch + b) * a.kv_heads + h) * live + row;
-      reinterpret_cast<float4*>(ws.suffix_o + part * D)[(i % (D / 4)) ^ (row & 7)] = v;
-    }
+    if (SOLO) reinterpret_cast<float4*>(cta_o)[i] = v;
+    else reinterpret_cast<float4*>(ws.suffix_o + (part0 + row) * D)[(i % (D / 4)) ^ (row & 7)] = v;
   }
   if constexpr (!SOLO) {
-    if (t < live)
-      ws.suffix_ml[((size_t(split) * a.batch + b) * a.kv_heads + h) * live + t] = make_float2(cta_m[t], cta_l[t]);
+    if (t < live) ws.suffix_ml[part0 + t] = make_float2(cta_m[t], cta_l[t]);
     // One block outlasts the tile kernel, so that this kernel's end, which the
     // join waits for, is the end of both; the others make room at once.
     if (split == int(gridDim.x) - 1 && h == int(gridDim.y) - 1 && b == int(gridDim.z) - 1) wait_prior();
@@ -432,111 +446,134 @@ __global__ void __launch_bounds__(kThreads, NB == 1 ? 4 : 1) shared_rows_kernel(
   const int ctas = pl.suffix_splits;
   if (ctas > 1) tc::cluster_sync();
   else __syncthreads();
-  for (int row = warp; row < live; row += kWarps) {
-    const RowJoin j = join_row(
-        ctas, [&](int s) { return make_float2(remote_f32(&cta_m[row], s), remote_f32(&cta_l[row], s)); }, part_f[row]);
-    if (lane == 0) {
+  static_assert(kMaxSuffixSplits == 8 && R <= 4 * kWarps, "a warp joins four rows of eight parts");
+  if (4 * warp < live) {
+    const int row = 4 * warp + lane / 8, part = lane % 8;
+    float f;
+    const RowJoin j = join_four_rows(
+        row < live && part < ctas,
+        [&] { return make_float2(remote_f32(&cta_m[row], part), remote_f32(&cta_l[row], part)); }, f);
+    part_f[row][part] = f;
+    if (part == 0 && row < live) {
       row_m[row] = j.m;
       row_r[row] = j.inv;
       if (split == 0) {
-        if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
-        if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+        if (a.lse) a.lse[row_index(a, b, h, row0 + row)] = j.lse;
+        if (a.pw) ws.norm[row_index(a, b, h, row0 + row)] = RowNorm{j.m, j.inv};
       }
     }
   }
   __syncthreads();
   for (int i = split * kThreads + t; i < live * (D / 4); i += ctas * kThreads) {
     const int row = i / (D / 4);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r < ctas; ++r) add_part(v, remote_f32x4(joined + i * 4, r), part_f[row][r]);
-    store_piece<D>(a, b, h, row, (i % (D / 4)) ^ (row & 7), v);
+    float4 y[kMaxSuffixSplits], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMaxSuffixSplits; ++r)
+      if (r < ctas) y[r] = remote_f32x4(cta_o + i * 4, r);
+#pragma unroll
+    for (int r = 0; r < kMaxSuffixSplits; ++r)
+      if (r < ctas) add_part(v, y[r], part_f[row][r]);
+    store_piece<D>(a, b, h, row0 + row, (i % (D / 4)) ^ (row & 7), v);
   }
   if (a.sw)  // of this CTA's suffix keys
     add_suffix_weights(a, ws, scale_log2, b, h, n, max(0, g0 - ps) * kStep, min(n, max(0, g1 - ps) * kStep), row_m, row_r);
   if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Joins the prefix ranges and the suffix ranges of the rows of unit (b, h);
-// with weights, blockIdx.x is a chunk of the suffix keys whose sums it adds.
-// Bound by latency (a few KB per block), so the work is spread thin: four warps
-// share a row, each every fourth part with all its loads in flight, lane =
-// 16-byte piece of the row; every one of them makes the row's factors itself.
-constexpr int kJoinThreads = 512, kJoinWarps = 4;  // warps of a row
-constexpr int kInFlight = 5;                       // parts that a warp has in flight
+// Joins the prefix ranges and the suffix ranges of the rows of unit (b, h).
+// Bound by latency (a few KB per block), so the work is spread thin: a block
+// takes four rows, four warps share a row, each every fourth part with all its
+// loads in flight, lane = 16-byte piece of the row; every one of them makes the
+// row's factors itself.  With weights, further blocks of the unit add the sums
+// of a chunk of its suffix keys each.
+constexpr int kJoinThreads = 512, kJoinWarps = 4;                // warps of a row
+constexpr int kJoinRows = kJoinThreads / 32 / kJoinWarps;        // rows of a block
+constexpr int kInFlight = 5;                                     // parts that a warp has in flight
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads, 2) shared_join_kernel(const SharedAttnArgs a, const Plan pl,
                                                                   const Workspace ws, const float scale_log2) {
-  constexpr int kAtOnce = kJoinThreads / 32 / kJoinWarps;  // rows of a pass
   __shared__ float row_m[kFewRows], row_r[kFewRows], factors[kJoinThreads / 32][kMaxParts];
   __shared__ float4 sums[kJoinThreads / 32][D / 4];
-  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = warp % kJoinWarps, live = a.rows * a.group, parts = pl.splits + pl.suffix_splits;
+  const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int live = a.rows * a.group, blocks = (live + kJoinRows - 1) / kJoinRows;
+  const int parts = pl.splits + pl.suffix_splits;
   const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;       // rows between two prefix ranges
   const size_t suffix_stride = size_t(a.batch) * a.kv_heads * live;  // and two suffix ranges
+  // The row's place in a prefix range, and in its tile; in a suffix range.
+  auto place = [&](int row, size_t& first, int& r, size_t& suffix_row) {
+    const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
+    r = token % pl.per_tile * a.group + row % a.group;
+    first = (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows;
+    suffix_row = (size_t(b) * a.kv_heads + h) * live + row;
+  };
+  auto join = [&](size_t first, int r, size_t suffix_row) {
+    return join_row(
+        parts,
+        [&](int s) {
+          return s < pl.splits ? ws.part_ml[first + r + s * stride]
+                               : ws.suffix_ml[suffix_row + (s - pl.splits) * suffix_stride];
+        },
+        factors[warp]);
+  };
+  size_t first, suffix_row;
+  int r;
   wait_prior();
   allow_next();
-#pragma unroll 1
-  for (int row0 = 0; row0 < live; row0 += kAtOnce) {
-    const int row = row0 + warp / kJoinWarps;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < live) {
-      const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
-      const int r = token % pl.per_tile * a.group + row % a.group;
-      const size_t first = (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows;
-      const size_t suffix_row = (size_t(b) * a.kv_heads + h) * live + row;
-      const float* pre = ws.part_o + first * D + part_offset<D>(r, lane * 4);
-      const float* suf = ws.suffix_o + suffix_row * D + lane * 4;
-      float4 y[kInFlight];
-      auto load = [&](int s0) {
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
-          const int s = s0 + u * kJoinWarps;
-          if (s < parts && lane < D / 4)
-            y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
-                                                                  : suf + (s - pl.splits) * suffix_stride * D);
-        }
-      };
-      load(sub);
-      const RowJoin j = join_row(
-          parts,
-          [&](int s) {
-            return s < pl.splits ? ws.part_ml[first + r + s * stride]
-                                 : ws.suffix_ml[suffix_row + (s - pl.splits) * suffix_stride];
-          },
-          factors[warp]);
-      __syncwarp();
-#pragma unroll 1
-      for (int s0 = sub; s0 < parts; s0 += kInFlight * kJoinWarps) {
-        if (s0 != sub) load(s0);
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
-          const int s = s0 + u * kJoinWarps;
-          if (s < parts) add_part(v, y[u], factors[warp][s]);
-        }
-      }
-      if (lane == 0 && sub == 0) {
+  if (int(blockIdx.x) >= blocks) {
+    for (int row = warp; row < live; row += kJoinThreads / 32) {
+      place(row, first, r, suffix_row);
+      const RowJoin j = join(first, r, suffix_row);
+      if (lane == 0) {
         row_m[row] = j.m;
         row_r[row] = j.inv;
-        if (chunk == 0) {
-          if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
-          if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
-        }
       }
     }
-    if (lane < D / 4) sums[warp][lane] = v;
     __syncthreads();
-    if (row < live && sub == 0 && chunk == 0 && lane < D / 4) {
-#pragma unroll
-      for (int w = 1; w < kJoinWarps; ++w) add_part(v, sums[warp + w][lane], 1.f);
-      store_piece<D>(a, b, h, row, lane, v);
-    }
-    __syncthreads();
-  }
-  if (a.sw) {
-    const int n = suffix_len(a, b), chunks = gridDim.x;
+    const int n = suffix_len(a, b), chunk = blockIdx.x - blocks, chunks = gridDim.x - blocks;
     add_suffix_weights(a, ws, scale_log2, b, h, n, int((long long)n * chunk / chunks),
                        int((long long)n * (chunk + 1) / chunks), row_m, row_r);
+    return;
+  }
+  const int row = blockIdx.x * kJoinRows + warp / kJoinWarps, sub = warp % kJoinWarps;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row < live) {
+    place(row, first, r, suffix_row);
+    const float* pre = ws.part_o + first * D + part_offset<D>(r, lane * 4);
+    const float* suf = ws.suffix_o + suffix_row * D + lane * 4;
+    float4 y[kInFlight];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int s = s0 + u * kJoinWarps;
+        if (s < parts && lane < D / 4)
+          y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
+                                                                : suf + (s - pl.splits) * suffix_stride * D);
+      }
+    };
+    load(sub);
+    const RowJoin j = join(first, r, suffix_row);
+    __syncwarp();
+#pragma unroll 1
+    for (int s0 = sub; s0 < parts; s0 += kInFlight * kJoinWarps) {
+      if (s0 != sub) load(s0);
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int s = s0 + u * kJoinWarps;
+        if (s < parts) add_part(v, y[u], factors[warp][s]);
+      }
+    }
+    if (lane == 0 && sub == 0) {
+      if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
+      if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+    }
+  }
+  if (lane < D / 4) sums[warp][lane] = v;
+  __syncthreads();
+  if (row < live && sub == 0 && lane < D / 4) {
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) add_part(v, sums[warp + w][lane], 1.f);
+    store_piece<D>(a, b, h, row, lane, v);
   }
 }
 
@@ -545,16 +582,16 @@ cudaError_t launch_shape(const SharedAttnArgs& a, const Plan& p, const Workspace
   constexpr int smem = RowsShape<D, NB>::smem;
   const cudaError_t e = allow_smem<shared_rows_kernel<D, NB, SOLO>>(smem);
   if (e != cudaSuccess) return e;
-  DependentLaunch d(dim3(p.suffix_splits, a.kv_heads, a.batch), kThreads, smem, stream, SOLO ? p.suffix_splits : 1);
+  const int blocks = (a.rows * a.group + 8 * NB - 1) / (8 * NB);
+  DependentLaunch d(dim3(p.suffix_splits, a.kv_heads * blocks, a.batch), kThreads, smem, stream,
+                    SOLO ? p.suffix_splits : 1);
   return cudaLaunchKernelEx(&d.cfg, shared_rows_kernel<D, NB, SOLO>, a, p, ws, attention_scale(D) * kLog2e);
 }
 
 template <int D, bool SOLO>
 cudaError_t launch_width(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  const int live = a.rows * a.group;
-  return live <= 8    ? launch_shape<D, 1, SOLO>(a, p, ws, stream)
-         : live <= 16 ? launch_shape<D, 2, SOLO>(a, p, ws, stream)
-                      : launch_shape<D, 4, SOLO>(a, p, ws, stream);
+  return a.rows * a.group <= 8 ? launch_shape<D, 1, SOLO>(a, p, ws, stream)
+                               : launch_shape<D, 2, SOLO>(a, p, ws, stream);
 }
 
 }  // namespace
@@ -565,8 +602,9 @@ cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace&
 }
 
 cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  const int chunks = a.sw ? std::min(16, (a.scap + 1023) / 1024) : 1;
-  DependentLaunch d(dim3(chunks, a.kv_heads, a.batch), kJoinThreads, 0, stream);
+  const int chunks = a.sw ? std::min(16, (a.scap + kJoinThreads - 1) / kJoinThreads) : 0;
+  DependentLaunch d(dim3((a.rows * a.group + kJoinRows - 1) / kJoinRows + chunks, a.kv_heads, a.batch), kJoinThreads, 0,
+                    stream);
   const float scale = attention_scale(a.width) * kLog2e;
   const cudaError_t e = a.width == 64 ? allow_smem<shared_join_kernel<64>>(0) : allow_smem<shared_join_kernel<128>>(0);
   if (e != cudaSuccess) return e;
