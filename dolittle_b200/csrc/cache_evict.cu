@@ -463,13 +463,16 @@ cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cud
   int ctas = 1;
   while (ctas < kMaxCtas && a.capacity > 8 * kThreads * ctas) ctas *= 2;
   const int tiles = (a.capacity + ctas * kThreads - 1) / (ctas * kThreads);
-  // Moving in the selecting CTAs saves the second kernel's start (2 us) while
-  // they are few rows each and one wave; not when the lengths are updated in
-  // place, since a CTA of another head may still have to read them.
+  // Moving in the selecting CTAs when they fill the SMs, in one wave, with few
+  // rows each: some copy while others still select.  Below that the second
+  // kernel's even spread is faster (microseconds, moving there / here: 2 caches
+  // of 320 slots to 256 8.3 / 11.2, 8 of 1024 to 512 16.4 / 22.8, 32 of 320 to
+  // 256 22.6 / 20.7, 36 of 1024 to 512 40.7 / 37.9).  Not when the lengths are
+  // updated in place, since a CTA of another head may still have to read them.
   const int own_rows = std::min(a.budget, tiles * kThreads);
   const size_t bytes = size_t(own_rows) * a.width * 4;
-  const bool move =
-      tiles <= 8 && bytes <= (size_t(256) << 10) && units * ctas <= 2 * sms && a.lengths_out != a.lengths;
+  const bool move = tiles <= 8 && bytes <= (size_t(256) << 10) && units * ctas > sms && units * ctas <= 2 * sms &&
+                    a.lengths_out != a.lengths;
   const size_t smem = size_t(tiles) * kWarps * 8 + (tiles <= 32 ? size_t(tiles) * kThreads * 4 : 0) +
                       (move ? size_t(own_rows) * 4 : 0);
   cudaLaunchConfig_t cfg = {};

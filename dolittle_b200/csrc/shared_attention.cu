@@ -23,60 +23,128 @@ namespace {
 
 using namespace sa;
 
-// Prefix elements, over all sequences, up to which reading the prefix once per
-// sequence from L2 costs less than a second kernel.
-constexpr size_t kSoloElements = size_t(4) << 20;
+// How a call is cut is chosen by an estimate of its time in microseconds, with
+// constants measured on a B200 (148 SMs; 32 query and 8 KV heads of width 128
+// unless said otherwise).  The alternatives measured against one another:
+//
+//   few-row kernel alone / beside tiles, one token: batch 8 on 1024 + 64 keys
+//     10.9 / 13.2, batch 64 on 256 + 64 14.1 / 20; batch 2 on 8192 + 64 24.1 /
+//     19.7, batch 16 on 2048 + 64 21.1 / 14.0
+//   few rows beside tiles / tiles per sequence: batch 32 of one token on 8192 +
+//     256 keys 24 / 183, batch 8 of 8 tokens on 8192 + 256 27 / 56; batch 16 of
+//     8 tokens on 1024 + 128 21.4 / 18.6
+//   key ranges of the pooled tiles, batch 64 of one token on 32768 + 2048 keys
+//     (16 row tiles): 2 203, 4 119, 6 119, 9 139: ranges beyond an SM's fair
+//     share of the products take the room that the suffixes stream through
+//   one / two row tiles per CTA: batch 8 of 48 tokens on 4096 + 112 keys 49.3
+//     (whole) / 57.5 (two ranges); batch 8 of 512 on 8192 + 512 662 / 638
+inline int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
-// CTAs per (sequence, KV head) of the few-row kernel: the fewest waves x time
-// of a CTA, in units of a step of 64 keys at the HBM rate shared by three
-// resident CTAs (about 2.2 us); start and join cost about 1.4 such steps.
-int suffix_splits(long long units, int keys, int slots) {
-  int best = 1;
+// Tiles of row tiles alone (a turn, a document): sets per_cta, groups, tasks,
+// full and splits.  A step is a pair of a row tile and a key tile on each
+// stream, 2.3 us; a split costs the merge kernel and 42 ns per 128-row part.
+double plan_tiles(const SharedAttnArgs& a, int key_tiles, int units, int sms, Plan* best) {
   double best_cost = 0;
-  for (int s = 1; s <= kMaxSuffixSplits; s *= 2) {
-    const double waves = double((units * s + slots - 1) / slots), steps = (keys + 64 * s - 1) / (64 * s);
-    const double cost = waves * (steps + 1.4);
-    if (s == 1 || cost < best_cost) {
-      best = s;
+  for (int per_cta = 1; per_cta <= (best->tiles > 1 ? 2 : 1); ++per_cta) {
+    Plan p = *best;
+    p.per_cta = per_cta;
+    p.groups = ceil_div(p.tiles, per_cta);
+    p.tasks = p.groups * units;
+    // Whole tasks fill the SMs as often as they can; what is left is cut into
+    // key ranges that fill them once more, if that pays.
+    const int whole = p.tasks / sms * sms, rest = p.tasks - whole;
+    auto steps = [&](int splits) { return per_cta == 2 ? ceil_div(key_tiles, splits) : ceil_div(key_tiles, 2 * splits); };
+    for (int s = 1; s <= std::max(1, std::min({rest ? sms / rest : 1, key_tiles / 2, kMaxSplits})); ++s) {
+      const int waves = ceil_div(p.tasks, sms);
+      const double cost = 7 + (per_cta == 2 ? 2.3 : 2.37) * (whole / sms * steps(1) + (rest ? steps(s) : 0)) +
+                          4 * (waves - 1) + (s > 1 ? 3 + 0.042 * s * rest * per_cta * a.width / 128 : 0);
+      if (best_cost && cost >= best_cost) continue;
       best_cost = cost;
+      p.splits = s;
+      p.full = s == 1 ? p.tasks : whole;
+      *best = p;
     }
   }
-  return best;
+  return best_cost;
+}
+
+// The few-row kernel alone: sets suffix_splits.  A step is 64 keys of a CTA, of
+// which four fit an SM.
+double plan_solo(const SharedAttnArgs& a, int units, int sms, Plan* best) {
+  const double step = (a.rows * a.group > 8 ? 1.5 : 1) * a.width / 128;
+  double best_cost = 0;
+  for (int s = 1; s <= kMaxSuffixSplits; s *= 2) {
+    const int ctas = units * s, waves = ceil_div(ctas, 4 * sms), beside = std::min(4, ceil_div(ctas, sms));
+    const double cost = waves * (3.4 + 0.4 * beside +
+                                 std::max(1.05, 0.45 * beside) * step * ceil_div(a.scap + a.pcap, 64 * s)) +
+                        (s > 1 ? 1 : 0);
+    if (best_cost && cost >= best_cost) continue;
+    best_cost = cost;
+    best->suffix_splits = s;
+  }
+  return best_cost;
+}
+
+// The few-row kernel over the suffixes beside the tile kernel over the prefix:
+// sets splits and suffix_splits.  An SM holds a tile CTA and a few-row CTA, or
+// four of the latter.
+double plan_beside(const SharedAttnArgs& a, int key_tiles, int units, int sms, Plan* best) {
+  const double width = a.width / 128.0, few = a.rows * a.group > 8 ? 1.5 : 1;
+  const double rows = double(a.batch) * a.rows * a.query_heads;
+  const double bytes = (double(a.pcap) + double(a.batch) * a.scap) * a.kv_heads * a.width * 4;
+  const int blocks = units * ceil_div(a.rows * a.group, a.rows * a.group > 8 ? kMostRows : 8);
+  double best_cost = 0;
+  for (int splits = 1; splits <= std::max(1, std::min({sms / best->tasks, (key_tiles + 1) / 2, kMaxSplits})); ++splits) {
+    const int ctas = best->tasks * splits, waves = ceil_div(ctas, sms);
+    const double tile = 6.3 + waves * (0.7 + 3.2 * ceil_div(key_tiles, 2 * splits));
+    const int slots = waves == 1 ? ctas + 4 * (sms - ctas) : sms;
+    for (int s = 1; s <= kMaxSuffixSplits; s *= 2) {
+      const double one = few * (2.8 + 1.6 * width * ceil_div(a.scap, 64 * s));
+      double suffix = one * ceil_div((long long)blocks * s, slots);
+      if (suffix > tile) suffix = std::max(one, tile + (suffix - tile) * slots / (4 * sms));
+      const double cost = std::max({tile, suffix, bytes / 6.9e6}) + join_cost(rows, splits + s, sms).time * width;
+      if (best_cost && cost >= best_cost) continue;
+      best_cost = cost;
+      best->splits = splits;
+      best->suffix_splits = s;
+    }
+  }
+  return best_cost;
 }
 
 Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
+  const int tokens = a.batch * a.rows, units = a.batch * a.kv_heads;
+  const int prefix_tiles = ceil_div(a.pcap, kKeys), suffix_tiles = ceil_div(a.scap, kKeys);
   Plan p = {};
-  const int tokens = a.batch * a.rows;
   p.per_tile = kRows / a.group;
-  p.pooled = a.rows * a.group <= kFewRows;
-  const int unit_tokens = p.pooled ? tokens : a.rows;
-  p.tiles = (unit_tokens + p.per_tile - 1) / p.per_tile;
-  const int units = a.batch * a.kv_heads;
-  p.per_cta = p.tiles > 1 ? 2 : 1;
-  p.groups = (p.tiles + p.per_cta - 1) / p.per_cta;
-  p.tasks = p.groups * (p.pooled ? a.kv_heads : units);
-  const int prefix_tiles = (a.pcap + kKeys - 1) / kKeys, suffix_tiles = (a.scap + kKeys - 1) / kKeys;
-  const int key_tiles = prefix_tiles + (p.pooled ? 0 : suffix_tiles);
-  // Whole tasks fill the SMs as often as they can; what is left is cut into
-  // key ranges (of two key tiles at least) that fill them once more.  Pooled
-  // tasks are always joined with a suffix, so they are all cut alike.
-  p.full = p.pooled ? 0 : p.tasks / sms * sms;
-  const int rest = p.tasks - p.full;
-  p.splits = std::max(1, std::min({sms / std::max(1, rest), key_tiles / 2, kMaxSplits}));
-  // No more ranges than their longest one needs to stay as short as it is.
-  const int longest = (key_tiles + p.splits - 1) / p.splits;
-  const int step = p.per_cta == 2 ? longest : (longest + 1) / 2 * 2;  // two streams share a narrow task's key tiles
-  if (key_tiles) p.splits = std::min(p.splits, (key_tiles + step - 1) / step);
-  if (!p.pooled && p.splits == 1) p.full = p.tasks;
-  // (Not with rows for two CTAs, which could not add a key's weight together.)
-  if (p.pooled && a.rows * a.group <= kMostRows && units * size_t(a.pcap) * a.width <= kSoloElements) p.splits = 0;
-  const int unit_keys = a.scap + (p.splits ? 0 : a.pcap);
-  p.suffix_splits = p.pooled ? suffix_splits(units, unit_keys, 3 * sms) : 1;
+  p.tiles = ceil_div(a.rows, p.per_tile);
+  p.suffix_splits = 1;
+  const double by_sequence = plan_tiles(a, prefix_tiles + suffix_tiles, units, sms, &p);
+  if (a.rows * a.group <= kFewRows) {
+    Plan q = p;
+    q.pooled = true;
+    q.tiles = q.groups = ceil_div(tokens, q.per_tile);
+    q.tasks = q.tiles * a.kv_heads;
+    q.per_cta = 1;
+    q.full = 0;
+    double cost = plan_beside(a, prefix_tiles, units, sms, &q);
+    // (Rows for two CTAs could not add a key's weight together.)
+    if (a.rows * a.group <= kMostRows) {
+      Plan solo = q;
+      solo.splits = 0;
+      const double alone = plan_solo(a, units, sms, &solo);
+      if (alone < cost) {
+        q = solo;
+        cost = alone;
+      }
+    }
+    if (cost < by_sequence) p = q;
+  }
   p.weight_ranks = 1;
   if (weights) {
     const long long key_units =  // pairs of key tiles
         ((prefix_tiles + 1) / 2 + (long long)(p.pooled ? 0 : (suffix_tiles + 1) / 2) * a.batch) * a.kv_heads;
-    const int row_tiles = (tokens + p.per_tile - 1) / p.per_tile;
+    const int row_tiles = ceil_div(tokens, p.per_tile);
     while (p.weight_ranks < 8 && key_units * p.weight_ranks * 2 <= sms && row_tiles >= 2 * p.weight_ranks)
       p.weight_ranks *= 2;
   }
@@ -101,7 +169,7 @@ size_t lay_out(const SharedAttnArgs& a, const Plan& p, bool weights, char* base,
   ws->suffix_o = reinterpret_cast<float*>(take(suffix_rows * a.width * 4));
   ws->suffix_ml = reinterpret_cast<float2*>(take(suffix_rows * 8));
   ws->norm = reinterpret_cast<RowNorm*>(take(weights ? rows * 8 : 0));
-  ws->scores = reinterpret_cast<float*>(take(weights && p.pooled ? rows * a.scap * 4 : 0));
+  ws->scores = reinterpret_cast<float*>(take(weights && p.pooled ? rows * score_pitch(a) * 4 : 0));
   return std::max<size_t>(at, 256);
 }
 
@@ -119,7 +187,7 @@ cudaError_t launch_shared_attention(const SharedAttnArgs& a, void* workspace, in
   lay_out(a, p, weights, static_cast<char*>(workspace), &ws);
   cudaError_t e = p.splits ? launch_tiles(a, p, ws, stream) : cudaSuccess;
   if (e == cudaSuccess && p.pooled) e = launch_rows(a, p, ws, stream);
-  if (e == cudaSuccess && p.pooled && p.splits) e = launch_join(a, p, ws, stream);
+  if (e == cudaSuccess && p.pooled && p.splits) e = launch_join(a, p, ws, sms, stream);
   if (e == cudaSuccess && !p.pooled && p.full < p.tasks) e = launch_merge(a, p, ws, stream);
   if (e == cudaSuccess && (a.pw || (a.sw && !p.pooled))) e = launch_weights(a, p, ws, sms, stream);
   return e;

@@ -2,6 +2,7 @@
 // length arithmetic, the workspace, tensor-core and copy primitives.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -37,8 +38,11 @@ struct Workspace {
   float* suffix_o;    // [suffix splits][B][Hkv][rows x group][D]
   float2* suffix_ml;  // [suffix splits][B][Hkv][rows x group]
   RowNorm* norm;    // [tokens * Hq]
-  float* scores;    // [B][Hq * rows][scap]
+  float* scores;    // [B][Hq * rows][score_pitch]
 };
+
+// Suffix scores of a row, in 16-byte pieces.
+__host__ __device__ __forceinline__ int score_pitch(const SharedAttnArgs& a) { return (a.scap + 3) / 4 * 4; }
 
 // How a call is cut into work, from sizes alone.
 struct Plan {
@@ -54,10 +58,24 @@ struct Plan {
   int weight_ranks;   // CTAs (one cluster) per pair of key tiles in the weights kernel
 };
 
+// Warps that share a row in the join kernel (four, or one when that would take
+// several waves of blocks and there are few parts: 4096 rows of 6 parts 12 us
+// with four and 5 us with one, 2048 rows of 22 parts 7 us and 11 us), and the
+// time of the join in microseconds.
+struct JoinCost {
+  int warps;
+  double time;
+};
+inline JoinCost join_cost(double rows, int parts, int sms) {
+  const double four = std::max(1.0, rows / (8 * sms)) * (2 + 1.5 * ((parts + 19) / 20));
+  const double one = std::max(1.0, rows / (32 * sms)) * (2 + 1.5 * ((parts + 4) / 5));
+  return {four <= one ? 4 : 1, std::min(four, one) + 2.56e-4 * rows * parts};
+}
+
 cudaError_t launch_tiles(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_merge(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
 cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
-cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream);
+cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream);
 cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream);
 
 // Launch configuration of a programmatic dependent launch (every kernel here

@@ -22,6 +22,7 @@
 #include "shared_attention.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace dl {
 namespace sa {
@@ -161,19 +162,61 @@ __device__ __forceinline__ void store_piece(const SharedAttnArgs& a, int b, int 
 }
 
 // Adds the weights of suffix keys [j0, j1) of unit (b, h) to their sums, from
-// the stored scores and the rows' norms in shared memory.
+// the stored scores and the rows' norms in shared memory, which are there when
+// ready() returns; one of `threads`, which all call ready() once.  j0 is a
+// multiple of 4, j1 at most the suffix length n.  The scores of four rows x
+// eight keys are in flight together (one key after another took as long as a
+// kernel: 9 us of a step of batch 32).
+template <class Ready>
 __device__ __forceinline__ void add_suffix_weights(const SharedAttnArgs& a, const Workspace& ws, float scale_log2, int b,
                                                    int h, int n, int j0, int j1, const float* row_m,
-                                                   const float* row_r) {
-  const int live = a.rows * a.group;
+                                                   const float* row_r, int thread, int threads, Ready&& ready) {
+  constexpr int kPieces = 1, kAtOnce = 4;  // of 4 keys; rows
+  const int live = a.rows * a.group, pitch = score_pitch(a);
   float* sums = a.sw + (size_t(b) * a.kv_heads + h) * a.scap;
-  const float* scores = ws.scores + (size_t(b) * a.kv_heads + h) * live * a.scap;
-  for (int j = j0 + int(threadIdx.x); j < j1; j += blockDim.x) {
-    float w = 0.f;
-    for (int row = 0; row < live; ++row)
-      if (j < suffix_seen(n, a.rows, row / a.group))
-        w = fmaf(exp2_approx(fmaf(scores[size_t(row) * a.scap + j], scale_log2, -row_m[row])), row_r[row], w);
-    sums[j] += w;
+  const float* scores = ws.scores + (size_t(b) * a.kv_heads + h) * live * pitch;
+  bool waiting = true;
+  for (int base = j0; base < j1 || waiting; base += 4 * kPieces * threads) {
+    float w[kPieces][4] = {}, old[kPieces][4];
+    int j[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      j[p] = base + 4 * (thread + p * threads);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) old[p][k] = j[p] + k < j1 ? sums[j[p] + k] : 0.f;
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < live; r0 += kAtOnce) {
+      float4 y[kAtOnce][kPieces];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r)
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+          if (r0 + r < live && j[p] < j1)
+            y[r][p] = *reinterpret_cast<const float4*>(scores + size_t(r0 + r) * pitch + j[p]);
+      if (waiting) {
+        ready();
+        waiting = false;
+      }
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) {
+        if (r0 + r >= live) break;
+        const int seen = min(j1, suffix_seen(n, a.rows, (r0 + r) / a.group));
+        const float m = row_m[r0 + r], f = row_r[r0 + r];
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          const float x[4] = {y[r][p].x, y[r][p].y, y[r][p].z, y[r][p].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (j[p] + k < seen) w[p][k] = fmaf(exp2_approx(fmaf(x[k], scale_log2, -m)), f, w[p][k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j[p] + k < j1) sums[j[p] + k] = old[p][k] + w[p][k];
   }
 }
 
@@ -272,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
 #pragma unroll
       for (int f = 0; f < D / 16; ++f) o[nb][f][0] = o[nb][f][1] = o[nb][f][2] = o[nb][f][3] = 0.f;
     }
-    float* scores = a.sw ? ws.scores + ((size_t(b) * a.kv_heads + h) * unit_rows + row0) * a.scap : nullptr;
+    float* scores = a.sw ? ws.scores + ((size_t(b) * a.kv_heads + h) * unit_rows + row0) * score_pitch(a) : nullptr;
 
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
@@ -307,8 +350,8 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
         for (int u = 0; u < 2; ++u) {
           const int row = 8 * nb + c2 + u, end = row < rows ? (pre ? np : seen[nb][u]) : 0;
           if (scores && row < rows && !pre) {
-            if (ka < n) scores[size_t(row) * a.scap + ka] = s[nb][u];
-            if (kb < n) scores[size_t(row) * a.scap + kb] = s[nb][2 + u];
+            if (ka < n) scores[size_t(row) * score_pitch(a) + ka] = s[nb][u];
+            if (kb < n) scores[size_t(row) * score_pitch(a) + kb] = s[nb][2 + u];
           }
           if (ka >= end) s[nb][u] = -INFINITY;
           if (kb >= end) s[nb][2 + u] = -INFINITY;
@@ -476,38 +519,42 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
     store_piece<D>(a, b, h, row0 + row, (i % (D / 4)) ^ (row & 7), v);
   }
   if (a.sw)  // of this CTA's suffix keys
-    add_suffix_weights(a, ws, scale_log2, b, h, n, max(0, g0 - ps) * kStep, min(n, max(0, g1 - ps) * kStep), row_m, row_r);
+    add_suffix_weights(a, ws, scale_log2, b, h, n, max(0, g0 - ps) * kStep, min(n, max(0, g1 - ps) * kStep), row_m, row_r, t,
+                       kThreads, [] {});
   if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Joins the prefix ranges and the suffix ranges of the rows of unit (b, h).
-// Bound by latency (a few KB per block), so the work is spread thin: a block
-// takes four rows, four warps share a row, each every fourth part with all its
-// loads in flight, lane = 16-byte piece of the row; every one of them makes the
-// row's factors itself.  With weights, further blocks of the unit add the sums
-// of a chunk of its suffix keys each.
-constexpr int kJoinThreads = 512, kJoinWarps = 4;                // warps of a row
-constexpr int kJoinRows = kJoinThreads / 32 / kJoinWarps;        // rows of a block
-constexpr int kInFlight = 5;                                     // parts that a warp has in flight
+// Joins the prefix ranges and the suffix ranges of each row.  Bound by latency
+// (a few KB per block), so the work is spread thin: W warps share a row, each
+// every W-th part with all its loads in flight, lane = 16-byte piece of the row;
+// every one of them makes the row's factors itself.  With weights, the first
+// blocks add the sums of the suffix keys, two warps for each chunk of a
+// (sequence, KV head).
+constexpr int kJoinThreads = 512;
+constexpr int kInFlight = 5;  // parts that a warp has in flight
+constexpr int kChunkThreads = 128, kChunkKeys = 512, kChunks = kJoinThreads / kChunkThreads;  // of a block
 
-template <int D>
+template <int D, int W>
 __global__ void __launch_bounds__(kJoinThreads, 2) shared_join_kernel(const SharedAttnArgs a, const Plan pl,
-                                                                  const Workspace ws, const float scale_log2) {
-  __shared__ float row_m[kFewRows], row_r[kFewRows], factors[kJoinThreads / 32][kMaxParts];
+                                                                  const Workspace ws, const float scale_log2,
+                                                                  const int weight_blocks, const int chunks) {
+  __shared__ float row_m[kChunks][kFewRows], row_r[kChunks][kFewRows], factors[kJoinThreads / 32][kMaxParts];
   __shared__ float4 sums[kJoinThreads / 32][D / 4];
-  const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int live = a.rows * a.group, blocks = (live + kJoinRows - 1) / kJoinRows;
-  const int parts = pl.splits + pl.suffix_splits;
-  const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;       // rows between two prefix ranges
-  const size_t suffix_stride = size_t(a.batch) * a.kv_heads * live;  // and two suffix ranges
-  // The row's place in a prefix range, and in its tile; in a suffix range.
-  auto place = [&](int row, size_t& first, int& r, size_t& suffix_row) {
-    const int token = b * a.rows + row / a.group, tile = token / pl.per_tile;
-    r = token % pl.per_tile * a.group + row % a.group;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit_rows = a.rows * a.group, parts = pl.splits + pl.suffix_splits;
+  const size_t stride = size_t(pl.tasks) * pl.per_cta * kRows;            // rows between two prefix ranges
+  const size_t suffix_stride = size_t(a.batch) * a.kv_heads * unit_rows;  // and two suffix ranges
+  // Row of query head hq of a token: its tile's first row in a prefix range, its
+  // place in the tile, its place in a suffix range.
+  size_t first, suffix_row;
+  int r;
+  auto place = [&](int token, int hq) {
+    const int h = hq / a.group, tile = token / pl.per_tile;
+    r = token % pl.per_tile * a.group + hq % a.group;
     first = (size_t(h * pl.groups + tile / pl.per_cta) * pl.per_cta + tile % pl.per_cta) * kRows;
-    suffix_row = (size_t(b) * a.kv_heads + h) * live + row;
+    suffix_row = (size_t(token / a.rows) * a.kv_heads + h) * unit_rows + token % a.rows * a.group + hq % a.group;
   };
-  auto join = [&](size_t first, int r, size_t suffix_row) {
+  auto join = [&] {
     return join_row(
         parts,
         [&](int s) {
@@ -516,64 +563,71 @@ __global__ void __launch_bounds__(kJoinThreads, 2) shared_join_kernel(const Shar
         },
         factors[warp]);
   };
-  size_t first, suffix_row;
-  int r;
   wait_prior();
   allow_next();
-  if (int(blockIdx.x) >= blocks) {
-    for (int row = warp; row < live; row += kJoinThreads / 32) {
-      place(row, first, r, suffix_row);
-      const RowJoin j = join(first, r, suffix_row);
-      if (lane == 0) {
-        row_m[row] = j.m;
-        row_r[row] = j.inv;
-      }
-    }
-    __syncthreads();
-    const int n = suffix_len(a, b), chunk = blockIdx.x - blocks, chunks = gridDim.x - blocks;
-    add_suffix_weights(a, ws, scale_log2, b, h, n, int((long long)n * chunk / chunks),
-                       int((long long)n * (chunk + 1) / chunks), row_m, row_r);
+  if (int(blockIdx.x) < weight_blocks) {
+    const int mine = threadIdx.x / kChunkThreads, thread = threadIdx.x % kChunkThreads;
+    const int at = blockIdx.x * kChunks + mine, unit = at / chunks, chunk = at % chunks;
+    const int h = unit % a.kv_heads, b = unit / a.kv_heads;
+    const int n = b < a.batch ? suffix_len(a, b) : 0;
+    add_suffix_weights(a, ws, scale_log2, min(b, a.batch - 1), h, n, chunk * kChunkKeys, min(n, (chunk + 1) * kChunkKeys),
+                       row_m[mine], row_r[mine], thread, kChunkThreads, [&] {
+                         for (int row = thread / 32; row < unit_rows && b < a.batch; row += kChunkThreads / 32) {
+                           place(b * a.rows + row / a.group, h * a.group + row % a.group);
+                           const RowJoin j = join();
+                           if (lane == 0) {
+                             row_m[mine][row] = j.m;
+                             row_r[mine][row] = j.inv;
+                           }
+                         }
+                         __syncthreads();
+                       });
     return;
   }
-  const int row = blockIdx.x * kJoinRows + warp / kJoinWarps, sub = warp % kJoinWarps;
+  const int row = (blockIdx.x - weight_blocks) * (kJoinThreads / 32 / W) + warp / W, sub = warp % W;
+  const int token = row / a.query_heads, hq = row % a.query_heads;
+  const bool live = token < a.batch * a.rows;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (row < live) {
-    place(row, first, r, suffix_row);
+  if (live) {
+    place(token, hq);
     const float* pre = ws.part_o + first * D + part_offset<D>(r, lane * 4);
     const float* suf = ws.suffix_o + suffix_row * D + lane * 4;
     float4 y[kInFlight];
     auto load = [&](int s0) {
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
-        const int s = s0 + u * kJoinWarps;
+        const int s = s0 + u * W;
         if (s < parts && lane < D / 4)
           y[u] = *reinterpret_cast<const float4*>(s < pl.splits ? pre + s * stride * D
                                                                 : suf + (s - pl.splits) * suffix_stride * D);
       }
     };
     load(sub);
-    const RowJoin j = join(first, r, suffix_row);
+    const RowJoin j = join();
     __syncwarp();
 #pragma unroll 1
-    for (int s0 = sub; s0 < parts; s0 += kInFlight * kJoinWarps) {
+    for (int s0 = sub; s0 < parts; s0 += kInFlight * W) {
       if (s0 != sub) load(s0);
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
-        const int s = s0 + u * kJoinWarps;
+        const int s = s0 + u * W;
         if (s < parts) add_part(v, y[u], factors[warp][s]);
       }
     }
     if (lane == 0 && sub == 0) {
-      if (a.lse) a.lse[row_index(a, b, h, row)] = j.lse;
-      if (a.pw) ws.norm[row_index(a, b, h, row)] = RowNorm{j.m, j.inv};
+      if (a.lse) a.lse[row] = j.lse;
+      if (a.pw) ws.norm[row] = RowNorm{j.m, j.inv};
     }
   }
-  if (lane < D / 4) sums[warp][lane] = v;
-  __syncthreads();
-  if (row < live && sub == 0 && lane < D / 4) {
+  if constexpr (W > 1) {
+    if (lane < D / 4) sums[warp][lane] = v;
+    __syncthreads();
+  }
+  if (live && sub == 0 && lane < D / 4) {
 #pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) add_part(v, sums[warp + w][lane], 1.f);
-    store_piece<D>(a, b, h, row, lane, v);
+    for (int w = 1; w < W; ++w) add_part(v, sums[warp + w][lane], 1.f);
+    reinterpret_cast<uint2*>(a.out + size_t(token) * a.ldo + size_t(hq) * D)[lane] =
+        make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
   }
 }
 
@@ -594,6 +648,21 @@ cudaError_t launch_width(const SharedAttnArgs& a, const Plan& p, const Workspace
                                : launch_shape<D, 2, SOLO>(a, p, ws, stream);
 }
 
+template <int D, int W>
+cudaError_t launch_join_shape(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
+  const cudaError_t e = allow_smem<shared_join_kernel<D, W>>(0);
+  if (e != cudaSuccess) return e;
+  constexpr int at_once = kJoinThreads / 32 / W;
+  const long long blocks = ((long long)a.batch * a.rows * a.query_heads + at_once - 1) / at_once;
+  const int chunks = a.sw ? (a.scap + kChunkKeys - 1) / kChunkKeys : 0;
+  const long long weight_blocks = ((long long)a.batch * a.kv_heads * chunks + kChunks - 1) / kChunks;
+  const long long grid = blocks + weight_blocks;
+  if (grid > INT_MAX / kChunks) return cudaErrorInvalidValue;
+  DependentLaunch d(dim3(unsigned(grid)), kJoinThreads, 0, stream);
+  return cudaLaunchKernelEx(&d.cfg, shared_join_kernel<D, W>, a, p, ws, attention_scale(D) * kLog2e,
+                            int(weight_blocks), chunks);
+}
+
 }  // namespace
 
 cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
@@ -601,15 +670,10 @@ cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace&
   return a.width == 64 ? launch_width<64, false>(a, p, ws, stream) : launch_width<128, false>(a, p, ws, stream);
 }
 
-cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, cudaStream_t stream) {
-  const int chunks = a.sw ? std::min(16, (a.scap + kJoinThreads - 1) / kJoinThreads) : 0;
-  DependentLaunch d(dim3((a.rows * a.group + kJoinRows - 1) / kJoinRows + chunks, a.kv_heads, a.batch), kJoinThreads, 0,
-                    stream);
-  const float scale = attention_scale(a.width) * kLog2e;
-  const cudaError_t e = a.width == 64 ? allow_smem<shared_join_kernel<64>>(0) : allow_smem<shared_join_kernel<128>>(0);
-  if (e != cudaSuccess) return e;
-  return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_join_kernel<64>, a, p, ws, scale)
-                       : cudaLaunchKernelEx(&d.cfg, shared_join_kernel<128>, a, p, ws, scale);
+cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream) {
+  const bool four = join_cost(double(a.batch) * a.rows * a.query_heads, p.splits + p.suffix_splits, sms).warps == 4;
+  if (a.width == 64) return four ? launch_join_shape<64, 4>(a, p, ws, stream) : launch_join_shape<64, 1>(a, p, ws, stream);
+  return four ? launch_join_shape<128, 4>(a, p, ws, stream) : launch_join_shape<128, 1>(a, p, ws, stream);
 }
 
 }  // namespace sa

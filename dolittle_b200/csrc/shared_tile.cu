@@ -42,9 +42,10 @@ constexpr float kRescale = 8.f;     // base-2 growth of the maximum that moves t
 // suffixes while this one is busy with products.
 template <int D, bool WIDE, bool BESIDE>
 struct Shape {
+  static_assert(!(WIDE && BESIDE), "room for a few-row block is left by one row tile only");
   static constexpr int slot = D / 64 * kAtom;  // a K, V or Q tile
   static constexpr int queries = WIDE ? 2 : 1;
-  static constexpr int stages = D == 64 ? 8 : !WIDE ? 4 : BESIDE ? 3 : 5;
+  static constexpr int stages = D == 64 ? 8 : WIDE ? 5 : 4;
   static constexpr int smem = (queries + stages) * slot + 1024;
   static constexpr int bound = BESIDE ? 512 : kThreads;  // threads that the registers are shared out for
 };
@@ -662,9 +663,7 @@ cudaError_t launch_tiles_shape(const TileArgs& t, cudaStream_t stream) {
 
 template <int D>
 cudaError_t launch_tiles_width(const TileArgs& t, cudaStream_t stream) {
-  if (t.plan.pooled)
-    return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, true>(t, stream)
-                               : launch_tiles_shape<D, false, true>(t, stream);
+  if (t.plan.pooled) return launch_tiles_shape<D, false, true>(t, stream);
   return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, false>(t, stream)
                              : launch_tiles_shape<D, false, false>(t, stream);
 }
