@@ -227,11 +227,11 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float warp_m[kWarps][R], warp_l[kWarps][R], cta_m[R], cta_l[R], row_m[R], row_r[R];
   __shared__ float part_f[R][kMaxSuffixSplits];
-  const int split = blockIdx.x, h = blockIdx.y % a.kv_heads, b = blockIdx.z;
+  const int split = blockIdx.x % pl.suffix_splits, h = blockIdx.y, b = blockIdx.z;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int g4 = lane >> 2, c2 = (lane & 3) * 2;
   // Row = new token * group + query head of the group; this CTA's from row0 on.
-  const int unit_rows = a.rows * a.group, row0 = blockIdx.y / a.kv_heads * R, live = min(R, unit_rows - row0);
+  const int unit_rows = a.rows * a.group, row0 = blockIdx.x / pl.suffix_splits * R, live = min(R, unit_rows - row0);
   int np = 0, n = 0, ps = 0, g0 = 0, g1 = 0, steps = 0;  // keys of prefix and suffix; steps of 16: prefix steps, this CTA's [g0, g1), per warp
   float o[NB][D / 16][4], m[NB][2], l[NB][2];
   const uint32_t ring = smem_addr(smem) + warp * (kSlots * kStep * D * 2);
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
     if (t < live) ws.suffix_ml[part0 + t] = make_float2(cta_m[t], cta_l[t]);
     // One block outlasts the tile kernel, so that this kernel's end, which the
     // join waits for, is the end of both; the others make room at once.
-    if (split == int(gridDim.x) - 1 && h == int(gridDim.y) - 1 && b == int(gridDim.z) - 1) wait_prior();
+    if (blockIdx.x == gridDim.x - 1 && h == int(gridDim.y) - 1 && b == int(gridDim.z) - 1) wait_prior();
     return;
   }
   const int ctas = pl.suffix_splits;
@@ -637,7 +637,7 @@ cudaError_t launch_shape(const SharedAttnArgs& a, const Plan& p, const Workspace
   const cudaError_t e = allow_smem<shared_rows_kernel<D, NB, SOLO>>(smem);
   if (e != cudaSuccess) return e;
   const int blocks = (a.rows * a.group + 8 * NB - 1) / (8 * NB);
-  DependentLaunch d(dim3(p.suffix_splits, a.kv_heads * blocks, a.batch), kThreads, smem, stream,
+  DependentLaunch d(dim3(p.suffix_splits * blocks, a.kv_heads, a.batch), kThreads, smem, stream,
                     SOLO ? p.suffix_splits : 1);
   return cudaLaunchKernelEx(&d.cfg, shared_rows_kernel<D, NB, SOLO>, a, p, ws, attention_scale(D) * kLog2e);
 }
