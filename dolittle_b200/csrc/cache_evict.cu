@@ -15,6 +15,13 @@
 // the kept count and destinations below it, so moving in place needs no order
 // between rows.  Integer counts and prefix sums only: results do not depend on
 // scheduling.
+//
+// Measured, out of place, 8 heads of width 128: 32 caches of 2304 slots to 2048
+// in 87 us (435 MB, 5.0 TB/s: bound by the copy); one cache of 32768 to 8192 in
+// 36 us, two thirds of it the selection, whose dozen cluster-wide steps of 1 to
+// 2 us each bound it; two caches of 320 to 256 in 8.2 us, two launches.  Fewer
+// and longer CTAs: one cache of 32768 takes 36 us with 8 CTAs per head, 60 with
+// 4, 65 with 2; 32 caches of 2304 take 103 us with one, 117 with two.
 #include <algorithm>
 #include <climits>
 
@@ -459,6 +466,8 @@ size_t cache_evict_workspace_bytes(int caches, int kv_heads, int budget) {
 int cache_evict_most_slots() { return kMaxCtas * kMostTiles * kThreads; }
 
 cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  // A CTA takes up to eight slots per thread, in registers; more CTAs per head
+  // beyond that (measured above).
   const int units = a.caches * a.kv_heads;
   int ctas = 1;
   while (ctas < kMaxCtas && a.capacity > 8 * kThreads * ctas) ctas *= 2;

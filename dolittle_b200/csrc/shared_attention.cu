@@ -10,8 +10,9 @@
 //   few new tokens per sequence (rows x group <= 32, a decode step): the tile
 //   kernel over the prefix with the rows of all sequences pooled, beside it the
 //   few-row kernel over every suffix, the join kernel for the two; the weights
-//   kernel for the prefix sums (the join kernel adds the suffix sums).  Small
-//   calls: the few-row kernel alone over prefix and suffix.
+//   kernel for the prefix sums (the join kernel adds the suffix sums);
+//   small calls (rows x group <= 16): the few-row kernel alone over prefix and
+//   suffix, and the weights kernel;
 //   more (a turn, a document): the tile kernel per sequence over prefix and
 //   suffix, the merge kernel if key ranges were split, the weights kernel.
 #include "shared_attention.cuh"
@@ -140,6 +141,9 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
     }
     if (cost < by_sequence) p = q;
   }
+  // The rows of a pair of key tiles are shared by a cluster while that still
+  // leaves SMs idle (4 sequences of 64 tokens, microseconds with 1, 2 and 4
+  // ranks: on 1024 keys 44, 39 and 43, on 8192 keys 98, 113 and 150).
   p.weight_ranks = 1;
   if (weights) {
     const long long key_units =  // pairs of key tiles

@@ -14,6 +14,12 @@
 // the sums of the ones before.  When there are few key tiles, a cluster shares
 // the rows of a pair and rank 0 adds the ranks' sums in order.  The keys were
 // just read by the attention, so they come from L2 while the caches fit it.
+//
+// Measured: 8192 keys x 8 heads against 256 tokens x 4 heads (67 M weights) 38
+// us, 47 % of the exponential unit while a CTA has work; 256 pairs over 148 SMs
+// leave a seventh of the time idle.  Slower: scores of 64 columns in registers
+// at once (108 us against 94 for the whole call), the keys in TMEM (98.3 / 97.6),
+// the norms as one more product step (105.7 / 97.5).
 #include "shared_attention.cuh"
 
 #include <algorithm>
