@@ -154,6 +154,32 @@ def test_attention_matches_definition(batch, rows, prefix, suffix, hq, hkv, d, p
     assert torch.equal(got, got2) and torch.equal(lse, lse2)
 
 
+# Sizes around the limits between the plans: rows of a sequence and KV head in
+# one or two blocks of 16, one or four warps per joined row, one or more chunks
+# of suffix keys, key ranges of one and of two row tiles.
+PLANS = [
+    (64, 4, 300, 20, 32, 8, 128, None, [4 + 7919 * b % 17 for b in range(64)]),
+    (20, 7, 600, 30, 32, 8, 128, [600 - 30 * b for b in range(20)], None),
+    (6, 8, 900, 700, 32, 8, 128, None, [700, 8, 513, 512, 511, 7]),
+    (2, 5, 200, 1100, 20, 4, 64, None, [1100, 1]),
+    (3, 1, 3000, 1300, 16, 1, 128, [3000, 2999, 1], [1300, 1025, 0]),
+    (3, 2, 900, 530, 32, 2, 64, None, None),
+    (60, 1, 1500, 40, 28, 4, 64, None, None),
+    (9, 1, 2600, 600, 32, 1, 128, None, None),
+    (4, 48, 1300, 60, 32, 8, 128, None, [60, 48, 49, 50]),
+    (9, 64, 500, 64, 32, 8, 64, None, None),
+    (1, 200, 2000, 200, 16, 4, 128, None, None),
+]
+
+
+@pytest.mark.parametrize("batch,rows,prefix,suffix,hq,hkv,d,plens,slens", PLANS)
+def test_plans_match_definition_and_repeat(batch, rows, prefix, suffix, hq, hkv, d, plens, slens):
+    t = make(batch, rows, prefix, suffix, hq, hkv, d, seed=batch * 37 + rows, plens=plens, slens=slens)
+    got, lse, _ = check_attention(t)
+    again, lse2, _ = check_attention(t, weights=False)
+    assert torch.equal(got, again) and torch.equal(lse, lse2)
+
+
 @pytest.mark.parametrize("rows", [1, 70])
 def test_growing_and_huge_scores(rows):
     """Every block of keys raises the running maximum; scores up to several hundred."""
@@ -411,6 +437,13 @@ def test_eviction_of_equal_weights(n, capacity, budget):
     c["weights"][:] = 0.5
     c["weights"][:, :, capacity // 2::3] = 0.25
     check_eviction(c, budget, 0, 17, True)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("n,capacity,hkv,d", [(20, 300, 8, 64), (36, 600, 8, 64), (40, 200, 8, 128), (5, 5000, 3, 64)])
+def test_eviction_with_few_and_many_heads(n, capacity, hkv, d, in_place):
+    lengths = [capacity - 13 * b % capacity for b in range(n)]
+    check_eviction(make_caches(n, capacity, hkv, d, seed=n, lengths=lengths), capacity * 2 // 3, 4, 20, in_place)
 
 
 def test_eviction_in_place_with_lengths_of_its_own():
