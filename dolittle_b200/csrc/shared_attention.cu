@@ -11,8 +11,8 @@
 //   kernel over the prefix with the rows of all sequences pooled, beside it the
 //   few-row kernel over every suffix, the join kernel for the two; the weights
 //   kernel for the prefix sums (the join kernel adds the suffix sums);
-//   small calls (rows x group <= 16): the few-row kernel alone over prefix and
-//   suffix, and the weights kernel;
+//   small calls: the few-row kernel alone over prefix and suffix, 16 rows per
+//   CTA, and the weights kernel (for the suffixes too with more rows);
 //   more (a turn, a document): the tile kernel per sequence over prefix and
 //   suffix, the merge kernel if key ranges were split, the weights kernel.
 #include "shared_attention.cuh"
@@ -31,6 +31,8 @@ using namespace sa;
 //   few-row kernel alone / beside tiles, one token: batch 8 on 1024 + 64 keys
 //     10.9 / 13.2, batch 64 on 256 + 64 14.1 / 20; batch 2 on 8192 + 64 24.1 /
 //     19.7, batch 16 on 2048 + 64 21.1 / 14.0
+//   few-row kernel alone / tiles per sequence: one sequence of 88 tokens, 8
+//     query heads, on 291 + 91 keys 9.4 / 13.8; 2 of 33 on 1000 + 64 23.2 / 17.1
 //   few rows beside tiles / tiles per sequence: batch 32 of one token on 8192 +
 //     256 keys 24 / 183, batch 8 of 8 tokens on 8192 + 256 27 / 56; batch 16 of
 //     8 tokens on 1024 + 128 21.4 / 18.6
@@ -70,15 +72,17 @@ double plan_tiles(const SharedAttnArgs& a, int key_tiles, int units, int sms, Pl
 }
 
 // The few-row kernel alone: sets suffix_splits.  A step is 64 keys of a CTA, of
-// which four fit an SM.
+// which four (three of 16 rows) fit an SM.
 double plan_solo(const SharedAttnArgs& a, int units, int sms, Plan* best) {
-  const double step = (a.rows * a.group > 8 ? 1.5 : 1) * a.width / 128;
+  const bool many = a.rows * a.group > 8;
+  const int fit = many ? 3 : 4;
+  const long long blocks = (long long)units * ceil_div(a.rows * a.group, many ? kMostRows : 8);
   double best_cost = 0;
   for (int s = 1; s <= kMaxSuffixSplits; s *= 2) {
-    const int ctas = units * s, waves = ceil_div(ctas, 4 * sms), beside = std::min(4, ceil_div(ctas, sms));
-    const double cost = waves * (3.4 + 0.4 * beside +
-                                 std::max(1.05, 0.45 * beside) * step * ceil_div(a.scap + a.pcap, 64 * s)) +
-                        (s > 1 ? 1 : 0);
+    const int waves = ceil_div(blocks * s, fit * sms), beside = std::min(fit, ceil_div(blocks * s, sms));
+    const double start = many ? 4.8 + 0.8 * beside : 3.4 + 0.4 * beside;
+    const double step = (many ? 0.85 + 0.4 * beside : std::max(1.05, 0.45 * beside)) * a.width / 128;
+    const double cost = waves * (start + step * ceil_div(a.scap + a.pcap, 64 * s)) + (s > 1 ? 1 : 0);
     if (best_cost && cost >= best_cost) continue;
     best_cost = cost;
     best->suffix_splits = s;
@@ -120,7 +124,7 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
   p.per_tile = kRows / a.group;
   p.tiles = ceil_div(a.rows, p.per_tile);
   p.suffix_splits = 1;
-  const double by_sequence = plan_tiles(a, prefix_tiles + suffix_tiles, units, sms, &p);
+  double cost = plan_tiles(a, prefix_tiles + suffix_tiles, units, sms, &p);
   if (a.rows * a.group <= kFewRows) {
     Plan q = p;
     q.pooled = true;
@@ -128,18 +132,19 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
     q.tasks = q.tiles * a.kv_heads;
     q.per_cta = 1;
     q.full = 0;
-    double cost = plan_beside(a, prefix_tiles, units, sms, &q);
-    // (Rows for two CTAs could not add a key's weight together.)
-    if (a.rows * a.group <= kMostRows) {
-      Plan solo = q;
-      solo.splits = 0;
-      const double alone = plan_solo(a, units, sms, &solo);
-      if (alone < cost) {
-        q = solo;
-        cost = alone;
-      }
+    const double beside = plan_beside(a, prefix_tiles, units, sms, &q);
+    if (beside < cost) {
+      p = q;
+      cost = beside;
     }
-    if (cost < by_sequence) p = q;
+  }
+  Plan solo = p;
+  const double alone = plan_solo(a, units, sms, &solo);
+  if (alone < cost) {
+    p = solo;
+    p.pooled = a.rows * a.group <= kMostRows;  // rows of several CTAs cannot add a key's weight together
+    p.splits = 0;
+    p.full = p.tasks;
   }
   // The rows of a pair of key tiles are shared by a cluster while that still
   // leaves SMs idle (4 sequences of 64 tokens, microseconds with 1, 2 and 4
@@ -190,7 +195,7 @@ cudaError_t launch_shared_attention(const SharedAttnArgs& a, void* workspace, in
   Workspace ws;
   lay_out(a, p, weights, static_cast<char*>(workspace), &ws);
   cudaError_t e = p.splits ? launch_tiles(a, p, ws, stream) : cudaSuccess;
-  if (e == cudaSuccess && p.pooled) e = launch_rows(a, p, ws, stream);
+  if (e == cudaSuccess && (p.pooled || !p.splits)) e = launch_rows(a, p, ws, stream);
   if (e == cudaSuccess && p.pooled && p.splits) e = launch_join(a, p, ws, sms, stream);
   if (e == cudaSuccess && !p.pooled && p.full < p.tasks) e = launch_merge(a, p, ws, stream);
   if (e == cudaSuccess && (a.pw || (a.sw && !p.pooled))) e = launch_weights(a, p, ws, sms, stream);

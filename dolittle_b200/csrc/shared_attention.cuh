@@ -46,7 +46,8 @@ __host__ __device__ __forceinline__ int score_pitch(const SharedAttnArgs& a) { r
 
 // How a call is cut into work, from sizes alone.
 struct Plan {
-  bool pooled;    // row tiles hold tokens of several sequences and cover the prefix; the few-row kernel adds the suffixes
+  bool pooled;    // row tiles hold tokens of several sequences and cover the prefix; the few-row kernel adds the
+                  // suffixes and their weights
   int per_tile;   // tokens of a row tile: 128 / group
   int tiles;      // row tiles of a unit: a KV head (pooled) or a sequence's KV head
   int per_cta;    // 2: two row tiles share a CTA's key tiles; 1: one row tile, key tiles in two interleaved streams

@@ -230,7 +230,7 @@ __device__ __forceinline__ void add_suffix_weights(const SharedAttnArgs& a, cons
 }
 
 template <int D, int NB, bool SOLO>
-__global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
+__global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 3 : 4)
     shared_rows_kernel(const SharedAttnArgs a, const Plan pl, const Workspace ws, const float scale_log2) {
   constexpr int R = 8 * NB;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
 #pragma unroll
       for (int f = 0; f < D / 16; ++f) o[nb][f][0] = o[nb][f][1] = o[nb][f][2] = o[nb][f][3] = 0.f;
     }
-    float* scores = a.sw ? ws.scores + ((size_t(b) * a.kv_heads + h) * unit_rows + row0) * score_pitch(a) : nullptr;
+    float* scores = a.sw && pl.pooled ? ws.scores + ((size_t(b) * a.kv_heads + h) * unit_rows + row0) * score_pitch(a) : nullptr;
 
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
       row_r[row] = j.inv;
       if (split == 0) {
         if (a.lse) a.lse[row_index(a, b, h, row0 + row)] = j.lse;
-        if (a.pw) ws.norm[row_index(a, b, h, row0 + row)] = RowNorm{j.m, j.inv};
+        if (a.pw || (a.sw && !pl.pooled)) ws.norm[row_index(a, b, h, row0 + row)] = RowNorm{j.m, j.inv};
       }
     }
   }
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, SOLO && NB == 2 ? 2 : 4)
       if (r < ctas) add_part(v, y[r], part_f[row][r]);
     store_piece<D>(a, b, h, row0 + row, (i % (D / 4)) ^ (row & 7), v);
   }
-  if (a.sw)  // of this CTA's suffix keys
+  if (a.sw && pl.pooled)  // of this CTA's suffix keys
     add_suffix_weights(a, ws, scale_log2, b, h, n, max(0, g0 - ps) * kStep, min(n, max(0, g1 - ps) * kStep), row_m, row_r, t,
                        kThreads, [] {});
   if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory

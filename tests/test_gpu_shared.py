@@ -169,6 +169,10 @@ PLANS = [
     (4, 48, 1300, 60, 32, 8, 128, None, [60, 48, 49, 50]),
     (9, 64, 500, 64, 32, 8, 64, None, None),
     (1, 200, 2000, 200, 16, 4, 128, None, None),
+    (1, 88, 291, 91, 8, 4, 128, None, None),
+    (2, 8, 512, 64, 32, 8, 128, [512, 300], [64, 9]),
+    (3, 40, 300, 40, 28, 4, 64, [300, 0, 299], [40, 20, 3]),
+    (2, 64, None, 64, 4, 1, 128, None, None),
 ]
 
 
