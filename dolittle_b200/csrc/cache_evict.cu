@@ -4,9 +4,9 @@
 // evict_select_kernel: one cluster of 1-8 CTAs per (cache, KV head) gives each
 // slot a 32-bit key (protected highest, then the weight's order-preserving
 // bits, NaN lowest) and finds the last slot that stays: histograms of 11, 11
-// and 10 bits narrow the keys down until at most 256 slots share the bits found
+// and 10 bits narrow the keys down until at most 512 slots share the bits found
 // so far, those are ranked against one another by (key, slot); only more than
-// 256 equal keys need the ties counted in slot order.  Then a slot stays if its
+// 512 equal keys need the ties counted in slot order.  Then a slot stays if its
 // (key, slot) is at least the cut's, and prefix sums in slot order pair vacated
 // slots ("holes", below the kept count) with kept slots beyond it ("movers"):
 // hole i receives mover i.  Weights and positions move with the pairing; rows
@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kRanked = 256;       // slots of a unit ranked one against all
+constexpr int kRanked = 512;       // slots of a unit ranked one against all
 constexpr int kMostTiles = 1024;   // runs of kThreads slots per CTA
 constexpr int kMaxCtas = 8;
 
@@ -70,22 +70,28 @@ __device__ __forceinline__ T block_scan(T v, T* warp_sums, T* total) {
   return r;
 }
 
+// Words of shared memory at p in CTA `rank` of the cluster; MULTI = false: this CTA is alone.
+template <bool MULTI>
 __device__ __forceinline__ uint4 remote_u32x4(const unsigned* p, unsigned rank) {
+  if constexpr (!MULTI) return *reinterpret_cast<const uint4*>(p);
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "r"(tc::mapa_shared(smem_addr(p), rank)));
   return v;
 }
+template <bool MULTI>
 __device__ __forceinline__ unsigned remote_u32(const unsigned* p, unsigned rank) {
+  if constexpr (!MULTI) return *p;
   unsigned v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(tc::mapa_shared(smem_addr(p), rank)));
   return v;
 }
 // The word at p in every CTA of the cluster (0 past the last), loads in flight together.
+template <bool MULTI>
 __device__ __forceinline__ void remote_all(const unsigned* p, unsigned ctas, unsigned (&v)[kMaxCtas]) {
 #pragma unroll
-  for (int r = 0; r < kMaxCtas; ++r) v[r] = r < ctas ? remote_u32(p, r) : 0u;
+  for (int r = 0; r < kMaxCtas; ++r) v[r] = r < ctas ? remote_u32<MULTI>(p, r) : 0u;
 }
 
 // Larger = kept first.  -0 counts as +0, NaN below -infinity.
@@ -102,10 +108,11 @@ __device__ __forceinline__ void move_sums(const EvictArgs& a, int unit, int from
 }
 
 // TILES: runs of kThreads slots per CTA, a slot per thread, their keys in
-// registers; 0: any number, keys made again from global memory each time.
+// registers; 0: any number, keys made again from global memory each time.  MULTI:
+// a cluster of CTAs per unit.
 // Dynamic shared memory: counts [tiles * kWarps] (64 bits), then, with TILES,
 // the movers of the CTA [tiles * kThreads] and, to move, the slots that its rows come from.
-template <int TILES>
+template <int TILES, bool MULTI>
 __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kernel(const EvictArgs a, int* ws, int tiles_by_capacity,
                                                                bool move) {
   extern __shared__ __align__(16) unsigned long long counts[];
@@ -114,8 +121,9 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
   __shared__ __align__(16) unsigned hist[kBins];
   __shared__ unsigned long long near_order[kRanked], scan_l[33], cut_s;
   __shared__ unsigned scan_u[33], found[3], newest_s, listed, hole_total, mover_total;
-  static_assert(sizeof(hist) >= sizeof(near_order), "the histogram's memory takes the unit's list afterwards");
-  const unsigned ctas = gridDim.x / (a.caches * a.kv_heads), rank = tc::cluster_ctarank();
+  static_assert(sizeof(hist) >= sizeof(near_order) && kRanked <= kThreads,
+                "the histogram's memory takes the unit's list afterwards, a thread ranks a slot");
+  const unsigned ctas = MULTI ? gridDim.x / (a.caches * a.kv_heads) : 1, rank = MULTI ? tc::cluster_ctarank() : 0;
   const int unit = blockIdx.x / ctas, cache = unit / a.kv_heads, t = threadIdx.x, warp = t >> 5, lane = t & 31;
   for (int i = t; i < kBins; i += kThreads) hist[i] = 0;
   if (t == 0) {
@@ -134,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
   const int* positions = a.positions + size_t(unit) * a.capacity;
   const bool all = n <= a.budget;  // nothing is evicted
   auto sync = [&] {
-    if (ctas > 1) tc::cluster_sync();
+    if constexpr (MULTI) tc::cluster_sync();
     else __syncthreads();
   };
   // f(e, slot) for this thread's slot of tile e, in slot order; with TILES also
@@ -159,8 +167,8 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
   auto order = [](unsigned k, int s) { return (unsigned long long)k << 32 | (0xffffffffu - unsigned(s)); };
   auto cut_of_all = [&] {  // one CTA of the cluster found it
     unsigned v[kMaxCtas], u[kMaxCtas];
-    remote_all(reinterpret_cast<const unsigned*>(&cut_s), ctas, u);
-    remote_all(reinterpret_cast<const unsigned*>(&cut_s) + 1, ctas, v);
+    remote_all<MULTI>(reinterpret_cast<const unsigned*>(&cut_s), ctas, u);
+    remote_all<MULTI>(reinterpret_cast<const unsigned*>(&cut_s) + 1, ctas, v);
     unsigned long long c = 0;
 #pragma unroll
     for (int r = 0; r < kMaxCtas; ++r) c = max(c, (unsigned long long)v[r] << 32 | u[r]);
@@ -185,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
     if (lane == 0) atomicMax(&newest_s, newest);
     sync();
     unsigned v[kMaxCtas];
-    remote_all(&newest_s, ctas, v);
+    remote_all<MULTI>(&newest_s, ctas, v);
     for (int r = 0; r < kMaxCtas; ++r) newest = max(newest, v[r]);
     recent_from = (long long)int(newest ^ 0x80000000u) - a.recent;
     if constexpr (TILES > 0)
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
       if (top >= 0) {
         uint4 y[kMaxCtas];
 #pragma unroll
-        for (int r = 0; r < kMaxCtas; ++r) y[r] = r < ctas ? remote_u32x4(&hist[top], r) : make_uint4(0, 0, 0, 0);
+        for (int r = 0; r < kMaxCtas; ++r) y[r] = r < ctas ? remote_u32x4<MULTI>(&hist[top], r) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < kMaxCtas; ++r) {
           c[0] += y[r].w;
@@ -244,15 +252,18 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
       __syncthreads();
     }
     if (near <= kRanked) {
+      unsigned mine = 0, at = 0;
+      each([&](int e, int s) { mine += s < s1 && (key_at(e, s) & mask) == prefix; });
+      if (mine) at = atomicAdd(&listed, mine);  // the slots' ranks do not depend on it
       each([&](int e, int s) {
         if (s >= s1) return;
         const unsigned k = key_at(e, s);
-        if ((k & mask) == prefix) near_order[atomicAdd(&listed, 1u)] = order(k, s);  // their ranks do not depend on it
+        if ((k & mask) == prefix) near_order[at++] = order(k, s);
       });
       sync();
-      // Every CTA ranks its own against the unit's.
+      // Every CTA lists the unit's and ranks them, a thread each.
       unsigned long long* list = reinterpret_cast<unsigned long long*>(hist);
-      remote_all(&listed, ctas, v);
+      remote_all<MULTI>(&listed, ctas, v);
       for (unsigned i = t; i < near; i += kThreads) {
         unsigned j = i, r = 0;
 #pragma unroll
@@ -262,18 +273,17 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
             r = u + 1;
           }
         const unsigned* word = reinterpret_cast<const unsigned*>(&near_order[j]);
-        list[i] = (unsigned long long)remote_u32(word + 1, r) << 32 | remote_u32(word, r);
+        list[i] = (unsigned long long)remote_u32<MULTI>(word + 1, r) << 32 | remote_u32<MULTI>(word, r);
       }
       __syncthreads();
-      for (unsigned i = warp; i < listed; i += kWarps) {
-        const unsigned long long mine = near_order[i];
+      if (t < near) {
         unsigned better = 0;
-        for (unsigned j = lane; j < near; j += 32) better += list[j] > mine;
-        better = __reduce_add_sync(0xffffffffu, better);
-        if (lane == 0 && better == need - 1) cut_s = mine;
+#pragma unroll 8
+        for (unsigned j = 0; j < near; ++j) better += list[j] > list[t];
+        if (better == need - 1) cut_s = list[t];
       }
-      sync();
-      cut = cut_of_all();
+      __syncthreads();
+      cut = cut_s;
     } else {  // more than kRanked equal keys: the need-th of them in slot order
       each([&](int e, int s) {
         const unsigned m = __ballot_sync(0xffffffffu, s < s1 && key_at(e, s) == prefix);
@@ -290,9 +300,9 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
       }
       if (t == 0) listed = unsigned(run);
       sync();
-      remote_all(&listed, ctas, v);
+      remote_all<MULTI>(&listed, ctas, v);
       unsigned before = 0;
-      for (unsigned r = 0; r < rank; ++r) before += remote_u32(&listed, r);
+      for (unsigned r = 0; r < rank; ++r) before += remote_u32<MULTI>(&listed, r);
       each([&](int e, int s) {
         const bool tie = s < s1 && key_at(e, s) == prefix;
         const unsigned m = __ballot_sync(0xffffffffu, tie);
@@ -329,8 +339,8 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
   unsigned hole0 = 0, mover0 = 0, holes = 0, movers[kMaxCtas];
   {
     unsigned h[kMaxCtas];
-    remote_all(&hole_total, ctas, h);
-    remote_all(&mover_total, ctas, movers);
+    remote_all<MULTI>(&hole_total, ctas, h);
+    remote_all<MULTI>(&mover_total, ctas, movers);
 #pragma unroll
     for (unsigned r = 0; r < kMaxCtas; ++r) {
       hole0 += r < rank ? h[r] : 0;
@@ -358,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
           i -= movers[u];
           r = u + 1;
         }
-      return int(remote_u32(reinterpret_cast<const unsigned*>(own_movers) + i, r));
+      return int(remote_u32<MULTI>(reinterpret_cast<const unsigned*>(own_movers) + i, r));
     } else {
       return *reinterpret_cast<volatile int*>(src + a.budget + i);
     }
@@ -378,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
       src[s] = from;  // its destination is s
     }
   });
-  if (ctas > 1) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
+  if constexpr (MULTI) tc::cluster_sync();  // no CTA leaves while another reads its shared memory
   if (!move) {
     if (rank == 0 && t == 0)
       list_of(ws, a.caches * a.kv_heads, a.budget)[unit] = a.in_place ? int(holes) : keep;
@@ -499,20 +509,22 @@ cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cud
   cfg.numAttrs = ctas > 1 ? 2 : 1;
   int* ws = static_cast<int*>(workspace);
   cudaError_t e;
-  if (tiles <= 1) {
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<1>, a, ws, tiles, move);
+  if (tiles <= 1) {  // one CTA: a second one only comes with more than eight tiles
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<1, false>, a, ws, tiles, move);
+  } else if (ctas == 1) {
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8, false>, a, ws, tiles, move);
   } else if (tiles <= 8) {
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a, ws, tiles, move);
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8, true>, a, ws, tiles, move);
   } else if (tiles <= 32) {  // up to 68 KB: an opt-in of the current device
-    e = cudaFuncSetAttribute(evict_select_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(evict_select_kernel<32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              32 * (kWarps * 8 + kThreads * 4));
     if (e != cudaSuccess) return e;
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<32>, a, ws, tiles, move);
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<32, true>, a, ws, tiles, move);
   } else {
-    e = cudaFuncSetAttribute(evict_select_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(evict_select_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kMostTiles * kWarps * 8);
     if (e != cudaSuccess) return e;
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<0>, a, ws, tiles, move);
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<0, true>, a, ws, tiles, move);
   }
   if (e != cudaSuccess || move) return e;
   const int pieces = 2 * (a.width / 8);
