@@ -17,11 +17,10 @@
 // scheduling.
 //
 // Measured, out of place, 8 heads of width 128: 32 caches of 2304 slots to 2048
-// in 87 us (435 MB, 5.0 TB/s: bound by the copy); one cache of 32768 to 8192 in
-// 36 us, two thirds of it the selection, whose dozen cluster-wide steps of 1 to
-// 2 us each bound it; two caches of 320 to 256 in 8.2 us, two launches.  Fewer
-// and longer CTAs: one cache of 32768 takes 36 us with 8 CTAs per head, 60 with
-// 4, 65 with 2; 32 caches of 2304 take 103 us with one, 117 with two.
+// in 95 us (5.7 TB/s: bound by the copy); one cache of 32768 to 8192 in 35 us,
+// two thirds of it the selection, whose dozen cluster-wide steps of 1 to 2 us
+// each bound it; two caches of 320 to 256 in 6.3 us, two launches.  Adding the
+// histograms up in slices, one per CTA, instead of all by each CTA: no gain.
 #include <algorithm>
 #include <climits>
 
@@ -302,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
       sync();
       remote_all<MULTI>(&listed, ctas, v);
       unsigned before = 0;
-      for (unsigned r = 0; r < rank; ++r) before += remote_u32<MULTI>(&listed, r);
+      for (int r = 0; r < int(rank); ++r) before += remote_u32<MULTI>(&listed, r);
       each([&](int e, int s) {
         const bool tie = s < s1 && key_at(e, s) == prefix;
         const unsigned m = __ballot_sync(0xffffffffu, tie);
@@ -343,8 +342,8 @@ __global__ void __launch_bounds__(kThreads, TILES > 8 ? 1 : 2) evict_select_kern
     remote_all<MULTI>(&mover_total, ctas, movers);
 #pragma unroll
     for (unsigned r = 0; r < kMaxCtas; ++r) {
-      hole0 += r < rank ? h[r] : 0;
-      mover0 += r < rank ? movers[r] : 0;
+      hole0 += int(r) < int(rank) ? h[r] : 0;
+      mover0 += int(r) < int(rank) ? movers[r] : 0;
       holes += h[r];
     }
   }
@@ -477,16 +476,19 @@ int cache_evict_most_slots() { return kMaxCtas * kMostTiles * kThreads; }
 
 cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cudaStream_t stream) {
   // A CTA takes up to eight slots per thread, in registers; more CTAs per head
-  // beyond that (measured above).
+  // beyond that, and four rather than two while SMs are idle (21 heads of 7544
+  // slots 25.7 us with four, 27.4 with two, 43 with eight; 8 of 8192 21.0, 22.8
+  // and 21.6; 8 of 32768 50.6 with four, 35.1 with eight).
   const int units = a.caches * a.kv_heads;
   int ctas = 1;
   while (ctas < kMaxCtas && a.capacity > 8 * kThreads * ctas) ctas *= 2;
+  if (ctas == 2 && units <= sms / 4) ctas = 4;
   const int tiles = (a.capacity + ctas * kThreads - 1) / (ctas * kThreads);
   // Moving in the selecting CTAs when they fill the SMs, in one wave, with few
   // rows each: some copy while others still select.  Below that the second
   // kernel's even spread is faster (microseconds, moving there / here: 2 caches
-  // of 320 slots to 256 8.3 / 11.2, 8 of 1024 to 512 16.4 / 22.8, 32 of 320 to
-  // 256 22.6 / 20.7, 36 of 1024 to 512 40.7 / 37.9).  Not when the lengths are
+  // of 320 slots to 256 6.3 / 9.3, 20 of 1024 to 512 25.7 / 29.8, 32 of 320 to
+  // 256 18.9 / 17.3, 36 of 1024 to 512 36.3 / 34.1).  Not when the lengths are
   // updated in place, since a CTA of another head may still have to read them.
   const int own_rows = std::min(a.budget, tiles * kThreads);
   const size_t bytes = size_t(own_rows) * a.width * 4;
@@ -509,10 +511,9 @@ cudaError_t launch_cache_evict(const EvictArgs& a, void* workspace, int sms, cud
   cfg.numAttrs = ctas > 1 ? 2 : 1;
   int* ws = static_cast<int*>(workspace);
   cudaError_t e;
-  if (tiles <= 1) {  // one CTA: a second one only comes with more than eight tiles
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<1, false>, a, ws, tiles, move);
-  } else if (ctas == 1) {
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8, false>, a, ws, tiles, move);
+  if (ctas == 1) {  // at most eight tiles
+    e = tiles <= 1 ? cudaLaunchKernelEx(&cfg, evict_select_kernel<1, false>, a, ws, tiles, move)
+                   : cudaLaunchKernelEx(&cfg, evict_select_kernel<8, false>, a, ws, tiles, move);
   } else if (tiles <= 8) {
     e = cudaLaunchKernelEx(&cfg, evict_select_kernel<8, true>, a, ws, tiles, move);
   } else if (tiles <= 32) {  // up to 68 KB: an opt-in of the current device

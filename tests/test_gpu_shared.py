@@ -444,7 +444,8 @@ def test_eviction_of_equal_weights(n, capacity, budget):
 
 
 @pytest.mark.parametrize("in_place", [True, False])
-@pytest.mark.parametrize("n,capacity,hkv,d", [(20, 300, 8, 64), (36, 600, 8, 64), (40, 200, 8, 128), (5, 5000, 3, 64)])
+@pytest.mark.parametrize("n,capacity,hkv,d", [(20, 300, 8, 64), (36, 600, 8, 64), (40, 200, 8, 128), (5, 5000, 3, 64),
+                                                  (10, 16000, 4, 8), (3, 7000, 1, 8), (80, 4200, 1, 8)])
 def test_eviction_with_few_and_many_heads(n, capacity, hkv, d, in_place):
     lengths = [capacity - 13 * b % capacity for b in range(n)]
     check_eviction(make_caches(n, capacity, hkv, d, seed=n, lengths=lengths), capacity * 2 // 3, 4, 20, in_place)
