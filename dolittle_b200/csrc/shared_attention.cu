@@ -117,6 +117,33 @@ double plan_beside(const SharedAttnArgs& a, int key_tiles, int units, int sms, P
   return best_cost;
 }
 
+// The parts of the row tiles in the weights kernel, for both caches: the least
+// work of the busiest CTA, which takes every sms-th unit, in tiles of 128 rows
+// against a pair of key tiles (2.3 us); a unit costs half a tile besides, adding
+// the parts up one and a half.  41 sequences of 150 tokens, 2 heads per KV head,
+// on 71 keys take 200 us in one part (two CTAs take all rows past the prefix),
+// 54 in 8, 41 in 33; 8 of 48 tokens on 4096 keys 83 in one, 85 in 4, 95 in 8.
+void plan_weights(const SharedAttnArgs& a, int sms, Plan* p) {
+  const long long prefix = (long long)ceil_div(a.pcap, kPair) * a.kv_heads;
+  const long long suffix = p->pooled ? 0 : (long long)ceil_div(a.scap, kPair) * a.kv_heads * a.batch;
+  const int prefix_rows = ceil_div((long long)a.batch * a.rows, p->per_tile), suffix_rows = ceil_div(a.rows, p->per_tile);
+  double best_cost = 0;
+  for (int parts = 1; parts <= std::min(prefix_rows, kMaxWeightParts); ++parts) {
+    const int longest = ceil_div(prefix_rows, parts);
+    const int of_suffix = suffix ? std::min(kMaxWeightParts, ceil_div(suffix_rows, longest)) : 1;
+    const long long first = prefix * parts, all = first + suffix * of_suffix;
+    auto load = [&](long long cta) {
+      const int mine = ceil_div(std::max(0ll, first - cta), sms), rest = ceil_div(std::max(0ll, all - cta), sms) - mine;
+      return mine * (longest + 0.5) + rest * (ceil_div(suffix_rows, of_suffix) + 0.5);
+    };
+    const double cost = std::max(load(0), load(first % sms)) + (parts > 1 || of_suffix > 1 ? 1.5 : 0);
+    if (best_cost && cost >= best_cost) continue;
+    best_cost = cost;
+    p->prefix_parts = parts;
+    p->suffix_parts = of_suffix;
+  }
+}
+
 Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
   const int tokens = a.batch * a.rows, units = a.batch * a.kv_heads;
   const int prefix_tiles = ceil_div(a.pcap, kKeys), suffix_tiles = ceil_div(a.scap, kKeys);
@@ -146,17 +173,8 @@ Plan plan_of(const SharedAttnArgs& a, bool weights, int sms) {
     p.splits = 0;
     p.full = p.tasks;
   }
-  // The rows of a pair of key tiles are shared by a cluster while that still
-  // leaves SMs idle (4 sequences of 64 tokens, microseconds with 1, 2 and 4
-  // ranks: on 1024 keys 44, 39 and 43, on 8192 keys 98, 113 and 150).
-  p.weight_ranks = 1;
-  if (weights) {
-    const long long key_units =  // pairs of key tiles
-        ((prefix_tiles + 1) / 2 + (long long)(p.pooled ? 0 : (suffix_tiles + 1) / 2) * a.batch) * a.kv_heads;
-    const int row_tiles = ceil_div(tokens, p.per_tile);
-    while (p.weight_ranks < 8 && key_units * p.weight_ranks * 2 <= sms && row_tiles >= 2 * p.weight_ranks)
-      p.weight_ranks *= 2;
-  }
+  p.prefix_parts = p.suffix_parts = 1;
+  if (weights) plan_weights(a, sms, &p);
   return p;
 }
 
@@ -178,6 +196,10 @@ size_t lay_out(const SharedAttnArgs& a, const Plan& p, bool weights, char* base,
   ws->suffix_o = reinterpret_cast<float*>(take(suffix_rows * a.width * 4));
   ws->suffix_ml = reinterpret_cast<float2*>(take(suffix_rows * 8));
   ws->norm = reinterpret_cast<RowNorm*>(take(weights ? rows * 8 : 0));
+  const size_t prefix_keys = p.prefix_parts > 1 ? size_t(ceil_div(a.pcap, kPair)) * kPair : 0;
+  const size_t suffix_keys = p.suffix_parts > 1 && !p.pooled ? size_t(ceil_div(a.scap, kPair)) * kPair : 0;
+  ws->prefix_sums = reinterpret_cast<float*>(take(p.prefix_parts * a.kv_heads * prefix_keys * 4));
+  ws->suffix_sums = reinterpret_cast<float*>(take(size_t(p.suffix_parts) * a.batch * a.kv_heads * suffix_keys * 4));
   ws->scores = reinterpret_cast<float*>(take(weights && p.pooled ? rows * score_pitch(a) * 4 : 0));
   return std::max<size_t>(at, 256);
 }

@@ -17,6 +17,8 @@ constexpr int kRows = 128;   // query rows of a tile = TMEM lanes
 constexpr int kKeys = 128;   // keys of a tile
 constexpr int kMaxSplits = 32;  // key ranges of a row tile
 constexpr int kMaxSuffixSplits = 8;
+constexpr int kPair = 2 * kKeys;  // keys of a unit of the weights kernel
+constexpr int kMaxWeightParts = 64;
 constexpr int kFewRows = 32;    // rows of a unit (new tokens x group) that the few-row kernels take
 constexpr int kMostRows = 16;   // and one CTA of them
 constexpr float kLog2e = 1.4426950408889634f;
@@ -39,6 +41,7 @@ struct Workspace {
   float2* suffix_ml;  // [suffix splits][B][Hkv][rows x group]
   RowNorm* norm;    // [tokens * Hq]
   float* scores;    // [B][Hq * rows][score_pitch]
+  float *prefix_sums, *suffix_sums;  // of the weights kernel's parts: [parts][Hkv][keys], [parts][B][Hkv][keys]
 };
 
 // Suffix scores of a row, in 16-byte pieces.
@@ -56,7 +59,7 @@ struct Plan {
   int full;       // tasks done whole, by the first CTAs; the rest are cut into key ranges
   int splits;     // key ranges of the rest (0: no tile kernel; the few-row kernel reads the prefix too)
   int suffix_splits;  // CTAs (a cluster if there is no tile kernel) per sequence and KV head in the few-row kernel
-  int weight_ranks;   // CTAs (one cluster) per pair of key tiles in the weights kernel
+  int prefix_parts, suffix_parts;  // of the row tiles that a pair of key tiles goes through in the weights kernel
 };
 
 // Warps that share a row in the join kernel (four, or one when that would take

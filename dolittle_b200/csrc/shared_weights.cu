@@ -11,9 +11,10 @@
 // The exponentials bound it (16 per cycle and SM): sixteen warps cover one
 // another's latencies, two key tiles share each query tile that comes through
 // L2, scores and queries are double-buffered, and the next key tiles load under
-// the sums of the ones before.  When there are few key tiles, a cluster shares
-// the rows of a pair and rank 0 adds the ranks' sums in order.  The keys were
-// just read by the attention, so they come from L2 while the caches fit it.
+// the sums of the ones before.  When there are few key tiles and many rows, the
+// row tiles of a pair are cut into parts and a second kernel adds the parts'
+// sums in order.  The keys were just read by the attention, so they come from L2
+// while the caches fit it.
 //
 // Measured: 8192 keys x 8 heads against 256 tokens x 4 heads (67 M weights) 38
 // us, 47 % of the exponential unit while a CTA has work; 256 pairs over 148 SMs
@@ -30,7 +31,6 @@ namespace {
 
 using namespace tc;
 
-constexpr int kPair = 2 * kKeys;      // keys of a unit
 constexpr int kWork = 2 * kPair;      // threads that sum, two per key
 constexpr int kThreads = kWork + 32;  // and a warp that loads and issues
 constexpr int kIssueWarp = kWork / 32;
@@ -41,17 +41,47 @@ struct alignas(64) WeightArgs {
   CUtensorMap q, pk, sk;
   SharedAttnArgs a;
   const RowNorm* norm;
-  int per_tile, prefix_pairs, suffix_pairs, ranks;  // pairs of key tiles by capacity; CTAs per pair
-  int units;                                        // pairs x KV heads (x sequences)
+  int per_tile, prefix_pairs, suffix_pairs;  // pairs of key tiles by capacity
+  int prefix_parts, suffix_parts;            // of a pair's row tiles
+  float *prefix_sums, *suffix_sums;          // of the parts, if there is more than one: [part][(b,) h][256 keys x pairs]
+  int prefix_units, units;                   // parts x pairs x KV heads (x sequences)
   float scale_log2;
 };
+
+// The longest and shortest prefix of any sequence; whole warps.
+__device__ __forceinline__ void prefix_extent(const SharedAttnArgs& a, int& longest, int& shortest) {
+  longest = 0;
+  shortest = a.pcap;
+  for (int s = threadIdx.x & 31; s < a.batch; s += 32) {
+    const int l = prefix_len(a, s);
+    longest = max(longest, l);
+    shortest = min(shortest, l);
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  shortest = __reduce_min_sync(0xffffffffu, shortest);
+}
+
+// Row tiles [first, first + span) that see keys from j0 on, of `tokens` tokens:
+// all of them for a prefix, of a sequence's rows for its suffix of n keys.
+__device__ __forceinline__ int row_span(const WeightArgs& w, bool suffix, int tokens, int j0, int n, int& first) {
+  first = suffix ? max(0, j0 - n + w.a.rows) / w.per_tile : 0;
+  return j0 >= n ? 0 : max(0, (tokens + w.per_tile - 1) / w.per_tile - first);
+}
+__device__ __forceinline__ int part_start(int span, int part, int parts) {
+  return span / parts * part + min(part, span % parts);
+}
+// The sums of a part of pair (b, h, j0).
+__device__ __forceinline__ float* part_sums(const WeightArgs& w, bool suffix, int part, int b, int h, int j0) {
+  const size_t head = suffix ? (size_t(part) * w.a.batch + b) * w.a.kv_heads + h : size_t(part) * w.a.kv_heads + h;
+  return (suffix ? w.suffix_sums : w.prefix_sums) + head * kPair * (suffix ? w.suffix_pairs : w.prefix_pairs) + j0;
+}
 
 // A pair of key tiles of one KV head and the row tiles [i0, i0 + n) that this
 // CTA takes it through: of all tokens for a prefix key, of the sequence's rows
 // that can see the first tile for a suffix key.
 struct Unit {
   bool suffix;
-  int h, b, j0, tokens, token0, i0, n, span;
+  int h, b, j0, tokens, token0, i0, n, part;
   int longest, shortest;  // prefix lengths of all sequences; a suffix's own
 };
 
@@ -69,7 +99,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
   const SharedAttnArgs& a = w.a;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;  // two pairs of key tiles, two query tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned rank = cluster_ctarank();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -99,39 +128,35 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
   fence_after_sync();
   const uint32_t tmem = tmem_slot;
 
-  int longest = 0, shortest = a.pcap;
-  for (int s = lane; s < a.batch; s += 32) {
-    const int l = prefix_len(a, s);
-    longest = max(longest, l);
-    shortest = min(shortest, l);
-  }
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  shortest = __reduce_min_sync(0xffffffffu, shortest);
+  int longest, shortest;
+  prefix_extent(a, longest, shortest);
   auto unit_of = [&](int at) {
     Unit u;
-    u.suffix = at >= w.prefix_pairs * a.kv_heads;
-    if (u.suffix) at -= w.prefix_pairs * a.kv_heads;
+    u.suffix = at >= w.prefix_units;
+    if (u.suffix) at -= w.prefix_units;
+    const int parts = u.suffix ? w.suffix_parts : w.prefix_parts;
     u.h = at % a.kv_heads;
     at /= a.kv_heads;
+    u.part = at % parts;
+    at /= parts;
     u.b = u.suffix ? at / w.suffix_pairs : 0;
     u.j0 = (u.suffix ? at % w.suffix_pairs : at) * kPair;
     u.tokens = u.suffix ? a.rows : a.batch * a.rows;
     u.token0 = u.suffix ? u.b * a.rows : 0;
     u.longest = u.suffix ? suffix_len(a, u.b) : longest;
     u.shortest = shortest;
-    const int first = u.suffix ? max(0, u.j0 - u.longest + a.rows) / w.per_tile : 0;
-    u.span = u.j0 >= u.longest ? 0 : max(0, (u.tokens + w.per_tile - 1) / w.per_tile - first);
-    u.i0 = first + int((long long)u.span * rank / w.ranks);
-    u.n = first + int((long long)u.span * (rank + 1) / w.ranks) - u.i0;
+    int first;
+    const int span = row_span(w, u.suffix, u.tokens, u.j0, u.longest, first);
+    u.i0 = first + part_start(span, u.part, parts);
+    u.n = first + part_start(span, u.part + 1, parts) - u.i0;
     return u;
   };
-  // The units of this CTA (of its cluster: one) that have row tiles.
-  const int step = gridDim.x / w.ranks;
+  // The units of this CTA that have row tiles.
   auto next = [&](int& at, Unit& u) {
-    for (; at < w.units; at += step) {
+    for (; at < w.units; at += gridDim.x) {
       u = unit_of(at);
       if (u.n > 0) {
-        at += step;
+        at += gridDim.x;
         return true;
       }
     }
@@ -171,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
         return true;
       };
       Unit u, v;
-      int at = blockIdx.x / w.ranks, li = 0;  // li: next row tile to load, of u or (ahead) of v
+      int at = blockIdx.x, li = 0;  // li: next row tile to load, of u or (ahead) of v
       bool have = next(at, u), more = false, ahead = false;
       if (have) {
         load_keys(u);
@@ -260,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
       return false;
     };
     Unit u, following;
-    int at = blockIdx.x / w.ranks;
+    int at = blockIdx.x;
     unsigned g = 0;
     bool ok = true, more = next_active(at, u);
     RowNorm nm = {0.f, 0.f};
@@ -326,9 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
       }
       if (!ok) sum = NAN;
       sums[threadIdx.x] = sum;
-      if (w.ranks > 1) break;  // joined across the cluster below
       named_sync(1 + p, kPair);
-      if (half == 0 && key < (u.suffix ? a.scap : a.pcap)) {
+      if ((u.suffix ? w.suffix_parts : w.prefix_parts) > 1) {
+        if (half == 0)
+          part_sums(w, u.suffix, u.part, u.b, u.h, u.j0)[key - u.j0] = sum + sums[threadIdx.x + kKeys];
+      } else if (half == 0 && key < (u.suffix ? a.scap : a.pcap)) {
         float* out = u.suffix ? a.sw + (size_t(u.b) * a.kv_heads + u.h) * a.scap : a.pw + size_t(u.h) * a.pcap;
         out[key] += sum + sums[threadIdx.x + kKeys];
       }
@@ -336,30 +363,37 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
     }
     fence_before_sync();
   }
-  if (w.ranks > 1) {
-    cluster_sync();
-    const Unit u = unit_of(blockIdx.x / w.ranks);
-    if (threadIdx.x < kPair && rank == 0 && u.span > 0) {
-      const int p = threadIdx.x / kKeys, r = threadIdx.x % kKeys, key = u.j0 + int(threadIdx.x);
-      float total = 0.f;
-      for (int x = 0; x < 2 * w.ranks; ++x) {  // ranks in order, the halves of each
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                     : "=f"(v)
-                     : "r"(mapa_shared(smem_addr(&sums[p * kPair + (x & 1) * kKeys + r]), x >> 1))
-                     : "memory");
-        total += v;
-      }
-      if (active(u, p) && key < (u.suffix ? a.scap : a.pcap)) {
-        float* out = u.suffix ? a.sw + (size_t(u.b) * a.kv_heads + u.h) * a.scap : a.pw + size_t(u.h) * a.pcap;
-        out[key] += total;
-      }
-    }
-    cluster_sync();
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   if (warp == kIssueWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Adds the parts' sums of a pair, a thread per key, in order: a block for each
+// pair that was cut, prefix pairs first.
+__global__ void __launch_bounds__(kPair) shared_weights_add_kernel(const __grid_constant__ WeightArgs w) {
+  const SharedAttnArgs& a = w.a;
+  const int prefix = w.prefix_parts > 1 ? w.prefix_pairs * a.kv_heads : 0;
+  const bool suffix = int(blockIdx.x) >= prefix;
+  int at = blockIdx.x - (suffix ? prefix : 0), first;
+  const int h = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int b = suffix ? at / w.suffix_pairs : 0, j0 = (suffix ? at % w.suffix_pairs : at) * kPair;
+  const int key = j0 + int(threadIdx.x), parts = suffix ? w.suffix_parts : w.prefix_parts;
+  // Lengths and sums are from before the weights kernel, which began when what
+  // came before it was over; only the parts' sums have to be waited for.
+  int n, shortest;
+  if (suffix) n = suffix_len(a, b);
+  else prefix_extent(a, n, shortest);
+  const int span = row_span(w, suffix, suffix ? a.rows : a.batch * a.rows, j0, n, first);
+  const bool live = key < n && span > 0;
+  float* out = suffix ? a.sw + (size_t(b) * a.kv_heads + h) * a.scap : a.pw + size_t(h) * a.pcap;
+  const float old = live ? out[key] : 0.f;
+  wait_prior();
+  allow_next();
+  if (!live) return;
+  float total = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < min(parts, span); ++p) total += part_sums(w, suffix, p, b, h, j0)[threadIdx.x];
+  out[key] = old + total;
 }
 
 }  // namespace
@@ -371,25 +405,31 @@ cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspa
   w.per_tile = p.per_tile;
   w.prefix_pairs = a.pw ? (a.pcap + kPair - 1) / kPair : 0;
   w.suffix_pairs = a.sw && !p.pooled ? (a.scap + kPair - 1) / kPair : 0;
-  w.ranks = p.weight_ranks;
+  w.prefix_parts = p.prefix_parts;
+  w.suffix_parts = p.suffix_parts;
+  w.prefix_sums = ws.prefix_sums;
+  w.suffix_sums = ws.suffix_sums;
   w.scale_log2 = attention_scale(a.width) * kLog2e;
   if (!encode_query_map(&w.q, a, p.per_tile)) return cudaErrorInvalidValue;
   if (w.prefix_pairs && !encode_prefix_map(&w.pk, a, a.pk)) return cudaErrorInvalidValue;
   if (w.suffix_pairs && !encode_suffix_map(&w.sk, a, a.sk)) return cudaErrorInvalidValue;
-  const long long units = (w.prefix_pairs + (long long)w.suffix_pairs * a.batch) * a.kv_heads;
+  const long long prefix = (long long)w.prefix_pairs * a.kv_heads, suffix = (long long)w.suffix_pairs * a.batch * a.kv_heads;
+  const long long units = prefix * w.prefix_parts + suffix * w.suffix_parts;
   if (units == 0) return cudaSuccess;
   if (units > (1 << 30)) return cudaErrorInvalidValue;
+  w.prefix_units = int(prefix * w.prefix_parts);
   w.units = int(units);
-  // At least half of an SM's memory, so that two blocks never share an SM: each
-  // takes all of its TMEM, and blocks of two clusters could wait for one another.
+  // At least half of an SM's memory: each block takes all of the SM's TMEM.
   const int smem = std::max(6 * (a.width / 64) * kAtom + 1024, 120 << 10);
-  const cudaError_t e = a.width == 64 ? allow_smem<shared_weights_kernel<64>>(smem)
-                                      : allow_smem<shared_weights_kernel<128>>(smem);
+  cudaError_t e = a.width == 64 ? allow_smem<shared_weights_kernel<64>>(smem) : allow_smem<shared_weights_kernel<128>>(smem);
   if (e != cudaSuccess) return e;
-  const int grid = w.ranks > 1 ? w.units * w.ranks : std::min(w.units, sms);
-  DependentLaunch d(dim3(unsigned(grid)), kThreads, smem, stream, w.ranks);
-  return a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<64>, w)
-                       : cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<128>, w);
+  DependentLaunch d(dim3(unsigned(std::min(w.units, sms))), kThreads, smem, stream);
+  e = a.width == 64 ? cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<64>, w)
+                    : cudaLaunchKernelEx(&d.cfg, shared_weights_kernel<128>, w);
+  const long long cut = (w.prefix_parts > 1 ? prefix : 0) + (w.suffix_parts > 1 ? suffix : 0);
+  if (e != cudaSuccess || cut == 0) return e;
+  DependentLaunch add(dim3(unsigned(cut)), kPair, 0, stream);
+  return cudaLaunchKernelEx(&add.cfg, shared_weights_add_kernel, w);
 }
 
 }  // namespace sa

@@ -173,6 +173,9 @@ PLANS = [
     (2, 8, 512, 64, 32, 8, 128, [512, 300], [64, 9]),
     (3, 40, 300, 40, 28, 4, 64, [300, 0, 299], [40, 20, 3]),
     (2, 64, None, 64, 4, 1, 128, None, None),
+    (13, 90, 71, 91, 4, 2, 64, [71, 0, 70] + [5 * b for b in range(10)], [91, 90, 60] + [91] * 10),
+    (1, 700, 40, 700, 2, 1, 64, None, None),
+    (3, 400, None, 600, 2, 1, 128, None, [600, 400, 3]),
 ]
 
 
