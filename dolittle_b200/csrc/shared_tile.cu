@@ -56,6 +56,11 @@ struct Shape {
   static_assert(!(WIDE && BESIDE), "room for a few-row block is left by one row tile only");
   static constexpr int slot = D / 64 * kAtom;  // a K, V or Q tile
   static constexpr int queries = WIDE ? 2 : 1;
+  // Parts in which the weights of a tile are handed over: products begin sooner
+  // with four (batch 64 on 32768 keys 87.8 -> 85.4 us, turns of 48 tokens 51.4 ->
+  // 49.1), but two cost less where the tensor core is busy (tails of 512 tokens
+  // 620.5 against 629).
+  static constexpr int parts = WIDE ? 2 : 4;
   static constexpr int stages = D == 64 ? 8 : WIDE ? 5 : 4;
   static constexpr int smem = (queries + stages) * slot + 1024;
   static constexpr int bound = BESIDE ? 512 : kThreads;  // threads that the registers are shared out for
@@ -81,14 +86,14 @@ __device__ __forceinline__ void mma_scores(uint32_t tmem_s, uint32_t q_tile, uin
   }
 }
 
-// Half of the key tile's keys (kk of 8 steps of 16).
-template <int D>
-__device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_tile, int half,
+// A half or a quarter of the key tile's keys (kk of 8 steps of 16).
+template <int D, int PARTS>
+__device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_tile, int part,
                                            bool accumulate) {
   constexpr uint32_t idesc = instr_desc_bf16(kRows, D) | (1u << 16);  // B is MN-major
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int kk = 4 * half + i;
+  for (int i = 0; i < 8 / PARTS; ++i) {
+    const int kk = 8 / PARTS * part + i;
     const uint64_t v = smem_desc_sw128_mn(v_tile + uint32_t(kk * 2048), kAtom);
     const uint32_t p = tmem_p + uint32_t((kk >> 1) * 32 + (kk & 1) * 8);  // 32 keys: 16 columns hi, 16 lo
     mma_bf16_ts(tmem_o, p, v, idesc, (accumulate || i) ? 1u : 0u);
@@ -101,7 +106,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     shared_tile_kernel(const __grid_constant__ TileArgs t) {
   using S = Shape<D, WIDE, BESIDE>;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_half[2], p_full[2], o_full[2];
+  __shared__ uint64_t q_full, full[S::stages], empty[S::stages], s_full[2], p_part[2][S::parts], o_full[2];
   __shared__ uint64_t begun, dirty, clean, drained;
   __shared__ uint32_t dirty_from, dirty_to;  // bytes of a value tile's first 64 features to clear
   __shared__ uint32_t tmem_slot;
@@ -133,8 +138,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_half[x], 4);
-      mbar_init(&p_full[x], 4);
+      for (int j = 0; j < S::parts; ++j) mbar_init(&p_part[x][j], 4);
       mbar_init(&o_full[x], 1);
     }
     mbar_init(&begun, 1);
@@ -272,13 +276,13 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
       };
       auto output = [&](int s, int slot, int i) {
         const uint32_t o = tmem + 256 + s * 128, p = tmem + s * kKeys, v = slot_addr(slot);
-        ok = role_wait(&p_half[s], i & 1, failed);
-        fence_after_sync();
-        if (!ok) return;
-        mma_output<D>(o, p, v, 0, i > 0);
-        ok = role_wait(&p_full[s], i & 1, failed);
-        fence_after_sync();
-        if (ok) mma_output<D>(o, p, v, 1, true);
+#pragma unroll
+        for (int j = 0; j < S::parts; ++j) {
+          ok = role_wait(&p_part[s][j], i & 1, failed);
+          fence_after_sync();
+          if (!ok) return;
+          mma_output<D, S::parts>(o, p, v, j, i > 0 || j > 0);
+        }
       };
       if constexpr (WIDE) {
         wait_key();
@@ -465,11 +469,12 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
         }
         tmem_st16(t_s + 32 * j, hi);  // over the 32 scores just used
         tmem_st16(t_s + 32 * j + 16, lo);
-        if (j & 1) {  // 64 keys are there: their products may begin
+        constexpr int chunks = 4 / S::parts;
+        if (j % chunks == chunks - 1) {  // a part is there: its products may begin
           tmem_st_wait();
           fence_before_sync();
           __syncwarp();
-          if (lane == 0 && i >= 0) mbar_arrive(j == 1 ? &p_half[x] : &p_full[x]);
+          if (lane == 0 && i >= 0) mbar_arrive(&p_part[x][j / chunks]);
         }
       };
       if constexpr (BESIDE) {
