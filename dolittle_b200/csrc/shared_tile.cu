@@ -28,7 +28,7 @@
 // Q K^T (both operands from shared memory, 103 cycles per 128 x 128 x 16 where
 // the products alone are 64) and 1024 of P V, two of them 3700; measured 3960
 // to 4300 for a pair.  Eight sequences of 512 tokens on 8192 + 512 keys, 32
-// heads of 128: 632 us, 897 TFLOP/s of useful work and 1345 with the second
+// heads of 128: 625 us, 907 TFLOP/s of useful work and 1361 with the second
 // half of P.  Calls of one or two steps are bound by the start instead: 9.7 us
 // for 5 x 74 tokens on 28 + 101 keys.
 #include "shared_attention.cuh"
