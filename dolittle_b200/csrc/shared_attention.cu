@@ -59,7 +59,7 @@ double plan_tiles(const SharedAttnArgs& a, int key_tiles, int units, int sms, Pl
     auto steps = [&](int splits) { return per_cta == 2 ? ceil_div(key_tiles, splits) : ceil_div(key_tiles, 2 * splits); };
     for (int s = 1; s <= std::max(1, std::min({rest ? sms / rest : 1, key_tiles / 2, kMaxSplits})); ++s) {
       const int waves = ceil_div(p.tasks, sms);
-      const double cost = 7 + (per_cta == 2 ? 2.3 : 2.37) * (whole / sms * steps(1) + (rest ? steps(s) : 0)) +
+      const double cost = 7 + (per_cta == 2 ? 2.3 : 2.37) * (double(whole / sms) * steps(1) + (rest ? steps(s) : 0)) +
                           4 * (waves - 1) + (s > 1 ? 3 + 0.042 * s * rest * per_cta * a.width / 128 : 0);
       if (best_cost && cost >= best_cost) continue;
       best_cost = cost;

@@ -121,8 +121,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
       if (w.suffix_pairs) prefetch_map(&w.sk);
     }
   }
-  wait_prior();
-  allow_next();
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -284,6 +282,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
         if (active(u, p)) return true;
       return false;
     };
+    // Only the norms come from the kernel before this one.  It began when what
+    // came before it was over, so keys, queries and lengths are there already:
+    // the first products run while it ends.
+    wait_prior();
+    allow_next();
     Unit u, following;
     int at = blockIdx.x;
     unsigned g = 0;
