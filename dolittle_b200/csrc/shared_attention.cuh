@@ -82,8 +82,10 @@ cudaError_t launch_rows(const SharedAttnArgs& a, const Plan& p, const Workspace&
 cudaError_t launch_join(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream);
 cudaError_t launch_weights(const SharedAttnArgs& a, const Plan& p, const Workspace& ws, int sms, cudaStream_t stream);
 
-// Launch configuration of a programmatic dependent launch (every kernel here
-// waits for its predecessor before it touches global memory).
+// Launch configuration of a programmatic dependent launch.  The first kernel of
+// a call waits for its predecessor before it touches global memory and only then
+// lets the next one start, and so on: a later kernel may read the call's inputs
+// at once and waits before it touches what the kernels before it write.
 struct DependentLaunch {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

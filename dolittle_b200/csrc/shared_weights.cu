@@ -8,9 +8,8 @@
 //
 // with the keys as TMEM lanes: two threads own a key and add up half of its row
 // of S^T each, in order, joined at the end: no exchange in between, no atomics.
-// The exponentials bound it (16 per cycle and SM): sixteen warps cover one
-// another's latencies, two key tiles share each query tile that comes through
-// L2, scores and queries are double-buffered, and the next key tiles load under
+// The latencies around the exponentials bound it: sixteen warps cover one
+// another's, two key tiles share each query tile that comes through L2, scores and queries are double-buffered, and the next key tiles load under
 // the sums of the ones before.  When there are few key tiles and many rows, the
 // row tiles of a pair are cut into parts and a second kernel adds the parts'
 // sums in order.  The keys were just read by the attention, so they come from L2
