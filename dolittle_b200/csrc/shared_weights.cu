@@ -9,11 +9,12 @@
 // with the keys as TMEM lanes: two threads own a key and add up half of its row
 // of S^T each, in order, joined at the end: no exchange in between, no atomics.
 // The latencies around the exponentials bound it: sixteen warps cover one
-// another's, two key tiles share each query tile that comes through L2, scores and queries are double-buffered, and the next key tiles load under
-// the sums of the ones before.  When there are few key tiles and many rows, the
-// row tiles of a pair are cut into parts and a second kernel adds the parts'
-// sums in order.  The keys were just read by the attention, so they come from L2
-// while the caches fit it.
+// another's, two key tiles share each query tile that comes through L2, scores
+// and queries are double-buffered, and the next key tiles load under the sums of
+// the ones before.  When there are few key tiles and many rows, the row tiles of
+// a pair are cut into parts and a second kernel adds the parts' sums in order.
+// The keys were just read by the attention, so they come from L2 while the
+// caches fit it.
 //
 // Measured: 8192 keys x 8 heads against 256 tokens x 4 heads (67 M weights) 38
 // us, 47 % of the exponential unit while a CTA has work; 256 pairs over 148 SMs
