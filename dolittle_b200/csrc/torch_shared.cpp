@@ -132,14 +132,17 @@ PyObject* py_attention_shared(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 11) throw ArgumentError("attention_shared takes 11 arguments");
     const at::Tensor& q = tensor(arg[0], "query");
-    if (q.scalar_type() != at::kBFloat16 || q.dim() != 4 || !q.is_cuda())
+    if (q.scalar_type() != at::kBFloat16 || q.dim() != 4)
       throw ArgumentError("query must be a bfloat16 CUDA tensor [batch, rows, heads, width]");
-    const c10::Device device = q.device();
     const int64_t batch = q.size(0), rows = q.size(1), heads = q.size(2), width = q.size(3);
+    // The stride between tokens, also where an expanded query has 0: the C
+    // ABI's 0 is dense rows, which the storage of one token does not hold.
     const int64_t stride = rows > 1 ? q.stride(1) : batch > 1 ? q.stride(0) : heads * width;
-    if ((q.stride(3) != 1 && width > 1) || (q.stride(2) != width && heads > 1) ||
+    if ((q.stride(3) != 1 && width > 1) || (q.stride(2) != width && heads > 1) || stride < heads * width ||
         (rows > 1 && batch > 1 && q.stride(0) != rows * stride))
-      throw ArgumentError("query: heads contiguous, one stride between tokens");
+      throw ArgumentError("query: heads contiguous, one stride between tokens, at least a token's heads");
+    if (!q.is_cuda()) throw ArgumentError("query must be a bfloat16 CUDA tensor [batch, rows, heads, width]");
+    const c10::Device device = q.device();
     dl_shared_attention a = {};
     a.batch = batch;
     a.rows = rows;
