@@ -883,6 +883,28 @@ bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
   return x < y + b_bytes && y < x + a_bytes;
 }
 
+// Rows of `width` elements at c * outer + s * inner, c < caches, s < slots
+// (width <= inner), and the same rows `offset` elements further: whether a row
+// of the one set meets a row of the other.  own: there is one set, whose rows
+// are only compared with one another.
+bool rows_meet(bool own, long long offset, size_t caches, size_t slots, size_t outer, size_t inner, size_t width) {
+  using wide = __int128;
+  const wide last_cache = wide(caches) - 1, last_slot = wide(slots) - 1, step = outer, row = inner, n = width;
+  const wide one = last_slot * row + n, extent = last_cache * step + one;  // a cache, all of them
+  if (own ? step >= one || (step >= n && row >= last_cache * step + n) : offset >= extent || -wide(offset) >= extent)
+    return false;
+  if (!own && step % row == 0) {  // beside one another within a position?
+    const wide at = (offset % row + row) % row;
+    if (at >= n && at + n <= row) return false;
+  }
+  for (wide c = own ? 1 : -last_cache; c <= last_cache; ++c) {
+    const wide d = offset + c * step, near = -d / row;  // the slots nearest to meeting are `near` or one off
+    for (wide s = near - 1; s <= near + 1; ++s)
+      if (s >= -last_slot && s <= last_slot && d + s * row < n && -(d + s * row) < n) return true;
+  }
+  return false;
+}
+
 dl_status evict_args(const dl_cache_eviction* e, dl::EvictArgs* o) {
   if (!e) return fail(DL_INVALID_ARGUMENT, "cache evict: null arguments");
   if (!e->caches || !e->kv_heads || !e->width || !e->capacity || !e->budget)
@@ -982,6 +1004,14 @@ DL_API dl_status dl_cache_evict(const dl_cache_eviction* e, void* workspace, voi
         overlap(e->weights_out, out4, e->weights, in4) || overlap(e->positions_out, out4, e->positions, in4))
       return fail(DL_INVALID_ARGUMENT, "cache evict: outputs overlap the inputs without being them");
   }
+  // Every row that is written has a place of its own, in place also among the
+  // slots that are only read.  Keys that are the values move alike in place.
+  const size_t slots = o.in_place ? e->capacity : size_t(o.budget), row = e->kv_heads * e->width;
+  const long long apart = (reinterpret_cast<intptr_t>(e->value_out) - reinterpret_cast<intptr_t>(e->key_out)) / 2;
+  if (rows_meet(true, 0, e->caches, slots, e->out_cache_stride, e->out_row_stride, row) ||
+      (!(o.in_place && apart == 0) &&
+       rows_meet(false, apart, e->caches, slots, e->out_cache_stride, e->out_row_stride, row)))
+    return fail(DL_INVALID_ARGUMENT, "cache evict: output rows overlap one another");
   return cuda_status(dl::launch_cache_evict(o, workspace, device_sms(), st(stream)), "cache evict");
 }
 

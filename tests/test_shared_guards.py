@@ -1,9 +1,12 @@
 """Calls of the shared-prefix operators that would read or write memory that is
 not theirs: refused on the host, before any device is touched."""
+import ctypes as C
+
 import pytest
 import torch
 
-from dolittle_b200 import shared
+import dolittle_b200 as dl
+from dolittle_b200 import _lib, shared
 
 
 def cache(*shape):
@@ -33,3 +36,65 @@ def test_one_token_may_have_any_strides():
     key = cache(20, 2, 128)
     with pytest.raises(ValueError, match="CUDA"):
         shared.attention_shared(q, key, key, None, None, torch.full((1,), 20), None)
+
+
+# ---------------------------------------------------------------------------
+# Eviction through the C ABI; the addresses are never read.
+# ---------------------------------------------------------------------------
+P = 1 << 30
+
+
+def eviction(apart, **change):
+    """Three caches of 100 slots, 2 heads of 64; values `apart` elements after the keys, all in place."""
+    e = _lib.CacheEviction(3, 2, 64, 100, 50, 0, 0, P, P + 2 * apart, 128, 12800, 2 * P, 3 * P, 4 * P, P, P + 2 * apart,
+                           100, 128, 12800, 2 * P, 3 * P, 4 * P)
+    for k, v in change.items():
+        setattr(e, k, v)
+    return e
+
+
+FRESH = dict(weights_out=6 * P, positions_out=7 * P, lengths_out=8 * P)
+
+
+@pytest.mark.parametrize("apart,change", [
+    # in place: every cache at one address, or a slot of one where another's lies
+    (1 << 20, dict(out_cache_stride=0)),
+    (1 << 20, dict(out_cache_stride=64)),
+    (1 << 20, dict(out_cache_stride=99 * 128)),
+    (64, dict(out_row_stride=256, out_cache_stride=25600)),
+    (12800, {}),  # the values are the next cache's keys
+    # into other buffers (50 slots): the same, and values over keys
+    (1 << 20, dict(key_out=9 * P, value_out=10 * P, out_cache_stride=0, **FRESH)),
+    (1 << 20, dict(key_out=9 * P, value_out=10 * P, out_cache_stride=49 * 128, **FRESH)),
+    (1 << 20, dict(key_out=9 * P, value_out=9 * P, **FRESH)),
+    (1 << 20, dict(key_out=9 * P, value_out=9 * P + 2 * 49 * 128, **FRESH)),
+    (1 << 20, dict(key_out=9 * P + 2 * 12800, value_out=9 * P, **FRESH)),
+])
+def test_evictions_whose_output_rows_overlap_are_refused(apart, change):
+    e = eviction(apart, **change)
+    if e.key_out == e.key:
+        e.row_stride, e.cache_stride = e.out_row_stride, e.out_cache_stride
+    L = dl.lib()
+    assert L.dl_cache_evict(C.byref(e), P, None) == _lib.DL_INVALID_ARGUMENT
+    assert b"rows overlap" in L.dl_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls would be made")
+@pytest.mark.parametrize("apart,change", [
+    (1 << 20, {}),
+    (0, {}),                                                        # keys that are the values
+    (128, dict(out_row_stride=256, out_cache_stride=25600)),        # keys and values of a position side by side
+    (1 << 20, dict(out_row_stride=3 * 128, out_cache_stride=128)),  # the caches' slots side by side
+    (3 * 128, dict(out_row_stride=6 * 128, out_cache_stride=128)),  # both
+    (1 << 20, dict(caches=1, out_cache_stride=0)),
+    (1 << 20, dict(key_out=9 * P, value_out=9 * P + 2 * 128, out_row_stride=256, out_cache_stride=25600, **FRESH)),
+    (1 << 20, dict(key_out=9 * P, value_out=10 * P, out_cache_stride=49 * 128 + 128, **FRESH)),
+    (1 << 20, dict(key_out=9 * P, value_out=9 * P + 2 * 50 * 128, **FRESH)),  # in each other's free slots
+])
+def test_evictions_into_rows_of_their_own_are_not_refused(apart, change):
+    """Without a device they come as far as the launch."""
+    e = eviction(apart, **change)
+    if e.key_out == e.key:
+        e.row_stride, e.cache_stride = e.out_row_stride, e.out_cache_stride
+    L = dl.lib()
+    assert L.dl_cache_evict(C.byref(e), P, None) == _lib.DL_CUDA_ERROR, L.dl_last_error()
