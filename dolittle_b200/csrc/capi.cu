@@ -1012,6 +1012,20 @@ DL_API dl_status dl_cache_evict(const dl_cache_eviction* e, void* workspace, voi
       (!(o.in_place && apart == 0) &&
        rows_meet(false, apart, e->caches, slots, e->out_cache_stride, e->out_row_stride, row)))
     return fail(DL_INVALID_ARGUMENT, "cache evict: output rows overlap one another");
+  // Nor do the sums, positions and lengths, whose blocks read and write at
+  // different times; an output may only be its own input.
+  const size_t in4 = 4 * e->caches * e->kv_heads * e->capacity, out4 = 4 * e->caches * e->kv_heads * e->out_capacity;
+  const size_t lengths = 8 * e->caches;
+  const struct {
+    const void* at;
+    size_t bytes;
+  } in[] = {{e->weights, in4}, {e->positions, in4}, {e->lengths, lengths}},
+    out[] = {{e->weights_out, out4}, {e->positions_out, out4}, {e->lengths_out, lengths}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j)
+      if ((!(i == j && in[i].at == out[i].at) && overlap(in[i].at, in[i].bytes, out[j].at, out[j].bytes)) ||
+          (i < j && overlap(out[i].at, out[i].bytes, out[j].at, out[j].bytes)))
+        return fail(DL_INVALID_ARGUMENT, "cache evict: weights, positions or lengths overlap one another");
   return cuda_status(dl::launch_cache_evict(o, workspace, device_sms(), st(stream)), "cache evict");
 }
 

@@ -531,7 +531,8 @@ DL_API dl_status dl_attention_shared(const dl_shared_attention* a, const void* q
  * moved rows are touched) or buffers that overlap none of them; slots from
  * min(length, budget) on are not written.  lengths_out may be lengths.  Rows
  * that are written do not overlap one another: no cache stride of 0, no values
- * in the keys' place.
+ * in the keys' place.  Nor do weights, positions and lengths: each output is
+ * its own input or apart from all.
  * width a multiple of 8, pointers 16-byte aligned, strides multiples of 8.
  * workspace: dl_cache_evict_workspace_bytes() bytes, any contents. */
 typedef struct {

@@ -98,3 +98,27 @@ def test_evictions_into_rows_of_their_own_are_not_refused(apart, change):
         e.row_stride, e.cache_stride = e.out_row_stride, e.out_cache_stride
     L = dl.lib()
     assert L.dl_cache_evict(C.byref(e), P, None) == _lib.DL_CUDA_ERROR, L.dl_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    dict(lengths_out=4 * P + 8),            # moved by one cache: a block may still read what another writes
+    dict(lengths_out=2 * P),                # the weights'
+    dict(lengths_out=3 * P + 4 * 599),      # the last position
+    dict(weights_out=6 * P, positions_out=6 * P, key_out=9 * P, value_out=10 * P),
+    dict(weights_out=3 * P + 2000, positions_out=7 * P, key_out=9 * P, value_out=10 * P),
+    dict(weights_out=4 * P, positions_out=7 * P, key_out=9 * P, value_out=10 * P),
+])
+def test_sums_positions_and_lengths_that_overlap_are_refused(change):
+    L = dl.lib()
+    assert L.dl_cache_evict(C.byref(eviction(1 << 20, **change)), P, None) == _lib.DL_INVALID_ARGUMENT
+    assert b"overlap" in L.dl_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls would be made")
+@pytest.mark.parametrize("change", [
+    dict(lengths_out=4 * P + 24),  # right behind the lengths
+    dict(key_out=9 * P, value_out=10 * P, weights_out=6 * P, positions_out=7 * P, lengths_out=4 * P),
+])
+def test_lengths_beside_or_in_place_are_not_refused(change):
+    L = dl.lib()
+    assert L.dl_cache_evict(C.byref(eviction(1 << 20, **change)), P, None) == _lib.DL_CUDA_ERROR, L.dl_last_error()
