@@ -965,6 +965,13 @@ DL_API dl_status dl_attention_shared(const dl_shared_attention* a, const void* q
   if (!query || !output || !workspace) return fail(DL_INVALID_ARGUMENT, "attention shared: null pointer");
   if (misaligned(query) || misaligned(output) || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(DL_UNSUPPORTED, "attention shared: query and output 16-byte, workspace 256-byte aligned");
+  // Queries are read until the last kernel of a call, after outputs were
+  // written: the two share no element (rows of one stride may interleave).
+  const size_t tokens = a->batch * a->rows, row = a->query_heads * a->width;
+  const long long apart = (reinterpret_cast<intptr_t>(output) - reinterpret_cast<intptr_t>(query)) / 2;
+  if (o.ldq == o.ldo ? rows_meet(false, apart, 1, tokens, 0, o.ldq, row)
+                     : overlap(query, 2 * ((tokens - 1) * o.ldq + row), output, 2 * ((tokens - 1) * o.ldo + row)))
+    return fail(DL_INVALID_ARGUMENT, "attention shared: output overlaps the query");
   o.q = static_cast<const bf16*>(query);
   o.out = static_cast<bf16*>(output);
   o.lse = lse;

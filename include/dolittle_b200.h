@@ -506,9 +506,10 @@ typedef struct {
  * weight each key received from every row, and query head of its group (and
  * from every sequence, for prefix keys), in this call.  width 64 or 128,
  * query_heads a multiple of kv_heads with a ratio up to 64, pointers 16-byte
- * aligned, strides multiples of 8.  Rows of a cache at or past every length
- * may hold anything (NaN too); a key some row attends must be finite.  Same
- * inputs, same bits: no sum depends on the order in which blocks run.
+ * aligned, strides multiples of 8; output and query share no element.  Rows
+ * of a cache at or past every length may hold anything (NaN too); a key some
+ * row attends must be finite.  Same inputs, same bits: no sum depends on the
+ * order in which blocks run.
  * workspace: dl_attention_shared_workspace_bytes() bytes, 256-byte aligned,
  * any contents; not shared by calls that may overlap on the device. */
 DL_API size_t dl_attention_shared_workspace_bytes(const dl_shared_attention* a, int weights);

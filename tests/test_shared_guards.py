@@ -122,3 +122,39 @@ def test_sums_positions_and_lengths_that_overlap_are_refused(change):
 def test_lengths_beside_or_in_place_are_not_refused(change):
     L = dl.lib()
     assert L.dl_cache_evict(C.byref(eviction(1 << 20, **change)), P, None) == _lib.DL_CUDA_ERROR, L.dl_last_error()
+
+
+# ---------------------------------------------------------------------------
+# Attention through the C ABI; the addresses are never read.
+# ---------------------------------------------------------------------------
+def attention(output, query_stride=0, output_stride=0):
+    """Three sequences of two tokens, 4 heads of 64 (256 elements a token), query at P."""
+    a = _lib.SharedAttention(3, 2, 4, 2, 64, query_stride, output_stride, 2 * P, 3 * P, 100, 128, 4 * P, 5 * P, 6 * P, 50,
+                             128, 6400, 7 * P)
+    L = dl.lib()
+    return L.dl_attention_shared(C.byref(a), P, output, None, None, None, 8 * P, None), L.dl_last_error()
+
+
+@pytest.mark.parametrize("output,strides", [
+    (P, (0, 0)),                        # in place
+    (P + 2 * 256, (0, 0)),              # over the next token
+    (P + 2 * (6 * 256 - 8), (0, 0)),    # the last token's end
+    (P - 2 * 248, (0, 0)),
+    (P + 2 * 256, (504, 504)),          # between the tokens of a fused row, eight elements too far
+    (P, (512, 256)),                    # dense over the tokens of a fused row
+    (P + 2 * 5 * 512, (512, 0)),
+])
+def test_outputs_over_the_query_are_refused(output, strides):
+    status, reason = attention(output, *strides)
+    assert status == _lib.DL_INVALID_ARGUMENT and b"overlaps the query" in reason
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls would be made")
+@pytest.mark.parametrize("output,strides", [
+    (P + 2 * 6 * 256, (0, 0)),       # right behind the query
+    (P + 2 * 256, (512, 512)),       # the other half of each fused row
+    (P - 2 * 256, (512, 512)),
+    (P + 2 * (5 * 512 + 256), (512, 0)),
+])
+def test_outputs_beside_the_query_are_not_refused(output, strides):
+    assert attention(output, *strides)[0] == _lib.DL_CUDA_ERROR
