@@ -90,6 +90,20 @@ T* flat(PyObject* o, const char* name, at::ScalarType type, at::IntArrayRef size
   return static_cast<T*>(t.data_ptr());
 }
 
+// A reference of our own.
+struct Reference {
+  PyObject* object = nullptr;
+  Reference() = default;
+  Reference(const Reference&) = delete;
+  Reference& operator=(const Reference&) = delete;
+  ~Reference() { Py_XDECREF(object); }
+  void hold(PyObject* o) {
+    Py_INCREF(o);
+    object = o;
+  }
+  operator PyObject*() const { return object; }
+};
+
 struct Refused {
   dl_status status;
 };
@@ -215,22 +229,23 @@ PyObject* py_attention_shared(PyObject*, PyObject* const* arg, Py_ssize_t n) {
 PyObject* py_cache_evict(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 9) throw ArgumentError("cache_evict takes 9 arguments");
-    const at::Tensor& key = tensor(arg[0], "key caches");
-    if (!key.is_cuda()) throw ArgumentError("the caches must be CUDA tensors");
-    const c10::Device device = key.device();
-    const Caches c = caches(arg[0], arg[1], "cache", 4, device);
-    PyObject* out[5];
+    // The results' own references, until they are returned: a sequence may
+    // make its elements on access and keep none, or change meanwhile.
+    Reference out[5];
     if (arg[8] == Py_None) {
-      for (int i = 0; i < 5; ++i) out[i] = arg[i];
+      for (int i = 0; i < 5; ++i) out[i].hold(arg[i]);
     } else {
       if (!PySequence_Check(arg[8]) || PySequence_Size(arg[8]) != 5)
         throw ArgumentError("out must be (key, value, weights, positions, lengths)");
       for (int i = 0; i < 5; ++i) {
-        out[i] = PySequence_GetItem(arg[8], i);
+        out[i].object = PySequence_GetItem(arg[8], i);
         if (!out[i]) throw ArgumentError("out must be (key, value, weights, positions, lengths)");
-        Py_DECREF(out[i]);  // the sequence keeps it
       }
     }
+    const at::Tensor& key = tensor(arg[0], "key caches");
+    if (!key.is_cuda()) throw ArgumentError("the caches must be CUDA tensors");
+    const c10::Device device = key.device();
+    const Caches c = caches(arg[0], arg[1], "cache", 4, device);
     const Caches o = arg[8] == Py_None ? c : caches(out[0], out[1], "out", 4, device);
     if (o.count != c.count || o.heads != c.heads || o.width != c.width)
       throw ArgumentError("the output caches must be [caches, positions, heads, width] like the inputs");
@@ -265,7 +280,7 @@ PyObject* py_cache_evict(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     status = cache_evict(&e, workspace.data_ptr(), stream);
     Py_END_ALLOW_THREADS
     require(status);
-    return PyTuple_Pack(5, out[0], out[1], out[2], out[3], out[4]);
+    return PyTuple_Pack(5, out[0].object, out[1].object, out[2].object, out[3].object, out[4].object);
   });
 }
 

@@ -1,6 +1,7 @@
 """Calls of the shared-prefix operators that would read or write memory that is
 not theirs: refused on the host, before any device is touched."""
 import ctypes as C
+import weakref
 
 import pytest
 import torch
@@ -158,3 +159,32 @@ def test_outputs_over_the_query_are_refused(output, strides):
 ])
 def test_outputs_beside_the_query_are_not_refused(output, strides):
     assert attention(output, *strides)[0] == _lib.DL_CUDA_ERROR
+
+
+# ---------------------------------------------------------------------------
+# Output sequences that keep nothing
+# ---------------------------------------------------------------------------
+class MadeOnAccess:
+    """Five elements, each made when it is asked for; counts those that went away before the call was over."""
+
+    def __init__(self, *make):
+        self.make, self.alive, self.lost = make, [], 0
+
+    def __len__(self):
+        return len(self.make)
+
+    def __getitem__(self, i):
+        self.lost += sum(r() is None for r in self.alive)
+        x = self.make[i]()
+        self.alive.append(weakref.ref(x))
+        return x
+
+
+def test_outputs_of_an_eviction_are_held_until_it_returns():
+    """The call comes as far as the device's check here; every element made so far is alive until then."""
+    t = cache(1, 8, 2, 64)
+    out = MadeOnAccess(*[lambda: cache(1, 4, 2, 64)] * 5)
+    with pytest.raises(ValueError, match="CUDA"):
+        shared.cache_evict(t, t.clone(), None, None, None, 4, out=out)
+    assert len(out.alive) == 5 and out.lost == 0
+    assert all(r() is None for r in out.alive)  # and given back afterwards
