@@ -162,22 +162,23 @@ class Branches:
 
     def evict_prefix(self, budget: int, first: int = 4, recent: int = 0) -> None:
         """Keep `budget` prompt keys per block and KV head, those the branches
-        looked at most (and the `first` and `recent` positions), in a cache of
-        the branches' own; the engine's is left as it is."""
+        looked at most (and the `first` and `recent` positions, together at
+        most `budget`), or all of a shorter prompt, in a cache of the branches'
+        own; the engine's is left as it is."""
         self._summed()
-        budget = min(budget, self.prefix)
+        kept = min(budget, self.prefix)
         lengths = torch.full((1,), self.prefix, dtype=torch.int64, device=self._device)
         for i, (key, value) in enumerate(self._prefix):
-            out = [torch.empty((1, budget, *key.shape[1:]), dtype=_BF16, device=self._device) for _ in range(2)]
-            out += [torch.empty((1, key.shape[1], budget), device=self._device),
-                    torch.empty((1, key.shape[1], budget), dtype=torch.int32, device=self._device),
+            out = [torch.empty((1, kept, *key.shape[1:]), dtype=_BF16, device=self._device) for _ in range(2)]
+            out += [torch.empty((1, key.shape[1], kept), device=self._device),
+                    torch.empty((1, key.shape[1], kept), dtype=torch.int32, device=self._device),
                     torch.empty_like(lengths)]
             shared.cache_evict(key[None], value[None], self.prefix_weights[i][None], self._prefix_positions[i], lengths,
                                budget, first=first, recent=recent, out=out)
             self._prefix[i] = (out[0][0], out[1][0])
             self.prefix_weights[i], self._prefix_positions[i] = out[2][0], out[3]
-        self.prefix = budget
-        self._prefix_lengths.fill_(budget)
+        self.prefix = kept
+        self._prefix_lengths.fill_(kept)
 
     def evict_suffix(self, budget: int, recent: int = 32) -> None:
         """Keep `budget` slots of every branch's own cache, in place: the

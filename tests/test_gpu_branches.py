@@ -99,3 +99,23 @@ def test_refusals():
         b.evict_prefix(2)  # no weights were summed
     with pytest.raises(dl.DolittleError):
         e.kv_device(99, False)
+
+
+@pytest.mark.parametrize("prompt,budget,first,recent", [(200, 256, 4, 200), (3, 64, 4, 0), (40, 40, 4, 36), (5, 1 << 40, 0, 9)])
+def test_a_budget_at_or_above_the_prompt_keeps_it(prompt, budget, first, recent):
+    """Everything fits the budget: all slots stay, whatever is protected."""
+    rng = np.random.default_rng(prompt)
+    e = engine()
+    e.consume_view(rng.integers(0, CONFIG.vocabulary, prompt))
+    b = Branches(e, 2, 8, weights=True)
+    ids = torch.from_numpy(rng.integers(0, CONFIG.vocabulary, (2, 3))).cuda()
+    b.step(ids[:, 0])
+    keys = [(k.clone(), v.clone()) for k, v in b._prefix]
+    sums = [w.clone() for w in b.prefix_weights]
+    b.evict_prefix(budget, first=first, recent=recent)
+    assert b.prefix == prompt and b._prefix_lengths.tolist() == [prompt] * 2
+    assert all(torch.equal(x[0], y[0]) and torch.equal(x[1], y[1]) for x, y in zip(b._prefix, keys))
+    assert all(torch.equal(x, y) for x, y in zip(b.prefix_weights, sums))
+    again = Branches(e, 2, 8)
+    again.step(ids[:, 0])
+    assert torch.equal(b.step(ids[:, 1]), again.step(ids[:, 1]))
