@@ -61,6 +61,7 @@ class Branches:
                                                                                                   device=dev)
         self._prefix_lengths = torch.full((batch,), self.prefix, dtype=torch.int64, device=dev)
         self._suffix_lengths = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self._unknown = torch.zeros(batch, dtype=torch.bool, device=dev)  # branches that were given unknown ids
         self._next = torch.full((1,), self.position, dtype=torch.int64, device=dev)  # position of the next token
         self.prefix_weights = self.suffix_weights = None
         if weights:
@@ -78,13 +79,22 @@ class Branches:
 
     # ---- one step ----------------------------------------------------------
     def step(self, tokens) -> torch.Tensor:
-        """The next tokens of every branch, [batch, rows] (or [batch]) ids on
-        the device; returns the last row's logits, [batch, V] BF16."""
-        tokens = torch.as_tensor(tokens, device=self._device).to(torch.int32)
-        tokens = (tokens if tokens.dim() == 2 else tokens[:, None]).contiguous()
+        """The next tokens of every branch, [batch, rows] (or [batch]) ids;
+        returns the last row's logits, [batch, V] BF16.  Ids outside the
+        vocabulary raise ValueError where the host has them; on the device they
+        are not waited for, and their branch's logits are NaN from there on."""
+        tokens = torch.as_tensor(tokens).to(torch.int64)
+        tokens = tokens if tokens.dim() == 2 else tokens[:, None]
         batch, rows = tokens.shape
         if batch != self.batch or rows < 1 or self.length + rows > self.capacity:
             raise ValueError("tokens must be [batch, rows] and fit the capacity")
+        unknown = (tokens < 0) | (tokens >= self.config.vocabulary)
+        if tokens.is_cuda:  # the embedding's rows are read as the ids say
+            self._unknown |= unknown.any(1)
+            tokens = tokens.masked_fill(unknown, 0)
+        elif bool(unknown.any()):
+            raise ValueError("token ids must be below the vocabulary's size")
+        tokens = tokens.to(self._device, torch.int32).contiguous()
         c, d = self.config, self.config.head_width
         stream = torch.cuda.current_stream().cuda_stream
         q_width, kv_width, m = c.query_heads * d, c.kv_heads * d, batch * rows
@@ -126,7 +136,7 @@ class Branches:
         self._norm(last, self._weight[1], normed, batch, c.hidden, stream)
         logits = torch.empty((batch, c.vocabulary), **new)
         self._project(normed[:batch], self._weight[2], logits, c.vocabulary, c.hidden, 0, stream)
-        return logits
+        return logits.masked_fill_(self._unknown[:, None], float("nan"))
 
     def _norm(self, x, weight, out, rows, width, stream):
         check(lib().dl_rms_norm(_lib.DL_BF16, x.data_ptr(), weight, out.data_ptr(), rows, width, self.config.epsilon,

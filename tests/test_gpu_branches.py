@@ -119,3 +119,35 @@ def test_a_budget_at_or_above_the_prompt_keeps_it(prompt, budget, first, recent)
     again = Branches(e, 2, 8)
     again.step(ids[:, 0])
     assert torch.equal(b.step(ids[:, 1]), again.step(ids[:, 1]))
+
+
+@pytest.mark.parametrize("bad", [-1, CONFIG.vocabulary, (1 << 32) + 5, -(1 << 31), 1 << 40])
+def test_ids_outside_the_vocabulary(bad):
+    """Refused where the host has them; on the device their branch turns NaN and no other branch changes."""
+    rng = np.random.default_rng(2)
+    e = engine()
+    e.consume_view(rng.integers(0, CONFIG.vocabulary, 30))
+    ids = torch.from_numpy(rng.integers(0, CONFIG.vocabulary, (3, 4)))
+    wrong = ids.clone()
+    wrong[1, 1] = bad
+    a, b = Branches(e, 3, 8, weights=True), Branches(e, 3, 8, weights=True)
+    with pytest.raises(ValueError, match="vocabulary"):
+        b.step(wrong)
+    assert b.length == 0 and b.position == 30
+    for at, rows in ((0, 1), (1, 2), (3, 1)):
+        right = a.step(ids[:, at:at + rows].cuda())
+        got = b.step(wrong[:, at:at + rows].cuda())
+        assert bool(torch.isfinite(right.float()).all())
+        assert torch.equal(got[0::2], right[0::2])
+        assert bool(torch.isnan(got[1]).all()) == (at >= 1) and (at >= 1 or torch.equal(got[1], right[1]))
+    assert all(bool(torch.isfinite(w).all()) for w in b.prefix_weights)
+
+
+def test_ids_may_come_from_the_host():
+    rng = np.random.default_rng(3)
+    e = engine()
+    e.consume_view(rng.integers(0, CONFIG.vocabulary, 30))
+    ids = rng.integers(0, CONFIG.vocabulary, (2, 3))
+    a, b = Branches(e, 2, 8), Branches(e, 2, 8)
+    assert torch.equal(a.step(torch.from_numpy(ids).cuda()), b.step(ids))
+    assert torch.equal(a.step(torch.from_numpy(ids[:, 0]).int().cuda()), b.step(ids[:, 0].tolist()))
