@@ -37,7 +37,8 @@ class Branches:
     """`batch` sequences that continue what `engine` has consumed so far, in
     lockstep; each may grow by `capacity` tokens.  The engine's cache is read in
     place: it must not be reset or extended while branches use it (until
-    `evict_prefix` has made a copy).  Head width 64 or 128, other widths as the
+    `evict_prefix` has made a copy), and the engine, whose weights they use,
+    stays open.  Head width 64 or 128, other widths as the
     tensor-core projections want them (hidden a multiple of 64, projections a
     multiple of 128 rows)."""
 
@@ -77,12 +78,18 @@ class Branches:
             raise ValueError("the engine's q, k and v weights must be one matrix")
         self._scratch = None
 
+    def _open(self):
+        """The weights are the engine's, and so is the prompt's cache at first."""
+        if not self.engine._h:
+            raise ValueError("the branches' engine is closed")
+
     # ---- one step ----------------------------------------------------------
     def step(self, tokens) -> torch.Tensor:
         """The next tokens of every branch, [batch, rows] (or [batch]) ids;
         returns the last row's logits, [batch, V] BF16.  Ids outside the
         vocabulary raise ValueError where the host has them; on the device they
         are not waited for, and their branch's logits are NaN from there on."""
+        self._open()
         tokens = torch.as_tensor(tokens).to(torch.int64)
         tokens = tokens if tokens.dim() == 2 else tokens[:, None]
         batch, rows = tokens.shape
@@ -176,6 +183,7 @@ class Branches:
         most `budget`), or all of a shorter prompt, in a cache of the branches'
         own; the engine's is left as it is."""
         self._summed()
+        self._open()
         kept = min(budget, self.prefix)
         lengths = torch.full((1,), self.prefix, dtype=torch.int64, device=self._device)
         for i, (key, value) in enumerate(self._prefix):

@@ -151,3 +151,19 @@ def test_ids_may_come_from_the_host():
     a, b = Branches(e, 2, 8), Branches(e, 2, 8)
     assert torch.equal(a.step(torch.from_numpy(ids).cuda()), b.step(ids))
     assert torch.equal(a.step(torch.from_numpy(ids[:, 0]).int().cuda()), b.step(ids[:, 0].tolist()))
+
+
+def test_a_closed_engine_is_refused():
+    e = engine(64)
+    e.consume_view([1, 2, 3])
+    b = Branches(e, 2, 4, weights=True)
+    b.step([1, 2])
+    torch.cuda.synchronize()
+    e.close()
+    with pytest.raises(ValueError, match="closed"):
+        b.step([1, 2])
+    with pytest.raises(ValueError, match="closed"):
+        b.evict_prefix(8)
+    assert b.length == 1
+    b.evict_suffix(1, recent=1)  # the branches' own
+    assert b.length == 1
