@@ -48,14 +48,14 @@ class Branches:
             raise ValueError("a consumed prompt, a batch and a capacity are required")
         self.engine, self.config, self.batch, self.capacity = engine, c, batch, capacity
         self.prefix, self.position, self.length = engine.position, engine.position, 0
-        self._device = torch.device("cuda", torch.cuda.current_device())
-        d, dev = c.head_width, self._device
+        d = c.head_width
 
         def cache(layer, values):
             pointer, stride = engine.kv_device(layer, values)
-            rows = torch.as_tensor(_Device(pointer, (self.prefix, stride), engine), device=dev).view(_BF16)
+            rows = torch.as_tensor(_Device(pointer, (self.prefix, stride), engine)).view(_BF16)
             return rows.view(self.prefix, c.kv_heads, d)
 
+        self._device = dev = cache(0, False).device  # the engine's, whichever is current
         self._prefix = [(cache(i, False), cache(i, True)) for i in range(c.layers)]
         kv = (c.layers, batch, capacity, c.kv_heads, d)
         self._suffix_key, self._suffix_value = torch.zeros(kv, dtype=_BF16, device=dev), torch.zeros(kv, dtype=_BF16,
@@ -102,6 +102,10 @@ class Branches:
         elif bool(unknown.any()):
             raise ValueError("token ids must be below the vocabulary's size")
         tokens = tokens.to(self._device, torch.int32).contiguous()
+        with torch.cuda.device(self._device):
+            return self._step(tokens, batch, rows)
+
+    def _step(self, tokens, batch: int, rows: int) -> torch.Tensor:
         c, d = self.config, self.config.head_width
         stream = torch.cuda.current_stream().cuda_stream
         q_width, kv_width, m = c.query_heads * d, c.kv_heads * d, batch * rows

@@ -167,3 +167,15 @@ def test_a_closed_engine_is_refused():
     assert b.length == 1
     b.evict_suffix(1, recent=1)  # the branches' own
     assert b.length == 1
+
+
+def test_branches_are_on_their_engine_s_device(monkeypatch):
+    """Wherever the current device points, which here is one that need not exist."""
+    e = engine(64)
+    e.consume_view([1, 2, 3])
+    want = Branches(e, 2, 4).step([1, 2])
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "current_device", lambda: 1)
+        b = Branches(e, 2, 4)
+    assert b._device == want.device and all(k.device == want.device for k, _ in b._prefix)
+    assert torch.equal(b.step([1, 2]), want)
