@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
         const int g = k0 + i;
         for (int b = 0; b < boxes; ++b) {
           if (g < np) tma_3d(dst + b * kAtom, value ? &t.pv : &t.pk, 64 * b, h, g * kKeys, bar);
-          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, seq, bar);
+          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, suffix_at(a, seq), bar);
         }
         at.next();
         ++c;

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from dolittle_b200 import shared
-from tests.test_gpu_shared import make_caches
+from tests.test_gpu_shared import check_attention, make, make_caches
 from tests.test_shared_guards import MadeOnAccess
 
 pytestmark = pytest.mark.gpu
@@ -20,3 +20,19 @@ def test_eviction_into_outputs_that_a_sequence_makes_on_access():
     assert out.lost == 0 and got[4].tolist() == [16, 16]
     assert all(torch.equal(x[:, :16], y[:, :16]) for x, y in zip(got[:2], want[:2]))
     assert all(torch.equal(x[..., :16], y[..., :16]) for x, y in zip(got[2:4], want[2:4]))
+
+
+@pytest.mark.parametrize("batch,rows,prefix,suffix,hq,hkv,d,slens", [
+    (5, 1, 300, 70, 32, 8, 128, [70, 69, 1, 0, 33]),   # the few-row kernel alone
+    (20, 1, 3000, 200, 32, 8, 128, None),              # beside tiles over the prefix
+    (3, 40, 260, 300, 28, 4, 64, [300, 40, 211]),      # tiles over both
+    (2, 129, None, 400, 8, 8, 128, [400, 333]),
+])
+def test_one_suffix_cache_expanded_over_the_sequences(batch, rows, prefix, suffix, hq, hkv, d, slens):
+    """Every sequence reads the same suffix rows (a sequence stride of 0), as far as its own length goes."""
+    t = make(batch, rows, prefix, suffix, hq, hkv, d, seed=batch, slens=slens)
+    for part in ("key", "value"):
+        longest = max(range(batch), key=lambda b: int(t["suffix_lengths"][b]))
+        t[f"suffix_{part}"] = t[f"suffix_{part}"][longest:longest + 1].expand(batch, -1, -1, -1)
+        assert t[f"suffix_{part}"].stride(0) == 0
+    check_attention(t)
