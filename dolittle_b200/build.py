@@ -11,9 +11,12 @@ no implicit multiply-add contraction.  Objects go to dolittle_b200/_build/.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -47,21 +50,32 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_torch_calls(force: bool = False) -> str:
+def build_torch_calls(force: bool = False):
     """The extension module that shared.py calls (host code only; torch's own
-    libraries are already loaded when it is imported)."""
+    libraries are already loaded when it is imported).  Returns its path, or
+    None where it cannot be built: the C ABI and everything else do without it,
+    and shared.py says what is missing."""
     header = os.path.join(ROOT, "include", "dolittle_b200.h")
     if not force and not _stale(TORCH_OUT, [TORCH_SRC, header]):
         return TORCH_OUT
-    import sysconfig
-
+    cxx, python = os.environ.get("CXX", "g++"), sysconfig.get_paths()["include"]
+    spec = importlib.util.find_spec("torch")
+    root = os.path.dirname(spec.origin) if spec else ""
+    missing = [what for what, there in (
+        ("torch", spec),
+        ("torch's headers", os.path.exists(os.path.join(root, "include", "ATen", "ATen.h"))),
+        ("torch's CUDA library", os.path.exists(os.path.join(root, "lib", "libc10_cuda.so"))),
+        ("Python's headers", os.path.exists(os.path.join(python, "Python.h"))),
+        (cxx, shutil.which(cxx))) if not there]
+    if missing:
+        sys.stderr.write(f"dolittle_b200: the torch calls (dolittle_b200.shared) are not built: no {missing[0]}\n")
+        return None
     import torch
-    root = os.path.dirname(torch.__file__)
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
            "-I", os.path.join(root, "include"),
            "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(CUDA_HOME, "include"), TORCH_SRC,
+           "-I", python, "-I", os.path.join(CUDA_HOME, "include"), TORCH_SRC,
            "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", TORCH_OUT]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
