@@ -6,8 +6,11 @@ There is no fallback: when it is missing, loading raises ImportError.
 from __future__ import annotations
 
 import ctypes as C
+import hashlib
+import importlib.util
 import os
 import re
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdolittle_b200.so")
@@ -20,6 +23,20 @@ DL_BF16, DL_F32 = 0, 1
 DL_PREFILL_PARITY, DL_PREFILL_FAST = 0, 1
 DL_DECODE_PERSISTENT, DL_DECODE_KERNELS = 0, 1
 DL_RNG_MT19937_64, DL_RNG_PHILOX4X32_10 = 0, 1
+
+
+def torch_calls_path() -> str:
+    """Where the extension module of shared.py lies for this Python and this
+    build of torch: it reads torch's objects by their C++ layout, so another
+    build's module is another file and never loaded.  Does not import torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise ImportError("dolittle_b200.shared needs torch")
+    root = os.path.dirname(spec.origin)
+    with open(os.path.join(root, "version.py"), "rb") as f:  # version, source revision, CUDA
+        build = hashlib.sha256(f.read())
+    build.update(str(os.path.getsize(os.path.join(root, "lib", "libtorch_python.so"))).encode())
+    return os.path.join(HERE, f"_torch_shared.{sysconfig.get_config_var('SOABI')}.{build.hexdigest()[:12]}.so")
 
 
 class DolittleError(RuntimeError):

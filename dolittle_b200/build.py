@@ -1,5 +1,6 @@
 """Build the sm_100a shared library in-tree, dolittle_b200/libdolittle_b200.so,
-and the torch-side calls of dolittle_b200/shared.py, dolittle_b200/_torch_shared.so.
+and the torch-side calls of dolittle_b200/shared.py, dolittle_b200/_torch_shared.*.so,
+named after the Python and the torch that they were built for.
 
     python -m dolittle_b200.build [--verbose-ptxas]
 
@@ -13,16 +14,18 @@ from __future__ import annotations
 import concurrent.futures as cf
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
 import sysconfig
 
+from ._lib import torch_calls_path
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdolittle_b200.so")
 TORCH_SRC = os.path.join(CSRC, "torch_shared.cpp")
-TORCH_OUT = os.path.join(HERE, "_torch_shared.so")
 BUILD = os.path.join(HERE, "_build")
 ROOT = os.path.dirname(HERE)
 
@@ -56,11 +59,12 @@ def build_torch_calls(force: bool = False):
     None where it cannot be built: the C ABI and everything else do without it,
     and shared.py says what is missing."""
     header = os.path.join(ROOT, "include", "dolittle_b200.h")
-    if not force and not _stale(TORCH_OUT, [TORCH_SRC, header]):
-        return TORCH_OUT
     cxx, python = os.environ.get("CXX", "g++"), sysconfig.get_paths()["include"]
     spec = importlib.util.find_spec("torch")
     root = os.path.dirname(spec.origin) if spec else ""
+    out = torch_calls_path() if spec else ""
+    if out and not force and not _stale(out, [TORCH_SRC, header]):
+        return out
     missing = [what for what, there in (
         ("torch", spec),
         ("torch's headers", os.path.exists(os.path.join(root, "include", "ATen", "ATen.h"))),
@@ -76,11 +80,14 @@ def build_torch_calls(force: bool = False):
            "-I", os.path.join(root, "include"),
            "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I", python, "-I", os.path.join(CUDA_HOME, "include"), TORCH_SRC,
-           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", TORCH_OUT]
+           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-o", out]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("torch calls failed to build:\n" + r.stdout + r.stderr)
-    return TORCH_OUT
+    for f in os.listdir(os.path.dirname(out)):  # of another torch or Python
+        if re.fullmatch(r"_torch_shared(\..*)?\.so", f) and f != os.path.basename(out):
+            os.remove(os.path.join(os.path.dirname(out), f))
+    return out
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:

@@ -27,7 +27,7 @@ def _extension():
     """The in-tree extension module that checks the tensors and makes the calls."""
     global _calls
     if _calls is None:
-        path = os.path.join(_lib.HERE, "_torch_shared.so")
+        path = _lib.torch_calls_path()
         if not os.path.exists(path):
             raise ImportError(f"{path} is missing: run `python -m dolittle_b200.build`")
         spec = importlib.util.spec_from_loader(
