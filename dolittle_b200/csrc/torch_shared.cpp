@@ -136,7 +136,6 @@ PyObject* wrap(PyObject* given, const at::Tensor& made) {
 }
 
 at::Tensor scratch(size_t bytes, c10::Device device) {
-  if (!bytes) throw Refused{DL_INVALID_ARGUMENT};  // the size query left the reason
   return at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(device));
 }
 
@@ -209,6 +208,7 @@ PyObject* py_attention_shared(PyObject*, PyObject* const* arg, Py_ssize_t n) {
       lse_ptr = flat<float>(arg[10], "lse", at::kFloat, {batch, rows, heads}, device);
     }
     const c10::cuda::OptionalCUDAGuard guard(device);
+    // A refused call has a workspace of 0 bytes, and the call itself says why.
     const at::Tensor workspace = scratch(attention_workspace_bytes(&a, pw || sw), device);
     void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     dl_status status;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from dolittle_b200 import shared
+from dolittle_b200 import _lib, shared
 from tests.test_gpu_shared import check_attention, make, make_caches
 from tests.test_shared_guards import MadeOnAccess
 
@@ -36,3 +36,27 @@ def test_one_suffix_cache_expanded_over_the_sequences(batch, rows, prefix, suffi
         t[f"suffix_{part}"] = t[f"suffix_{part}"][longest:longest + 1].expand(batch, -1, -1, -1)
         assert t[f"suffix_{part}"].stride(0) == 0
     check_attention(t)
+
+
+def test_refusals_carry_the_library_s_status():
+    """What is unsupported is told from what is invalid, as the C ABI does."""
+    key = torch.zeros(16, 8, 96, device="cuda", dtype=torch.bfloat16)
+    lengths = torch.full((2,), 16, device="cuda")
+
+    def status(call, *args, **kw):
+        with pytest.raises(_lib.DolittleError) as e:
+            call(*args, **kw)
+        return e.value.status, str(e.value)
+
+    q = torch.zeros(2, 1, 32, 96, device="cuda", dtype=torch.bfloat16)
+    got = status(shared.attention_shared, q, key, key, None, None, lengths, None)
+    assert got[0] == _lib.DL_UNSUPPORTED and "head width" in got[1]
+    got = status(shared.attention_shared, q[:, :0], key, key, None, None, lengths, None)
+    assert got[0] == _lib.DL_INVALID_ARGUMENT and "empty" in got[1]
+    c = make_caches(2, 64)
+    args = [c[k] for k in NAMES]
+    got = status(shared.cache_evict, *args, 0)
+    assert got[0] == _lib.DL_INVALID_ARGUMENT and "empty" in got[1]
+    odd = torch.zeros((2, 64, 2, 12), device="cuda", dtype=torch.bfloat16)
+    got = status(shared.cache_evict, odd, odd.clone(), *args[2:], 16)
+    assert got[0] == _lib.DL_UNSUPPORTED and "multiples of 8" in got[1]
