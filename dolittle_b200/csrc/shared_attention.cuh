@@ -140,17 +140,16 @@ inline bool encode_prefix_map(CUtensorMap* m, const SharedAttnArgs& a, const bf1
   const uint32_t box[3] = {64, 1, kKeys};
   return encode_bf16_map(m, base, 3, dims, strides, box);
 }
-// A suffix that all sequences share (sequence stride 0) is a map of one: strides
-// of 0 are not for tensor maps.
+// A suffix that all sequences share (sequence stride 0) is a map of one
+// sequence: strides of 0 are not for tensor maps.
+__host__ __device__ __forceinline__ bool one_suffix(const SharedAttnArgs& a) { return a.batch == 1 || a.s_seq == 0; }
 inline bool encode_suffix_map(CUtensorMap* m, const SharedAttnArgs& a, const bf16* base) {
-  const bool one = a.batch == 1 || a.s_seq == 0;
+  const bool one = one_suffix(a);
   const uint64_t dims[4] = {uint64_t(a.width), uint64_t(a.kv_heads), uint64_t(a.scap), uint64_t(one ? 1 : a.batch)};
   const uint64_t strides[3] = {uint64_t(a.width), a.s_row, one ? a.s_row * a.scap : a.s_seq};
   const uint32_t box[4] = {64, 1, kKeys, 1};
   return encode_bf16_map(m, base, 4, dims, strides, box);
 }
-// Sequence b in it.
-__device__ __forceinline__ int suffix_at(const SharedAttnArgs& a, int b) { return a.s_seq ? b : 0; }
 
 __device__ __forceinline__ int clamp_len(long long n, int cap) { return int(n < 0 ? 0 : n > cap ? cap : n); }
 __device__ __forceinline__ int prefix_len(const SharedAttnArgs& a, int b) {

@@ -101,7 +101,10 @@ __device__ __forceinline__ void mma_output(uint32_t tmem_o, uint32_t tmem_p, uin
   }
 }
 
-template <int D, bool WIDE, bool BESIDE>
+// ONE: all sequences share one suffix cache.  A kernel of its own, since the
+// loading thread asking for it cost the others 3 % (turns of 48 tokens on 4096
+// keys 48.4 -> 50.0 us).
+template <int D, bool WIDE, bool BESIDE, bool ONE>
 __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
     shared_tile_kernel(const __grid_constant__ TileArgs t) {
   using S = Shape<D, WIDE, BESIDE>;
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(Shape<D, WIDE, BESIDE>::bound, 1)
         const int g = k0 + i;
         for (int b = 0; b < boxes; ++b) {
           if (g < np) tma_3d(dst + b * kAtom, value ? &t.pv : &t.pk, 64 * b, h, g * kKeys, bar);
-          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, suffix_at(a, seq), bar);
+          else tma_4d(dst + b * kAtom, value ? &t.sv : &t.sk, 64 * b, h, (g - np) * kKeys, ONE ? 0 : seq, bar);
         }
         at.next();
         ++c;
@@ -669,19 +672,22 @@ __global__ void __launch_bounds__(32 * kMergeWarps) shared_merge_kernel(const Sh
   }
 }
 
-template <int D, bool WIDE, bool BESIDE>
+template <int D, bool WIDE, bool BESIDE, bool ONE = false>
 cudaError_t launch_tiles_shape(const TileArgs& t, cudaStream_t stream) {
   constexpr int smem = Shape<D, WIDE, BESIDE>::smem;
-  const cudaError_t e = allow_smem<shared_tile_kernel<D, WIDE, BESIDE>>(smem);
+  const cudaError_t e = allow_smem<shared_tile_kernel<D, WIDE, BESIDE, ONE>>(smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = unsigned(t.plan.full + (t.plan.tasks - t.plan.full) * t.plan.splits);
   DependentLaunch d(dim3(grid), kThreads, smem, stream);
-  return cudaLaunchKernelEx(&d.cfg, shared_tile_kernel<D, WIDE, BESIDE>, t);
+  return cudaLaunchKernelEx(&d.cfg, shared_tile_kernel<D, WIDE, BESIDE, ONE>, t);
 }
 
 template <int D>
 cudaError_t launch_tiles_width(const TileArgs& t, cudaStream_t stream) {
   if (t.plan.pooled) return launch_tiles_shape<D, false, true>(t, stream);
+  if (t.a.scap && t.a.batch > 1 && t.a.s_seq == 0)
+    return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, false, true>(t, stream)
+                               : launch_tiles_shape<D, false, false, true>(t, stream);
   return t.plan.per_cta == 2 ? launch_tiles_shape<D, true, false>(t, stream)
                              : launch_tiles_shape<D, false, false>(t, stream);
 }

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_weights_kernel(const __gri
         for (int p = 0; p < tiles; ++p)
           for (int c = 0; c < D / 64; ++c) {
             unsigned char* dst = mem(((keys & 1) * 2 + p) * slot + c * kAtom);
-            if (u.suffix) tma_4d(dst, &w.sk, 64 * c, u.h, u.j0 + p * kKeys, suffix_at(a, u.b), bar);
+            if (u.suffix) tma_4d(dst, &w.sk, 64 * c, u.h, u.j0 + p * kKeys, one_suffix(a) ? 0 : u.b, bar);
             else tma_3d(dst, &w.pk, 64 * c, u.h, u.j0 + p * kKeys, bar);
           }
         ++keys;
