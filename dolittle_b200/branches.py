@@ -10,6 +10,14 @@ verbalizer samples of one prefix).  A step here is the engine's block recipe
 also sums the weight each key receives, and `evict_prefix` / `evict_suffix` cut
 the caches by those sums (`shared.cache_evict`).
 
+The branches go in lockstep: one length for all, the whole prompt for each, and
+no steering (the batched server steers).  Batches whose sequences differ in
+length, or leave the prompt at different tokens, call `attention_shared` with
+lengths of their own.  A step launches about twenty kernels a block from
+Python, which bounds it: with the Qwen3-8B shapes 16 branches of a 2048-token
+prompt take 6.6 ms a step (5.4 on the device; the server with its full caches
+4.7), 32 of 8192 tokens 6.9 ms (the server 10.6).
+
     engine.consume_view(prompt, dl.DL_PREFILL_FAST)
     branches = Branches(engine, batch=16, capacity=128)
     logits = branches.step(tokens)             # [16, rows] ids -> [16, V]

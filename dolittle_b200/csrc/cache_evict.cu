@@ -16,11 +16,15 @@
 // between rows.  Integer counts and prefix sums only: results do not depend on
 // scheduling.
 //
-// Measured, out of place, 8 heads of width 128: 32 caches of 2304 slots to 2048
-// in 95 us (5.7 TB/s: bound by the copy); one cache of 32768 to 8192 in 35 us,
-// two thirds of it the selection, whose dozen cluster-wide steps of 1 to 2 us
-// each bound it; two caches of 320 to 256 in 6.3 us, two launches.  Adding the
-// histograms up in slices, one per CTA, instead of all by each CTA: no gain.
+// Measured, 8 heads of width 128, out of place: 32 caches of 2304 slots to 2048
+// in 95 us (5.7 TB/s: bound by the copy), of 1051 to 2304 slots in 80; one
+// cache of 32768 to 8192 in 36 us, two thirds of it the selection, whose dozen
+// cluster-wide steps of 1 to 2 us each bound it; two caches of 320 to 256 in 6.4
+// us, two launches.  In place: the same 32 caches in 41 and 37 us (58380 and 6300
+// rows move, a floor of 10 and 1.5 us: the selection, then blocks for every slot
+// of the budget that mostly find nothing to move), the others in 34 and 7.1 us.
+// Adding the histograms up in slices, one per CTA, instead of all by each CTA: no
+// gain.
 #include <algorithm>
 #include <climits>
 

@@ -24,23 +24,28 @@ namespace {
 
 using namespace sa;
 
-// How a call is cut is chosen by an estimate of its time in microseconds, with
-// constants measured on a B200 (148 SMs; 32 query and 8 KV heads of width 128
-// unless said otherwise).  The alternatives measured against one another:
+// How a call is cut is chosen by an estimate of its time in microseconds, from
+// the capacities (lengths are on the device), with constants measured on a B200
+// (148 SMs; 32 query and 8 KV heads of width 128 unless said otherwise) with
+// full caches: room beyond the lengths leads to plans for suffixes that are not
+// there (batch 32 on 8192 keys, suffixes of up to 256 in a capacity of 256 22.2,
+// of 1024 24.4, of 2048 39.3, of 4096 50.5).  The alternatives measured against
+// one another, in a graph of 18 calls at 1965 MHz:
 //
 //   few-row kernel alone / beside tiles, one token: batch 8 on 1024 + 64 keys
-//     10.9 / 13.2, batch 64 on 256 + 64 14.1 / 20; batch 2 on 8192 + 64 24.1 /
-//     19.7, batch 16 on 2048 + 64 21.1 / 14.0
+//     10.9 / 12.9, batch 64 on 256 + 64 14.0 / 13.1 (taken: alone); batch 2 on
+//     8192 + 64 23.8 / 19.2, batch 16 on 2048 + 64 21.1 / 13.8
 //   few-row kernel alone / tiles per sequence: one sequence of 88 tokens, 8
-//     query heads, on 291 + 91 keys 9.4 / 13.8; 2 of 33 on 1000 + 64 23.2 / 17.1
+//     query heads, on 291 + 91 keys 10.7 / 13.6; 2 of 33 on 1000 + 64 23.5 / 17.1
 //   few rows beside tiles / tiles per sequence: batch 32 of one token on 8192 +
-//     256 keys 24 / 183, batch 8 of 8 tokens on 8192 + 256 27 / 56; batch 16 of
-//     8 tokens on 1024 + 128 21.4 / 18.6
+//     256 keys 27 / 178, batch 8 of 8 tokens on 8192 + 256 28 / 57; batch 16 of
+//     8 tokens on 1024 + 128 19.5 / 18.9
 //   key ranges of the pooled tiles, batch 64 of one token on 32768 + 2048 keys
-//     (16 row tiles): 2 203, 4 119, 6 119, 9 139: ranges beyond an SM's fair
-//     share of the products take the room that the suffixes stream through
-//   one / two row tiles per CTA: batch 8 of 48 tokens on 4096 + 112 keys 49.3
-//     (whole) / 57.5 (two ranges); batch 8 of 512 on 8192 + 512 662 / 638
+//     (16 row tiles), the best suffix cut of each: 2 196, 3 144, 4 117, 5 115, 6
+//     115, 9 125; suffixes of half that on average 175, 123, 97, 86, 92, 96:
+//     with more ranges fewer SMs are left for the suffixes to stream through
+//   one / two row tiles per CTA: batch 8 of 48 tokens on 4096 + 112 keys 49.0
+//     (whole) / 58.7 (two ranges); batch 8 of 512 on 8192 + 512 637 / 615
 inline int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
 // Tiles of row tiles alone (a turn, a document): sets per_cta, groups, tasks,
@@ -121,8 +126,8 @@ double plan_beside(const SharedAttnArgs& a, int key_tiles, int units, int sms, P
 // work of the busiest CTA, which takes every sms-th unit, in tiles of 128 rows
 // against a pair of key tiles (2.3 us); a unit costs half a tile besides, adding
 // the parts up one and a half.  41 sequences of 150 tokens, 2 heads per KV head,
-// on 71 keys take 200 us in one part (two CTAs take all rows past the prefix),
-// 54 in 8, 41 in 33; 8 of 48 tokens on 4096 keys 83 in one, 85 in 4, 95 in 8.
+// on 71 keys take 199 us in one part (two CTAs take all rows past the prefix),
+// 54 in 8, 41 in 33; 8 of 48 tokens on 4096 keys 81 in one, 85 in 4, 93 in 8.
 void plan_weights(const SharedAttnArgs& a, int sms, Plan* p) {
   const long long prefix = (long long)ceil_div(a.pcap, kPair) * a.kv_heads;
   const long long suffix = p->pooled ? 0 : (long long)ceil_div(a.scap, kPair) * a.kv_heads * a.batch;

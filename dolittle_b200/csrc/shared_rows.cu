@@ -21,13 +21,13 @@
 // maximum and sum.  The four warps of a CTA, then the CTAs that share a row
 // are joined in a fixed order.  Rows past the length are loaded as zeros.
 //
-// Measured: the suffixes of 64 sequences of up to 2048 keys (271 MB) alone take
-// 39 us, 6.9 TB/s; a small call (64 sequences on 512 + 64 keys, mostly from L2)
-// 21 us, 7.1 TB/s.  Two branches of 256 + 64 keys take 5.9 us, nearly all of it
-// launch, first loads and join.  A row block of 32 rows instead of two of 16 had
-// to wait for the tile kernel's shared memory: batch 8 of 8 tokens on 8192 +
-// 256 keys 63 us against 36.  A ring of four slots left room for fewer CTAs:
-// batch 32 on 8192 + 256 keys 26.4 against 22.7 us.
+// Measured: the suffixes of 64 sequences of up to 2048 keys (271 MB) by
+// themselves take 53 us, 5.1 TB/s; a small call (64 sequences on 256 + 64 keys,
+// 84 MB mostly from L2) 14.0 us, 6.0 TB/s.  Two branches of 256 + 64 keys take 6.0
+// us, nearly all of it launch, first loads and join.  A row block of 32 rows
+// instead of two of 16 had to wait for the tile kernel's shared memory: batch 8
+// of 8 tokens on 8192 + 256 keys 63 us against 36.  A ring of four slots left
+// room for fewer CTAs: batch 32 on 8192 + 256 keys 26.4 against 22.7 us.
 #include "shared_attention.cuh"
 
 #include <algorithm>

@@ -28,9 +28,10 @@
 // Q K^T (both operands from shared memory, 103 cycles per 128 x 128 x 16 where
 // the products alone are 64) and 1024 of P V, two of them 3700; measured 3960
 // to 4300 for a pair.  Eight sequences of 512 tokens on 8192 + 512 keys, 32
-// heads of 128: 625 us, 907 TFLOP/s of useful work and 1361 with the second
-// half of P.  Calls of one or two steps are bound by the start instead: 9.7 us
-// for 5 x 74 tokens on 28 + 101 keys.
+// heads of 128: 620 us with the SMs at 1965 MHz, 914 TFLOP/s of useful work and
+// 1371 with the second half of P; called in a row 714 us, 794 TFLOP/s, since the
+// power cap then holds the SMs at 1.6 GHz.  Calls of one or two steps are bound
+// by the start instead: 9.6 us for 5 x 74 tokens on 28 + 101 keys.
 #include "shared_attention.cuh"
 
 namespace dl {
@@ -59,7 +60,7 @@ struct Shape {
   // Parts in which the weights of a tile are handed over: products begin sooner
   // with four (batch 64 on 32768 keys 87.8 -> 85.4 us, turns of 48 tokens 51.4 ->
   // 49.1), but two cost less where the tensor core is busy (tails of 512 tokens
-  // 620.5 against 629).
+  // 620.5 against 629; all at 1965 MHz).
   static constexpr int parts = WIDE ? 2 : 4;
   static constexpr int stages = D == 64 ? 8 : WIDE ? 5 : 4;
   static constexpr int smem = (queries + stages) * slot + 1024;

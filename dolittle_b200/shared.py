@@ -6,7 +6,8 @@ The reference runs every continuation of a prompt (its steered and unsteered
 branches, src/experiment/run.cpp:871-929) through a plan and a cache of its
 own; here the prompt's cache is held and read once.  Every call only enqueues
 work on torch's current stream of the tensors' device; wrong types, shapes and
-strides raise ValueError, refusals of the library DolittleError.
+strides raise ValueError, refusals of the library DolittleError.  Nothing here
+is recorded for gradients.
 """
 from __future__ import annotations
 
@@ -50,7 +51,10 @@ def attention_shared(query, prefix_key, prefix_value, suffix_key, suffix_value, 
     may be None.  Returns (out [B, rows, Hq, d] bfloat16, lse [B, rows, Hq]
     float32); a row without keys gives zeros and -inf.  prefix_weights
     [Hkv, P] and suffix_weights [B, Hkv, S] (float32) are added to: the softmax
-    weight each key received from every row and query head."""
+    weight each key received from every row and query head.  The query's tokens
+    lie apart, and `out` shares no memory with them; one suffix may be expanded
+    over the batch.  The work is cut by the caches' sizes P and S, whatever the
+    lengths: a cache far larger than what it holds costs time."""
     return (_calls or _extension()).attention_shared(query, prefix_key, prefix_value, suffix_key, suffix_value,
                                                      prefix_lengths, suffix_lengths, prefix_weights, suffix_weights,
                                                      out, lse)
@@ -65,5 +69,6 @@ def cache_evict(key, value, weights, positions, lengths, budget: int, *, first: 
     first, ties to the lowest slot.  Kept slots below the new length stay in
     place, kept slots beyond it move into the vacated ones.  out = (key, value,
     weights, positions, lengths) receives the result, None evicts in place.
-    Returns the five tensors that hold it."""
+    Returns the five tensors that hold it, rows that are written apart from one
+    another."""
     return (_calls or _extension()).cache_evict(key, value, weights, positions, lengths, budget, first, recent, out)

@@ -484,7 +484,9 @@ DL_API dl_status dl_attention_decode_batched(const void* query, const void* kv, 
  * the prompt at different tokens) and its own suffix; its `rows` newest
  * suffix positions are the query rows, so row i sees suffix keys
  * j < suffix_lengths[b] - (rows - 1 - i).  A side with capacity 0 is absent
- * and its pointers are not read. */
+ * and its pointers are not read.  A suffix_sequence_stride of 0 is one suffix
+ * cache that all sequences read.  How a call is cut into work follows the
+ * capacities, not the lengths. */
 typedef struct {
   size_t batch, rows, query_heads, kv_heads, width;
   size_t query_stride, output_stride; /* between tokens; 0 = query_heads * width */
