@@ -3,6 +3,7 @@
 // src/kernels/cuda/common.cuh:57-65): unsupported dtypes and shapes are
 // rejected, never silently converted.  Exceptions become dl_status codes and
 // a thread-local message.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cstring>
@@ -897,7 +898,12 @@ bool rows_meet(bool own, long long offset, size_t caches, size_t slots, size_t o
     const wide at = (offset % row + row) % row;
     if (at >= n && at + n <= row) return false;
   }
-  for (wide c = own ? 1 : -last_cache; c <= last_cache; ++c) {
+  wide from = own ? 1 : -last_cache, to = last_cache;
+  if (step > 0) {  // only caches within reach of each other
+    from = std::max(from, (-one - offset) / step - 1);
+    to = std::min(to, (one - offset) / step + 1);
+  }
+  for (wide c = from; c <= to; ++c) {
     const wide d = offset + c * step, near = -d / row;  // the slots nearest to meeting are `near` or one off
     for (wide s = near - 1; s <= near + 1; ++s)
       if (s >= -last_slot && s <= last_slot && d + s * row < n && -(d + s * row) < n) return true;
