@@ -30,12 +30,13 @@ def torch_calls_path() -> str:
     build of torch: it reads torch's objects by their C++ layout, so another
     build's module is another file and never loaded.  Does not import torch."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise ImportError("dolittle_b200.shared needs torch")
-    root = os.path.dirname(spec.origin)
-    with open(os.path.join(root, "version.py"), "rb") as f:  # version, source revision, CUDA
-        build = hashlib.sha256(f.read())
-    build.update(str(os.path.getsize(os.path.join(root, "lib", "libtorch_python.so"))).encode())
+    try:
+        root = os.path.dirname(spec.origin)
+        with open(os.path.join(root, "version.py"), "rb") as f:  # version, source revision, CUDA
+            build = hashlib.sha256(f.read())
+        build.update(str(os.path.getsize(os.path.join(root, "lib", "libtorch_python.so"))).encode())
+    except (AttributeError, TypeError, OSError) as e:  # no torch, a folder of that name, a part of it
+        raise ImportError("dolittle_b200.shared needs torch") from e
     return os.path.join(HERE, f"_torch_shared.{sysconfig.get_config_var('SOABI')}.{build.hexdigest()[:12]}.so")
 
 

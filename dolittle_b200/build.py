@@ -14,7 +14,6 @@ from __future__ import annotations
 import concurrent.futures as cf
 import importlib.util
 import os
-import re
 import shutil
 import subprocess
 import sys
@@ -60,13 +59,15 @@ def build_torch_calls(force: bool = False):
     and shared.py says what is missing."""
     header = os.path.join(ROOT, "include", "dolittle_b200.h")
     cxx, python = os.environ.get("CXX", "g++"), sysconfig.get_paths()["include"]
-    spec = importlib.util.find_spec("torch")
-    root = os.path.dirname(spec.origin) if spec else ""
-    out = torch_calls_path() if spec else ""
+    try:
+        out = torch_calls_path()
+        root = os.path.dirname(importlib.util.find_spec("torch").origin)
+    except ImportError:
+        out = root = ""
     if out and not force and not _stale(out, [TORCH_SRC, header]):
         return out
     missing = [what for what, there in (
-        ("torch", spec),
+        ("torch", out),
         ("torch's headers", os.path.exists(os.path.join(root, "include", "ATen", "ATen.h"))),
         ("torch's CUDA library", os.path.exists(os.path.join(root, "lib", "libc10_cuda.so"))),
         ("Python's headers", os.path.exists(os.path.join(python, "Python.h"))),
@@ -84,9 +85,6 @@ def build_torch_calls(force: bool = False):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("torch calls failed to build:\n" + r.stdout + r.stderr)
-    for f in os.listdir(os.path.dirname(out)):  # of another torch or Python
-        if re.fullmatch(r"_torch_shared(\..*)?\.so", f) and f != os.path.basename(out):
-            os.remove(os.path.join(os.path.dirname(out), f))
     return out
 
 
